@@ -18,9 +18,10 @@ LIB_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIB_DIR, "liblaya_b200.so")
 OBJ_DIR = os.path.join(ROOT, "_build", "obj")
 
-SOURCES = ["gemm.cu", "attn_tc.cu", "attn_short.cu", "rownorm.cu", "tail.cu", "tail_static.cu", "engine.cpp",
+SOURCES = ["gemm.cu", "attn_tc.cu", "attn_short.cu", "rownorm.cu", "tail.cu", "tail_static.cu", "rope.cu", "lora.cu",
+           "engine.cpp",
            "gguf_reader.cpp", "json.cpp", "frontend.cpp", "serve.cpp"]
-HEADERS = ["common.cuh", "kernels.h", "gguf_reader.h", "json.h", "unicode_tables.h"]
+HEADERS = ["common.cuh", "kernels.h", "ops_common.h", "rope.h", "lora.h", "gguf_reader.h", "json.h", "unicode_tables.h"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
@@ -38,7 +39,8 @@ def build(verbose: bool = False, force: bool = False) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)
     hdrs = [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(ROOT, "include", h)
-                                                       for h in ("laya_b200.h", "laya_frontend.h", "laya_serve.h")]
+                                                       for h in ("laya_b200.h", "laya_frontend.h", "laya_serve.h",
+                                                                 "laya_ops.h")]
     objs = []
     for src in SOURCES:
         s = os.path.join(CSRC, src)

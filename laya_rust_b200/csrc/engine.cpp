@@ -32,6 +32,8 @@
 #include "../../include/laya_b200.h"
 #include "gguf_reader.h"
 #include "kernels.h"
+#include "ops_common.h"
+#include "rope.h"
 
 namespace laya {
 
@@ -72,6 +74,9 @@ int guard(F&& f) {
     g_err.clear();
     return LAYA_OK;
   } catch (const Error& e) {
+    g_err = e.what();
+    return e.code;
+  } catch (const OpError& e) {
     g_err = e.what();
     return e.code;
   } catch (const std::bad_alloc&) {
@@ -537,6 +542,9 @@ struct Engine {
   // rope tables [rope_len][32] for the full (global) and sliding frequencies
   DevBuf cos_full, sin_full, cos_slide, sin_slide;
   int rope_len = 0;
+  // stretched frequencies (laya_set_rope_scaling): [0] full, [1] sliding
+  bool rope_scaled[2] = {false, false};
+  laya_rope_scaling rope_scaling[2] = {};
 
   // arena
   int cap_rows = 0, cap_mk = 0, cap_n = 0;
@@ -791,7 +799,36 @@ struct Engine {
     upload_sync(sin_full.p, sf.data(), sf.size() * 4, "rope upload");
     upload_sync(cos_slide.p, cs.data(), cs.size() * 4, "rope upload");
     upload_sync(sin_slide.p, ss.data(), ss.size() * 4, "rope upload");
+    if (rope_scaled[0]) fill_scaled(ff, rope_scaling[0], n, cos_full, sin_full);
+    if (rope_scaled[1]) fill_scaled(fs, rope_scaling[1], n, cos_slide, sin_slide);
     rope_len = n;
+  }
+
+  // cos/sin tables of n positions from the model's frequencies `f` stretched
+  // by `sc`, on the engine's stream.
+  void fill_scaled(const std::vector<float>& f, const laya_rope_scaling& sc, int n, const DevBuf& c, const DevBuf& s) {
+    std::vector<double> d(f.begin(), f.end());
+    const float m = rope_stretch(d.data(), HD, &sc);
+    ck(launch_rope_table(d.data(), HD / 2, m, n, c.as<float>(), s.as<float>(), stream), "rope table");
+  }
+
+  void set_rope_scaling(const laya_rope_scaling* full, const laya_rope_scaling* sliding) {
+    if (!finalized) throw Error(LAYA_E_STATE, "engine has no weights (call laya_finalize)");
+    const laya_rope_scaling* in[2] = {full, sliding};
+    for (const laya_rope_scaling* s : in) {
+      std::vector<double> probe(HD / 2, 1.0);
+      rope_stretch(probe.data(), HD, s);  // refuses bad parameters before anything changes
+    }
+    set_device();
+    ck(cudaStreamSynchronize(stream), "sync");
+    ck(cudaStreamSynchronize(side), "sync");
+    for (int i = 0; i < 2; ++i) {
+      rope_scaled[i] = in[i] != nullptr;
+      if (in[i]) rope_scaling[i] = *in[i];
+    }
+    const int len = std::max(rope_len, 512);
+    rope_len = 0;
+    ensure_rope(len);
   }
 
   // ---- arena ----------------------------------------------------------------------
@@ -1751,6 +1788,13 @@ int laya_plan_layout(const laya_req* req, int64_t* rows, int64_t* ntiles, int32_
         items[4 * i + 3] = p.items[i].w;
       }
     }
+  });
+}
+
+int laya_set_rope_scaling(laya_engine* e, const laya_rope_scaling* full, const laya_rope_scaling* sliding) {
+  return guard([&] {
+    if (!e) throw Error(LAYA_E_INVALID, "null engine");
+    e->e->set_rope_scaling(full, sliding);
   });
 }
 

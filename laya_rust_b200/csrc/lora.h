@@ -1,0 +1,75 @@
+// Low-rank adapters beside a shared projection: the host plan of a batch and
+// the device kernels' launchers.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <vector>
+
+namespace laya {
+
+// An adapter's rank is cut into chunks of 16 columns (one K step of an f16
+// MMA, 32 bytes a row), the last one filled up with zeros.  In a bank, chunk c
+// of slot s is chunk s * chunks_per_slot + c of
+//   A [chunk][16][in_pad]   (in_pad: in rounded up to 64)
+//   B [chunk][out_pad][16]  (out_pad: out rounded up to 256)
+constexpr int kLoraChunk = 16;
+// Rows of a block: the GEMM's row tile.
+constexpr int kLoraBlock = 256;
+
+inline int lora_chunks(int rank) { return (rank + kLoraChunk - 1) / kLoraChunk; }
+
+// The adapters each block of 256 rows needs.  Entry e in [off[b], off[b + 1])
+// is one chunk of one adapter that some row of block b has; a slot's chunks
+// are consecutive entries, slots in order of first use.  row_entry[m]: the
+// first entry of row m's adapter, or -1.  u, the rank-space vectors, is
+// [entries][256 rows][16 values | 16 remainders] in the 16-bit type, zero for
+// rows of other adapters.
+struct LoraLayout {
+  int rows = 0;
+  std::vector<int> off;
+  std::vector<int2> chunk;      // (slot, chunk of the slot)
+  std::vector<int> row_entry;   // [rows]
+};
+// Throws OpError; chunks_of(slot) is the slot's chunk count, 0 if it is empty.
+LoraLayout lora_layout(const int32_t* rows, const int32_t* slot, int n, const std::vector<int>& chunks_of);
+
+constexpr size_t kLoraEntryElems = static_cast<size_t>(kLoraBlock) * 2 * kLoraChunk;
+
+struct LoraShrinkArgs {
+  const void* x;          // [rows, in], pitch ldx
+  long long ldx;
+  const void* a;          // the bank's A
+  const int* row_entry;   // [rows]
+  const int* entry_chunk; // [entries]: chunk in the bank
+  const float* scale;     // per slot
+  void* u;
+  int rows, in, in_pad;
+  int chunks_per_slot;
+  const int* nchunks;     // [slots]
+  bool bf16;
+};
+// u entries of every row with an adapter: scale * (x A^T) as value + remainder.
+cudaError_t launch_lora_shrink(const LoraShrinkArgs& a, cudaStream_t s);
+
+struct LoraExpandArgs {
+  const void* x;
+  long long ldx;
+  const void* w;          // [out, in], pitch ldw
+  long long ldw;
+  const float* bias;      // [out] or nullptr
+  const void* b;          // the bank's B
+  const int* row_entry;
+  const int* entry_chunk;
+  const int* nchunks;
+  const void* u;
+  void* y;
+  long long ldy;
+  int rows, in, out, out_pad;
+  int chunks_per_slot;
+  bool bf16;
+};
+cudaError_t launch_lora_expand_simple(const LoraExpandArgs& a, cudaStream_t s);
+
+}  // namespace laya

@@ -1,0 +1,283 @@
+// Rotary positions on [tokens, heads, dim] views (laya_rope) and the cos/sin
+// tables of stretched frequencies the engine's Wqkv epilogue reads.
+//
+// A pair (a, b) of a head turns by the angle p f_j: (a c - b s, b c + a s).
+// Angles: p f_j needs more than 32 bits once p is large (at p = 2^20 an f32
+// product is off by up to 0.06 radian), so a frequency is kept as a 64-bit
+// fixed-point fraction of a turn per position.  The integer product p F drops
+// whole turns by itself (mod 2^64), is off by at most |p| 2^-65 of a turn from
+// F's rounding, and its top 32 bits (rounded) are the angle to 2^-33 of a turn.  Those
+// split into the nearest quadrant and a remainder of at most 1/8 turn, exact
+// as an integer, so the f32 sine and cosine see a reduced argument whose
+// conversion rounds relative to itself.
+//
+// Simple form: one thread per (token, head, pair or copied element).
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "common.cuh"
+#include "ops_common.h"
+#include "rope.h"
+
+#include <cuda_bf16.h>
+
+namespace laya {
+
+namespace {
+
+constexpr int kMaxPairs = LAYA_ROPE_MAX_DIM / 2;
+constexpr int kMaxTensors = 4;
+
+struct RopeTensorArg {
+  const void* x;
+  void* out;
+  long long x_token, x_head, out_token, out_head;
+  int heads;
+};
+
+struct RopeArgs {
+  RopeTensorArg t[kMaxTensors];
+  int count;
+  int dim, rot;
+  long long tokens;
+  const int* pos;
+  long long pos0;
+  float mscale, sign;
+  uint64_t turns[kMaxPairs];
+};
+
+// (cos, sin) of position p times the fixed-point frequency `turns`.
+__device__ __forceinline__ void rope_angle(uint64_t turns, long long p, float& c, float& s) {
+  const uint64_t t = turns * static_cast<uint64_t>(p);
+  const uint32_t v = static_cast<uint32_t>((t + 0x80000000ull) >> 32);  // angle in 2^-32 turns
+  const uint32_t quad = (v + 0x20000000u) >> 30;
+  const float r = static_cast<float>(static_cast<int32_t>(v - (quad << 30))) * 4.656612873077393e-10f;  // 2^-31: half turns
+  float rs, rc;
+  sincospif(r, &rs, &rc);
+  // angle = quad quarter turns + r
+  const float a = (quad & 1u) ? rs : rc, b = (quad & 1u) ? rc : rs;
+  c = (quad == 1u || quad == 2u) ? -a : a;
+  s = (quad & 2u) ? -b : b;
+}
+
+template <class T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+
+template <class T, bool HALF>
+__global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeArgs a) {
+  const int half = a.rot / 2, copied = a.dim - a.rot, units = half + copied;
+  const RopeTensorArg& t = a.t[blockIdx.z];
+  const long long n = a.tokens * t.heads * units;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
+       i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const int u = static_cast<int>(i % units);
+    const long long th = i / units;
+    const int h = static_cast<int>(th % t.heads);
+    const long long tok = th / t.heads;
+    const T* x = static_cast<const T*>(t.x) + tok * t.x_token + h * t.x_head;
+    T* o = static_cast<T*>(t.out) + tok * t.out_token + h * t.out_head;
+    if (u >= half) {
+      o[a.rot + u - half] = x[a.rot + u - half];
+      continue;
+    }
+    float c, s;
+    rope_angle(a.turns[u], a.pos ? a.pos[tok] : a.pos0 + tok, c, s);
+    c *= a.mscale;
+    s *= a.mscale * a.sign;
+    const int i0 = HALF ? u : 2 * u, i1 = HALF ? u + half : 2 * u + 1;
+    const float v0 = to_f32(x[i0]), v1 = to_f32(x[i1]);
+    o[i0] = from_f32<T>(v0 * c - v1 * s);
+    o[i1] = from_f32<T>(v1 * c + v0 * s);
+  }
+}
+
+struct TableArgs {
+  uint64_t turns[32];
+  int n, positions;
+  float mscale;
+  float* cosb;
+  float* sinb;
+};
+
+__global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__ TableArgs a) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.positions * a.n) return;
+  float c, s;
+  rope_angle(a.turns[i % a.n], i / a.n, c, s);
+  a.cosb[i] = a.mscale * c;
+  a.sinb[i] = a.mscale * s;
+}
+
+template <class T>
+cudaError_t launch_rope(const RopeArgs& a, bool half, cudaStream_t st) {
+  long long n = 0;
+  for (int i = 0; i < a.count; ++i)
+    n = std::max(n, a.tokens * a.t[i].heads * (a.rot / 2 + a.dim - a.rot));
+  if (n == 0) return cudaSuccess;
+  const dim3 grid(static_cast<unsigned>(std::min<long long>((n + 255) / 256, 1 << 20)), 1, a.count);
+  if (half)
+    rope_kernel<T, true><<<grid, 256, 0, st>>>(a);
+  else
+    rope_kernel<T, false><<<grid, 256, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+bool finite_positive(double v) { return std::isfinite(v) && v > 0; }
+
+}  // namespace
+
+float rope_stretch(double* f, int rot, const laya_rope_scaling* s) {
+  if (!s) return 1.0f;
+  op_require(std::isfinite(s->attn) && s->attn >= 0, "rope scaling: attn must not be negative");
+  if (s->kind == LAYA_ROPE_NONE) return s->attn != 0 ? static_cast<float>(s->attn) : 1.0f;
+  op_require(s->kind == LAYA_ROPE_LINEAR || s->kind == LAYA_ROPE_BASE || s->kind == LAYA_ROPE_PARTS,
+             "rope scaling: unknown kind");
+  op_require(std::isfinite(s->factor) && s->factor >= 1, "rope scaling: factor must be at least 1");
+  const int n = rot / 2;
+  double m = 1.0;
+  if (s->kind == LAYA_ROPE_LINEAR) {
+    for (int j = 0; j < n; ++j) f[j] /= s->factor;
+  } else if (s->kind == LAYA_ROPE_BASE) {
+    op_require(rot > 2, "rope scaling: LAYA_ROPE_BASE needs rot > 2");
+    for (int j = 0; j < n; ++j) f[j] *= std::pow(s->factor, -2.0 * j / (rot - 2));
+  } else {
+    op_require(finite_positive(s->trained_len) && std::isfinite(s->low) && std::isfinite(s->high) && s->low < s->high,
+               "rope scaling: LAYA_ROPE_PARTS needs trained_len > 0 and low < high");
+    for (int j = 0; j < n; ++j) {
+      const double turns = s->trained_len * f[j] / (2.0 * M_PI);
+      const double g = std::min(1.0, std::max(0.0, (turns - s->low) / (s->high - s->low)));
+      f[j] *= g + (1.0 - g) / s->factor;
+    }
+    m = 0.1 * std::log(s->factor) + 1.0;
+  }
+  return static_cast<float>(s->attn != 0 ? s->attn : m);
+}
+
+uint64_t rope_turns(double f) {
+  // 2 pi to the 64 bits of a long double
+  const long double two_pi = 6.283185307179586476925286766559L;
+  long double t = static_cast<long double>(f) / two_pi;
+  t -= floorl(t);
+  t = roundl(t * 18446744073709551616.0L);
+  return t >= 18446744073709551616.0L ? 0ull : static_cast<uint64_t>(t);
+}
+
+cudaError_t launch_rope_table(const double* freqs, int n, float mscale, int positions, float* cosb, float* sinb,
+                              cudaStream_t s) {
+  if (n < 1 || n > 32 || positions < 0) return cudaErrorInvalidValue;
+  if (positions == 0) return cudaSuccess;
+  TableArgs a{};
+  for (int j = 0; j < n; ++j) a.turns[j] = rope_turns(freqs[j]);
+  a.n = n;
+  a.positions = positions;
+  a.mscale = mscale;
+  a.cosb = cosb;
+  a.sinb = sinb;
+  rope_table_kernel<<<(positions * n + 255) / 256, 256, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace laya
+
+using namespace laya;
+
+extern "C" int laya_rope_freqs(double base, int rot, const laya_rope_scaling* s, double* freqs, float* mscale) {
+  return op_guard([&] {
+    op_require(freqs && mscale, "rope_freqs: null argument");
+    op_require(std::isfinite(base) && base > 0, "rope_freqs: base must be positive");
+    op_require(rot >= 2 && rot <= LAYA_ROPE_MAX_DIM && rot % 2 == 0, "rope_freqs: rot must be even, 2..LAYA_ROPE_MAX_DIM");
+    std::vector<double> f(rot / 2);
+    for (int j = 0; j < rot / 2; ++j) f[j] = std::pow(base, -2.0 * j / rot);
+    *mscale = rope_stretch(f.data(), rot, s);
+    std::copy(f.begin(), f.end(), freqs);
+  });
+}
+
+extern "C" int laya_rope(int device, const laya_rope_spec* spec, const laya_rope_tensor* tensors, int count,
+                         int64_t tokens, const int32_t* pos, int64_t pos0, void* stream) {
+  return op_guard([&] {
+    op_require(spec && tensors && spec->freqs, "rope: null argument");
+    op_require(spec->type == LAYA_F16 || spec->type == LAYA_BF16 || spec->type == LAYA_F32, "rope: unknown type");
+    op_require(spec->layout == LAYA_ROPE_HALF || spec->layout == LAYA_ROPE_INTERLEAVED, "rope: unknown layout");
+    op_require(spec->dim >= 2 && spec->dim <= LAYA_ROPE_MAX_DIM, "rope: dim must be 2..LAYA_ROPE_MAX_DIM");
+    op_require(spec->rot >= 2 && spec->rot <= spec->dim && spec->rot % 2 == 0, "rope: rot must be even, 2..dim");
+    op_require(std::isfinite(spec->mscale), "rope: mscale is not finite");
+    op_require(count >= 1 && count <= kMaxTensors, "rope: 1 to 4 tensors");
+    constexpr int64_t kMaxPos = 2147483647;
+    op_require(tokens >= 0 && tokens <= kMaxPos, "rope: tokens out of range");
+    op_require(pos || (pos0 >= -kMaxPos && pos0 + tokens <= kMaxPos + 1 && pos0 <= kMaxPos),
+               "rope: positions must fit 32 bits");
+    RopeArgs a{};
+    const size_t es = spec->type == LAYA_F32 ? 4 : 2;
+    for (int i = 0; i < count; ++i) {
+      const laya_rope_tensor& t = tensors[i];
+      op_require(t.heads >= 0 && t.heads <= 65535, "rope: heads must be 0..65535");
+      if (t.heads == 0 || tokens == 0) continue;
+      op_require(t.x && t.out, "rope: null tensor");
+      op_require(reinterpret_cast<uintptr_t>(t.x) % es == 0 && reinterpret_cast<uintptr_t>(t.out) % es == 0,
+                 "rope: address not aligned to its elements");
+      op_require(t.x_token >= 0 && t.x_head >= 0 && t.out_token >= 0 && t.out_head >= 0, "rope: negative stride");
+      constexpr int64_t kMaxStride = int64_t{1} << 40;
+      op_require(t.x_token <= kMaxStride && t.x_head <= kMaxStride && t.out_token <= kMaxStride && t.out_head <= kMaxStride,
+                 "rope: stride too large");
+      // distinct output elements: the smaller stride steps over a head's dims,
+      // the larger over everything the smaller one reaches
+      const int64_t sh = t.heads > 1 ? t.out_head : 0, sk = tokens > 1 ? t.out_token : 0;
+      const int64_t lo = std::min(sh, sk), hi = std::max(sh, sk), nlo = sh <= sk ? t.heads : tokens;
+      op_require(t.heads == 1 || tokens == 1
+                     ? hi >= spec->dim || (t.heads == 1 && tokens == 1)
+                     : lo >= spec->dim && hi >= static_cast<__int128>(lo) * (nlo - 1) + spec->dim,
+                 "rope: output elements overlap");
+      if (t.x == t.out)
+        op_require((t.x_token == t.out_token || tokens == 1) && (t.x_head == t.out_head || t.heads == 1),
+                   "rope: in place needs equal strides");
+      RopeTensorArg& r = a.t[a.count++];
+      r.x = t.x;
+      r.out = t.out;
+      r.x_token = t.x_token;
+      r.x_head = t.x_head;
+      r.out_token = t.out_token;
+      r.out_head = t.out_head;
+      r.heads = static_cast<int>(t.heads);
+    }
+    for (int j = 0; j < spec->rot / 2; ++j) {
+      op_require(std::isfinite(spec->freqs[j]), "rope: a frequency is not finite");
+      a.turns[j] = rope_turns(spec->freqs[j]);
+    }
+    if (a.count == 0) return;
+    DeviceScope scope(device);
+    for (int i = 0; i < a.count; ++i) {
+      require_device_ptr(a.t[i].x, device, "rope: x");
+      require_device_ptr(a.t[i].out, device, "rope: out");
+    }
+    if (pos) require_device_ptr(pos, device, "rope: pos");
+    a.dim = spec->dim;
+    a.rot = spec->rot;
+    a.tokens = tokens;
+    a.pos = pos;
+    a.pos0 = pos0;
+    a.mscale = spec->mscale;
+    a.sign = spec->inverse ? -1.0f : 1.0f;
+    const bool half = spec->layout == LAYA_ROPE_HALF;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e = spec->type == LAYA_F16    ? launch_rope<__half>(a, half, st)
+                    : spec->type == LAYA_BF16 ? launch_rope<__nv_bfloat16>(a, half, st)
+                                              : launch_rope<float>(a, half, st);
+    op_check(e, "rope launch");
+  });
+}
