@@ -246,6 +246,18 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
   return d;
 }
 
+// The same for rows of 16 values (32 bytes, one K step) with 32-byte swizzle:
+// 8-row atoms 256 B apart, layout type SWIZZLE_32B = 6.
+__device__ __forceinline__ uint64_t umma_desc_sw32(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(1u) << 16;
+  d |= static_cast<uint64_t>(256u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(6u) << 61;
+  return d;
+}
+
 // Instruction descriptor for kind::f16: D = F32, A = B = F16, both K-major.
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
   return (1u << 4)                                   // D format F32
@@ -253,6 +265,11 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
          | (0u << 15) | (0u << 16)                   // A, B K-major
          | (static_cast<uint32_t>(n >> 3) << 17)     // N / 8
          | (static_cast<uint32_t>(m >> 4) << 24);    // M / 16
+}
+
+// The same with A = B = BF16.
+__host__ __device__ constexpr uint32_t umma_idesc_bf16(int m, int n) {
+  return umma_idesc_f16(m, n) | (1u << 7) | (1u << 10);
 }
 
 // 2^x by the hardware's approximate exponential (one MUFU op).

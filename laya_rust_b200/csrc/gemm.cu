@@ -29,11 +29,22 @@
 // tiles leave the last wave mostly idle), the tiles of whole waves add into
 // the residual stream and the tiles of the last row blocks are split into K
 // parts the same way, so the last wave is short.
+// With EXT (rows that have low-rank adapters), a tile's K loop goes on over the
+// adapters its row block needs: entry e multiplies 16 columns of rank-space
+// vectors u (zero in rows of other adapters) with 16 columns of that adapter's
+// B.  A stage then holds two entries, each u's values and remainders (two
+// 128-row operands of 32 bytes a row, 32-byte swizzle) against one B operand:
+// four K = 16 MMAs, as many as a stage of the K loop.  So adapters cost a tile
+// entries / 2 more k-blocks and no pass of their own over the output.
 // No TMA load in this kernel uses multicast; every CTA loads its own operand
 // halves.  The MMA completion signal is delivered to both CTAs of the pair
 // with tcgen05.commit's cluster-multicast form.
 #include <cstdio>
 #include <cstdlib>
+
+#include <cuda_bf16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -59,6 +70,10 @@ constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int STAGING_BYTES = 4096;    // 32 rows x 128 B
 constexpr int BAR_BYTES = 256;
 constexpr size_t SMEM_LIMIT = 232448;
+// EXT: one adapter operand of a CTA's rows, 16 columns (32 bytes) a row; a
+// stage takes two entries of two such operands
+constexpr int EXT_A_BYTES = CTA_ROWS * 32;
+static_assert(4 * EXT_A_BYTES == CTA_ROWS * BK * 2, "two entries fill a stage's A operand");
 
 template <int BN>
 struct Cfg {
@@ -74,6 +89,11 @@ struct Cfg {
 };
 
 __device__ __forceinline__ float u2f(uint32_t v) { return __uint_as_float(v); }
+
+__device__ __forceinline__ uint32_t pack_bf162(float a, float b) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   __half2 h = __floats2half2_rn(a, b);
@@ -390,6 +410,50 @@ __device__ __forceinline__ void epilogue_tile(const GemmArgs& a, const CUtensorM
       stage_row(s, r, w);
       st.store(tmOut, oc0 + c0, row0, false);
     }
+  } else if constexpr (EPI == kEpiPlainF16 || EPI == kEpiPlainBf16) {
+#pragma unroll 1
+    for (int c0 = cb; c0 < ce; c0 += 64) {
+      if (n0 + c0 >= a.n_valid) break;
+      uint32_t v0[32], v1[32];
+      tmem_ld_32x32b_x32(t_row + c0, v0);
+      tmem_ld_32x32b_x32(t_row + c0 + 32, v1);
+      tmem_ld_wait();
+      if (a.bias) {
+        const float* b = a.bias + n0 + c0;
+        const int left = a.n_valid - n0 - c0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          v0[j] = __float_as_uint(u2f(v0[j]) + (j < left ? __ldg(b + j) : 0.0f));
+          v1[j] = __float_as_uint(u2f(v1[j]) + (32 + j < left ? __ldg(b + 32 + j) : 0.0f));
+        }
+      }
+      uint32_t w[32];
+#pragma unroll
+      for (int j = 0; j < 32; j += 2) {
+        if constexpr (EPI == kEpiPlainBf16) {
+          w[j / 2] = pack_bf162(u2f(v0[j]), u2f(v0[j + 1]));
+          w[16 + j / 2] = pack_bf162(u2f(v1[j]), u2f(v1[j + 1]));
+        } else {
+          w[j / 2] = pack_half2(u2f(v0[j]), u2f(v0[j + 1]));
+          w[16 + j / 2] = pack_half2(u2f(v1[j]), u2f(v1[j + 1]));
+        }
+      }
+      uint8_t* s = st.acquire();
+      stage_row(s, r, w);
+      // The output map ends at the last whole 16 bytes of a row: a TMA store
+      // writes whole 16-byte pieces, so with n_valid % 8 columns left it would
+      // reach past them (measured: it writes zeros there).  Each lane stores
+      // those columns of its row itself.
+      const int whole = a.n_valid & ~7;
+      if (n0 + c0 < whole) st.store(tmOut, n0 + c0, row0, false);
+      if (whole < a.n_valid && whole >= n0 + c0 && whole < n0 + c0 + 64 && valid) {
+        const int piece = (whole - n0 - c0) >> 3;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(s + r * 128 + ((piece ^ (r & 7)) << 4));
+        uint16_t* dst = static_cast<uint16_t*>(a.out) + static_cast<size_t>(row) * a.ldo + whole;
+        for (int j = 0; j < a.n_valid - whole; ++j) dst[j] = src[j];
+      }
+      __syncwarp();
+    }
   } else {  // kEpiScorer
     float s = 0.0f;
 #pragma unroll 1
@@ -414,11 +478,21 @@ __device__ __forceinline__ void epilogue_tile(const GemmArgs& a, const CUtensorM
   }
 }
 
-template <int EPI, int BN>
+// The EXT kernels' further parameters (nothing for the others).
+struct ExtParams {
+  CUtensorMap u, b;
+  const int* off;
+  const int* chunk;
+  int b_rows;
+};
+struct NoExt {};
+
+template <int EPI, int BN, bool EXT>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmOut2,
-                   const GemmArgs args) {
+                   const GemmArgs args,
+                   const __grid_constant__ std::conditional_t<EXT, ExtParams, NoExt> ext) {
   using C = Cfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -521,6 +595,34 @@ __global__ void __launch_bounds__(THREADS, 1)
             phase ^= 1u;
           }
         }
+        if constexpr (EXT) {
+          // the adapters of the row block, two entries a stage
+          if (!ok || w.kb1 != num_kb) continue;
+          const int mb = w.tile / num_n;
+          const int e1 = __ldg(ext.off + mb + 1);
+          for (int e = __ldg(ext.off + mb); e < e1; e += 2) {
+            const int n = min(2, e1 - e);
+            const int chunk[2] = {__ldg(ext.chunk + e), n > 1 ? __ldg(ext.chunk + e + 1) : 0};
+            if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, args.err, kErrGemmProducerWait, abort_flag,
+                                   args.wait_limit_ns)) {
+              ok = false;
+              break;
+            }
+            const uint32_t fb = map_to_rank(smem_u32(&full[stage]), 0);
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * n * (2 * EXT_A_BYTES + BN / 2 * 32));
+            for (int i = 0; i < n; ++i) {
+              uint8_t* sa = sA + stage * C::A_BYTES + i * 2 * EXT_A_BYTES;
+              const int y = (e + i) * BM + static_cast<int>(rank) * CTA_ROWS;
+              tma_load_2d_pair(sa, &ext.u, 0, y, fb);
+              tma_load_2d_pair(sa + EXT_A_BYTES, &ext.u, 16, y, fb);
+              tma_load_2d_pair(sB + stage * C::B_BYTES + i * (BN / 2 * 32), &ext.b, 0, chunk[i] * ext.b_rows + n0, fb);
+            }
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
       }
       if (!ok || *abort_flag) {
         // give loads already in flight time to land before teardown (also
@@ -531,7 +633,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp == 1) {
     if (leader && lane == 0) {
-      const uint32_t idesc = umma_idesc_f16(BM, BN);
+      const uint32_t idesc = EPI == kEpiPlainBf16 ? umma_idesc_bf16(BM, BN) : umma_idesc_f16(BM, BN);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -565,6 +667,33 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
         if (!ok) break;
+        if constexpr (EXT) {
+          if (kb1 == num_kb) {
+            const int mb = w.tile / num_n;
+            const int e1 = __ldg(ext.off + mb + 1);
+            for (int e = __ldg(ext.off + mb); e < e1; e += 2) {
+              if (!mbar_wait_bounded(&full[stage], phase, args.err, kErrGemmMmaWait, abort_flag, args.wait_limit_ns)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint32_t a_addr = smem_u32(sA + stage * C::A_BYTES);
+              const uint32_t b_addr = smem_u32(sB + stage * C::B_BYTES);
+              for (int i = 0; i < min(2, e1 - e); ++i) {
+                const uint64_t db = umma_desc_sw32(b_addr + i * (BN / 2 * 32));
+                const uint32_t sa = a_addr + i * 2 * EXT_A_BYTES;
+                umma2_f16(d_tmem, umma_desc_sw32(sa), db, idesc, 1u);
+                umma2_f16(d_tmem, umma_desc_sw32(sa + EXT_A_BYTES), db, idesc, 1u);
+              }
+              umma2_commit_both(&empty[stage]);
+              if (++stage == C::STAGES) {
+                stage = 0;
+                phase ^= 1u;
+              }
+            }
+            if (!ok) break;
+          }
+        }
         umma2_commit_both(&tfull[acc]);
         acc ^= 1;
         if (acc == 0) aphase ^= 1u;
@@ -626,15 +755,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-template <int EPI, int BN>
-cudaError_t launch_one(const GemmMaps& m, const GemmArgs& args, int num_sms, cudaStream_t stream) {
+template <int EPI, int BN, bool EXT>
+cudaError_t launch_one(const GemmMaps& m, const GemmArgs& args, int num_sms, cudaStream_t stream,
+                       const std::conditional_t<EXT, ExtParams, NoExt>& ext) {
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(gemm_tc_kernel<EPI, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(gemm_tc_kernel<EPI, BN, EXT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(Cfg<BN>::SMEM));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
@@ -651,14 +781,19 @@ cudaError_t launch_one(const GemmMaps& m, const GemmArgs& args, int num_sms, cud
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  return launch_pdl(gemm_tc_kernel<EPI, BN>, dim3(2 * clusters, 1, 1), dim3(THREADS, 1, 1), Cfg<BN>::SMEM, stream,
-                    attr, 1, *m.a, *m.b, *m.out, m.out2 ? *m.out2 : *m.out, args);
+  return launch_pdl(gemm_tc_kernel<EPI, BN, EXT>, dim3(2 * clusters, 1, 1), dim3(THREADS, 1, 1), Cfg<BN>::SMEM, stream,
+                    attr, 1, *m.a, *m.b, *m.out, m.out2 ? *m.out2 : *m.out, args, ext);
+}
+
+template <int EPI, int BN>
+cudaError_t launch_one(const GemmMaps& m, const GemmArgs& args, int num_sms, cudaStream_t stream) {
+  return launch_one<EPI, BN, false>(m, args, num_sms, stream, NoExt{});
 }
 
 }  // namespace
 
 cudaError_t launch_gemm(int epilogue, const GemmMaps& m, const GemmArgs& args, int num_sms, cudaStream_t stream,
-                        int bn) {
+                        int bn, const GemmExt* ext) {
   if (bn != kGemmBN && bn != kGemmBNNarrow) return cudaErrorInvalidValue;
   if (args.N % bn || args.K % BK || args.M < 0 || !m.a || !m.b || !m.out) return cudaErrorInvalidValue;
   if (epilogue == kEpiPartial &&
@@ -674,6 +809,29 @@ cudaError_t launch_gemm(int epilogue, const GemmMaps& m, const GemmArgs& args, i
         args.tail_row0 != (args.main_tiles / num_n) * BM || args.split_rows % BM ||
         args.split_rows < ((args.M - args.tail_row0 + BM - 1) / BM) * BM)
       return cudaErrorInvalidValue;
+  }
+  if (ext) {
+    if (!ext->u || !ext->b || !ext->off || !ext->chunk || ext->b_rows < args.N) return cudaErrorInvalidValue;
+    const ExtParams x{*ext->u, *ext->b, ext->off, ext->chunk, ext->b_rows};
+    if (bn == kGemmBNNarrow) {
+      switch (epilogue) {
+        case kEpiQkvRope: return launch_one<kEpiQkvRope, kGemmBNNarrow, true>(m, args, num_sms, stream, x);
+        case kEpiGeglu: return launch_one<kEpiGeglu, kGemmBNNarrow, true>(m, args, num_sms, stream, x);
+        case kEpiPlainF16: return launch_one<kEpiPlainF16, kGemmBNNarrow, true>(m, args, num_sms, stream, x);
+        case kEpiPlainBf16: return launch_one<kEpiPlainBf16, kGemmBNNarrow, true>(m, args, num_sms, stream, x);
+        default: return cudaErrorInvalidValue;
+      }
+    }
+    switch (epilogue) {
+      case kEpiQkvRope: return launch_one<kEpiQkvRope, kGemmBN, true>(m, args, num_sms, stream, x);
+      case kEpiResid: return launch_one<kEpiResid, kGemmBN, true>(m, args, num_sms, stream, x);
+      case kEpiGeglu: return launch_one<kEpiGeglu, kGemmBN, true>(m, args, num_sms, stream, x);
+      case kEpiPartial: return launch_one<kEpiPartial, kGemmBN, true>(m, args, num_sms, stream, x);
+      case kEpiResidTail: return launch_one<kEpiResidTail, kGemmBN, true>(m, args, num_sms, stream, x);
+      case kEpiPlainF16: return launch_one<kEpiPlainF16, kGemmBN, true>(m, args, num_sms, stream, x);
+      case kEpiPlainBf16: return launch_one<kEpiPlainBf16, kGemmBN, true>(m, args, num_sms, stream, x);
+      default: return cudaErrorInvalidValue;
+    }
   }
   if (bn == kGemmBNNarrow) {
     // narrow 256 x 128 tiles: twice the tiles per wave, for small M where a
@@ -733,6 +891,33 @@ int make_tmap_2d(CUtensorMap* map, const void* base, bool f32, uint64_t rows, ui
                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -3;
+}
+
+namespace {
+int encode_16bit(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols, uint64_t pitch,
+                 uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return -1;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) || pitch % 8 || rows == 0 || cols == 0) return -2;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {pitch * 2};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -3;
+}
+}  // namespace
+
+int make_tmap_pitched(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols, uint64_t pitch,
+                      uint32_t box_rows) {
+  return encode_16bit(map, base, bf16, rows, cols, pitch, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int make_tmap_lora(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+  if (cols != 16 && cols != 32) return -2;
+  return encode_16bit(map, base, bf16, rows, cols, cols, 16, box_rows, CU_TENSOR_MAP_SWIZZLE_32B);
 }
 
 int make_tmap_f16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t k, uint32_t box_rows) {

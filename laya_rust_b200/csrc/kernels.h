@@ -45,6 +45,10 @@ enum GemmEpilogue : int {
   // s * split_rows + (row - tail_row0) of the second output map (the parts
   // region), for the next LayerNorm to add in part order
   kEpiResidTail = 8,
+  // 16-bit out [M, n_valid] = acc (+ bias [n_valid]): the projections of
+  // laya_lora_run, in f16 and (operands and output) bf16
+  kEpiPlainF16 = 9,
+  kEpiPlainBf16 = 10,
 };
 
 struct GemmArgs {
@@ -60,7 +64,7 @@ struct GemmArgs {
   const float* sinb;   // [max_len][32]
   float scale;         // q/k scale
   const float* wvec;   // scorer output weights [N]
-  int n_valid;         // valid output columns for kEpiGeglu
+  int n_valid;         // valid output columns for kEpiGeglu and kEpiPlain*
   int splits;          // kEpiPartial / kEpiResidTail: K parts (>= 1)
   int split_rows;      // kEpiPartial: output rows per part (multiple of 256, >= M);
                        // kEpiResidTail: the same for the tail rows (>= M - tail_row0)
@@ -79,6 +83,15 @@ int make_tmap_f16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t k,
 int make_tmap_2d(CUtensorMap* map, const void* base, bool f32, uint64_t rows, uint64_t cols,
                  uint32_t box_cols, uint32_t box_rows);
 
+// 16-bit row-major map with a row pitch (elements, a multiple of 8), box 64
+// columns (128 bytes, 128-byte swizzle) x box_rows; columns past `cols` read
+// as zero and are not stored.
+int make_tmap_pitched(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols, uint64_t pitch,
+                      uint32_t box_rows);
+// 16-bit map of rows of `cols` (16 or 32) elements, box 16 columns (32 bytes,
+// 32-byte swizzle) x box_rows: the adapter operands of GemmExt.
+int make_tmap_lora(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols, uint32_t box_rows);
+
 // Tensor maps of one GEMM: A operand (box 64 x kGemmABoxRows), weights
 // (box 64 x kGemmBBoxRows) and the output (box 128 B x kGemmOutBoxRows; any
 // valid map for kEpiScorer, which writes through `out` directly).
@@ -89,10 +102,23 @@ struct GemmMaps {
   const CUtensorMap* out2 = nullptr;  // kEpiResidTail: the parts region
 };
 
+// Low-rank adapters of the rows (see lora.h): after its K loop, row block m of
+// every tile adds, for each entry e in [off[m], off[m + 1]), the product of
+// u's entry e (256 rows of 16 values and 16 remainders) with the 16 columns of
+// B's chunk chunk[e] (b_rows rows, ordered like the weight's).
+struct GemmExt {
+  const CUtensorMap* u;  // make_tmap_lora, box rows kGemmABoxRows
+  const CUtensorMap* b;  // make_tmap_lora, box rows bn / 2
+  const int* off;
+  const int* chunk;
+  int b_rows;
+};
+
 // bn: kGemmBN, or kGemmBNNarrow for kEpiResid / kEpiStoreF32 (then the
-// weight map's box has kGemmBNNarrow / 2 rows).
+// weight map's box has kGemmBNNarrow / 2 rows).  ext: adapters of the rows,
+// for the encoder's epilogues and kEpiPlain*.
 cudaError_t launch_gemm(int epilogue, const GemmMaps& maps, const GemmArgs& args, int num_sms,
-                        cudaStream_t stream, int bn = kGemmBN);
+                        cudaStream_t stream, int bn = kGemmBN, const GemmExt* ext = nullptr);
 
 // ---- attention over compacted sequences ----------------------------------------
 // Sequences longer than kAttnTcQRows (128) tokens: work items of at most 128

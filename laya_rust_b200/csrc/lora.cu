@@ -7,10 +7,10 @@
 // leaves it as a pair of 16-bit values (value and remainder, together 16 bits
 // more than one), so the second product's operands are 16-bit and the pair's
 // rounding stays far below that of y.  The second computes x W^T + u B^T in one f32
-// accumulator and rounds once.
+// accumulator and rounds once: the tcgen05 GEMM of gemm.cu, whose K loop goes on
+// over the adapters of its row block (GemmExt).
 //
-// Simple form: one warp per row for u, 32 x 32 output tiles in shared memory
-// for the products.
+// u, simple form: one warp per row.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -77,43 +77,6 @@ __global__ void __launch_bounds__(256) lora_shrink_rows(const LoraShrinkArgs a) 
   }
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) lora_expand_simple(const LoraExpandArgs a) {
-  __shared__ float sx[32][33], sw[32][33];
-  const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 32;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;  // 8 rows of threads, 4 output rows each
-  float acc[4] = {};
-  for (int k0 = 0; k0 < a.in; k0 += 32) {
-    for (int r = ty; r < 32; r += 8) {
-      const int m = m0 + r, n = n0 + r, k = k0 + tx;
-      sx[r][tx] = m < a.rows && k < a.in ? Num<T>::up(static_cast<const T*>(a.x)[m * a.ldx + k]) : 0.0f;
-      sw[r][tx] = n < a.out && k < a.in ? Num<T>::up(static_cast<const T*>(a.w)[n * a.ldw + k]) : 0.0f;
-    }
-    __syncthreads();
-    for (int k = 0; k < 32; ++k)
-      for (int i = 0; i < 4; ++i) acc[i] += sx[ty + 8 * i][k] * sw[tx][k];
-    __syncthreads();
-  }
-  const int n = n0 + tx;
-  if (n >= a.out) return;
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + ty + 8 * i;
-    if (m >= a.rows) continue;
-    float v = acc[i];
-    const int e0 = a.row_entry[m];
-    if (e0 >= 0) {
-      const int nc = a.nchunks[a.entry_chunk[e0] / a.chunks_per_slot];
-      for (int c = 0; c < nc; ++c) {
-        const T* u = static_cast<const T*>(a.u) + (e0 + c) * kLoraEntryElems + static_cast<size_t>(m % kLoraBlock) * 2 * kLoraChunk;
-        const T* B = static_cast<const T*>(a.b) + (static_cast<size_t>(a.entry_chunk[e0 + c]) * a.out_pad + n) * kLoraChunk;
-        for (int j = 0; j < kLoraChunk; ++j) v += (Num<T>::up(u[j]) + Num<T>::up(u[kLoraChunk + j])) * Num<T>::up(B[j]);
-      }
-    }
-    if (a.bias) v += a.bias[n];
-    static_cast<T*>(a.y)[m * a.ldy + n] = Num<T>::down(v);
-  }
-}
-
 }  // namespace
 
 cudaError_t launch_lora_shrink(const LoraShrinkArgs& a, cudaStream_t s) {
@@ -123,16 +86,6 @@ cudaError_t launch_lora_shrink(const LoraShrinkArgs& a, cudaStream_t s) {
     lora_shrink_rows<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
   else
     lora_shrink_rows<__half><<<grid, 256, 0, s>>>(a);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_lora_expand_simple(const LoraExpandArgs& a, cudaStream_t s) {
-  if (a.rows <= 0) return cudaSuccess;
-  const dim3 grid((a.out + 31) / 32, (a.rows + 31) / 32);
-  if (a.bf16)
-    lora_expand_simple<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
-  else
-    lora_expand_simple<__half><<<grid, 256, 0, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -205,6 +158,7 @@ struct Bank {
   const float* bias = nullptr;
   std::vector<Slot> slot;
   Buf a, b, scale, nchunks;
+  CUtensorMap b_map[2];  // B for 256- and 128-column tiles
   cudaStream_t stream = nullptr;  // uploads
   ~Bank() {
     int prev = -1;
@@ -233,6 +187,7 @@ struct Plan {
   const int* d_entry_chunk = nullptr;
   const int* d_off = nullptr;
   int* d_err = nullptr;
+  CUtensorMap u_map;
   ~Plan() {
     int prev = -1;
     cudaGetDevice(&prev);
@@ -297,7 +252,7 @@ int laya_lora_create(int device, int type, int64_t in, int64_t out, const void* 
     op_require(w, "lora_create: null weight");
     op_require(type == LAYA_F16 || type == LAYA_BF16, "lora_create: type must be LAYA_F16 or LAYA_BF16");
     op_require(in >= 1 && in <= (1 << 20) && out >= 1 && out <= (1 << 20), "lora_create: in and out must be 1..2^20");
-    op_require(ldw >= in && ldw <= (int64_t{1} << 31), "lora_create: ldw is smaller than in");
+    op_require(ldw >= in && ldw <= (int64_t{1} << 30), "lora_create: ldw is smaller than in");
     op_require(aligned16(w) && ldw % 8 == 0, "lora_create: W and its pitch must be multiples of 16 bytes");
     op_require(reinterpret_cast<uintptr_t>(bias) % 4 == 0, "lora_create: bias is not aligned");
     op_require(slots >= 1 && slots <= LAYA_LORA_MAX_SLOTS, "lora_create: slots must be 1..LAYA_LORA_MAX_SLOTS");
@@ -337,6 +292,9 @@ int laya_lora_create(int device, int type, int64_t in, int64_t out, const void* 
     op_check(cudaMemsetAsync(k->scale.p, 0, sizeof(float) * slots, k->stream), "lora clear");
     op_check(cudaMemsetAsync(k->nchunks.p, 0, sizeof(int) * slots, k->stream), "lora clear");
     op_check(cudaStreamSynchronize(k->stream), "lora clear");
+    if (make_tmap_lora(&k->b_map[0], k->b.p, k->bf16, chunks * out_pad, kLoraChunk, kGemmBBoxRows) ||
+        make_tmap_lora(&k->b_map[1], k->b.p, k->bf16, chunks * out_pad, kLoraChunk, kGemmBBoxRowsNarrow))
+      throw OpError(LAYA_E_CUDA, "lora_create: tensor map encode failed");
     *lora = new laya_lora{k};
   });
 }
@@ -408,11 +366,14 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     std::copy(L.row_entry.begin(), L.row_entry.end(), h.begin() + o_row);
     std::copy(entry_chunk.begin(), entry_chunk.end(), h.begin() + o_ent);
     q.dev.alloc(h.size() * 4, "lora plan");
-    q.u.alloc(L.chunk.size() * kLoraEntryElems * 2, "lora workspace");
+    const size_t entries = std::max<size_t>(1, L.chunk.size());
+    q.u.alloc(entries * kLoraEntryElems * 2, "lora workspace");
+    if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock, 2 * kLoraChunk, kGemmABoxRows))
+      throw OpError(LAYA_E_CUDA, "lora_plan_create: tensor map encode failed");
     op_check(cudaMemcpyAsync(q.dev.p, h.data(), h.size() * 4, cudaMemcpyHostToDevice, k.stream), "lora plan upload");
     // rows of other adapters are zero in an entry, and stay zero: every run
     // writes the same rows of each entry
-    op_check(cudaMemsetAsync(q.u.p, 0, L.chunk.size() * kLoraEntryElems * 2, k.stream), "lora workspace clear");
+    op_check(cudaMemsetAsync(q.u.p, 0, entries * kLoraEntryElems * 2, k.stream), "lora workspace clear");
     op_check(cudaStreamSynchronize(k.stream), "lora plan upload");
     q.d_err = q.dev.as<int>();
     q.d_off = q.dev.as<int>() + o_off;
@@ -431,7 +392,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     op_require(lora->bank == q.bank, "lora_run: the plan belongs to another projection");
     if (q.lay.rows == 0) return;
     op_require(x && y, "lora_run: null buffer");
-    constexpr int64_t kMaxPitch = int64_t{1} << 31;
+    constexpr int64_t kMaxPitch = int64_t{1} << 30;
     op_require(ldx >= k.in && ldx <= kMaxPitch, "lora_run: ldx is smaller than in");
     op_require(ldy >= k.out && ldy <= kMaxPitch, "lora_run: ldy is smaller than out");
     op_require(aligned16(x) && aligned16(y) && ldx % 8 == 0 && ldy % 8 == 0,
@@ -459,26 +420,28 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     s.nchunks = k.nchunks.as<int>();
     s.bf16 = k.bf16;
     if (!q.used.empty()) op_check(launch_lora_shrink(s, st), "lora launch");
-    LoraExpandArgs e{};
-    e.x = x;
-    e.ldx = ldx;
-    e.w = k.w;
-    e.ldw = k.ldw;
-    e.bias = k.bias;
-    e.b = k.b.p;
-    e.row_entry = q.d_row_entry;
-    e.entry_chunk = q.d_entry_chunk;
-    e.nchunks = k.nchunks.as<int>();
-    e.u = q.u.p;
-    e.y = y;
-    e.ldy = ldy;
-    e.rows = q.lay.rows;
-    e.in = k.in;
-    e.out = k.out;
-    e.out_pad = k.out_pad;
-    e.chunks_per_slot = k.cps;
-    e.bf16 = k.bf16;
-    op_check(launch_lora_expand_simple(e, st), "lora launch");
+    // x W^T and u B^T in one accumulator.  256 x 128 tiles where 256 x 256 ones
+    // would fill at most half the clusters, as in the engine.
+    const int tiles = (q.lay.rows + kGemmBM - 1) / kGemmBM * (k.out_pad / kGemmBN);
+    const bool narrow = tiles * 2 <= k.num_sms / 2;
+    const int bn = narrow ? kGemmBNNarrow : kGemmBN;
+    CUtensorMap mx, mw, my;
+    if (make_tmap_pitched(&mx, x, k.bf16, q.lay.rows, k.in, ldx, kGemmABoxRows) ||
+        make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, bn / 2) ||
+        make_tmap_pitched(&my, y, k.bf16, q.lay.rows, std::max(k.out & ~7, 8), ldy, kGemmOutBoxRows))
+      throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
+    GemmArgs g{};
+    g.M = q.lay.rows;
+    g.N = (k.out + bn - 1) / bn * bn;
+    g.K = k.in_pad;
+    g.err = q.d_err;
+    g.out = y;
+    g.ldo = static_cast<int>(ldy);
+    g.bias = k.bias;
+    g.n_valid = k.out;
+    const GemmExt ext{&q.u_map, &k.b_map[narrow], q.d_off, q.d_entry_chunk, k.out_pad};
+    op_check(launch_gemm(k.bf16 ? kEpiPlainBf16 : kEpiPlainF16, GemmMaps{&mx, &mw, &my}, g, k.num_sms, st, bn, &ext),
+             "lora launch");
   });
 }
 

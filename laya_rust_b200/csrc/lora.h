@@ -53,23 +53,4 @@ struct LoraShrinkArgs {
 // u entries of every row with an adapter: scale * (x A^T) as value + remainder.
 cudaError_t launch_lora_shrink(const LoraShrinkArgs& a, cudaStream_t s);
 
-struct LoraExpandArgs {
-  const void* x;
-  long long ldx;
-  const void* w;          // [out, in], pitch ldw
-  long long ldw;
-  const float* bias;      // [out] or nullptr
-  const void* b;          // the bank's B
-  const int* row_entry;
-  const int* entry_chunk;
-  const int* nchunks;
-  const void* u;
-  void* y;
-  long long ldy;
-  int rows, in, out, out_pad;
-  int chunks_per_slot;
-  bool bf16;
-};
-cudaError_t launch_lora_expand_simple(const LoraExpandArgs& a, cudaStream_t s);
-
 }  // namespace laya
