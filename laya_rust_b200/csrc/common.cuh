@@ -24,6 +24,7 @@ enum DeviceError : int {
   kErrGemmEpilogueWait = 3,
   kErrGemmTeardownWait = 4,
   kErrAttnWait = 5,
+  kErrLoraWait = 6,
 };
 
 // 2 s of wall clock: far above any legitimate wait in these kernels

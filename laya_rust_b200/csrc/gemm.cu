@@ -484,6 +484,7 @@ struct ExtParams {
   const int* off;
   const int* chunk;
   int b_rows;
+  int early;  // see GemmExt
 };
 struct NoExt {};
 
@@ -556,7 +557,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   // the prologue above touches only shared memory, TMEM and the tensor maps
-  grid_dep_wait();
+  bool early = false;
+  if constexpr (EXT) early = ext.early != 0;
+  if (!early) grid_dep_wait();
   grid_dep_trigger();
 
   if (warp == 0) {
@@ -600,6 +603,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (!ok || w.kb1 != num_kb) continue;
           const int mb = w.tile / num_n;
           const int e1 = __ldg(ext.off + mb + 1);
+          if (early) {
+            grid_dep_wait();  // u is complete
+            early = false;
+          }
           for (int e = __ldg(ext.off + mb); e < e1; e += 2) {
             const int n = min(2, e1 - e);
             const int chunk[2] = {__ldg(ext.chunk + e), n > 1 ? __ldg(ext.chunk + e + 1) : 0};
@@ -746,6 +753,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0) bulk_wait_all();
     __syncwarp();
   }
+  // this grid must not complete before the one that computes u: later launches
+  // wait for this grid only
+  if constexpr (EXT) grid_dep_wait();
   tc_fence_before();
   __syncwarp();
   cluster_sync();  // no CTA of the pair leaves while the other may still use it
@@ -812,7 +822,7 @@ cudaError_t launch_gemm(int epilogue, const GemmMaps& m, const GemmArgs& args, i
   }
   if (ext) {
     if (!ext->u || !ext->b || !ext->off || !ext->chunk || ext->b_rows < args.N) return cudaErrorInvalidValue;
-    const ExtParams x{*ext->u, *ext->b, ext->off, ext->chunk, ext->b_rows};
+    const ExtParams x{*ext->u, *ext->b, ext->off, ext->chunk, ext->b_rows, ext->early ? 1 : 0};
     if (bn == kGemmBNNarrow) {
       switch (epilogue) {
         case kEpiQkvRope: return launch_one<kEpiQkvRope, kGemmBNNarrow, true>(m, args, num_sms, stream, x);

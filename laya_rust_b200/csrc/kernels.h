@@ -112,6 +112,11 @@ struct GemmExt {
   const int* off;
   const int* chunk;
   int b_rows;
+  // The launch before this one computes u and nothing else this GEMM reads:
+  // only the adapter steps wait for it, and the K loop runs beside it.  Needs
+  // that launch to pass grid_dep_wait() before its grid_dep_trigger() (or to
+  // be an ordinary launch), so that everything before it has completed.
+  bool early;
 };
 
 // bn: kGemmBN, or kGemmBNNarrow for kEpiResid / kEpiStoreF32 (then the

@@ -8,9 +8,9 @@
 // more than one), so the second product's operands are 16-bit and the pair's
 // rounding stays far below that of y.  The second computes x W^T + u B^T in one f32
 // accumulator and rounds once: the tcgen05 GEMM of gemm.cu, whose K loop goes on
-// over the adapters of its row block (GemmExt).
-//
-// u, simple form: one warp per row.
+// over the adapters of its row block (GemmExt).  It is launched with programmatic
+// serialization and waits for u only before its adapter steps, so its K loop
+// runs beside the first launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -18,6 +18,7 @@
 #include <cmath>
 #include <cstring>
 #include <memory>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -50,43 +51,265 @@ __device__ __forceinline__ void split_value(float v, T& hi, T& lo) {
   lo = Num<T>::down(isfinite(h) ? v - h : 0.0f);
 }
 
+constexpr int kXBytes = kLoraItemRows * 64 * 2;   // x operand of a k-block: 16 KB
+constexpr int kABytes = kLoraChunk * 64 * 2;      // one entry's A operand: 2 KB
+constexpr int kRingBytes = 192 * 1024;
+constexpr int kMaxStages = 8;
+constexpr size_t kShrinkSmem = 1024 + kRingBytes + 256;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f4(const float* p, uint32_t rank) {
+  uint32_t r;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(r)
+               : "memory");
+  return v;
+}
+
+// u = scale (x A^T) for one item: 128 rows against up to 8 entries (M = 128,
+// N = 16 entries), K cut over the CTAs of a cluster.  Per CTA: warp 0 loads
+// (TMA ring of x and A k-blocks), warp 1 issues the MMAs, then all four warps
+// take the f32 sums from TMEM to shared memory, the CTAs of the cluster add
+// each other's parts in rank order (distributed shared memory, rows dealt out
+// over the CTAs) and store the entries each row owns.
 template <class T>
-__global__ void __launch_bounds__(256) lora_shrink_rows(const LoraShrinkArgs a) {
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= a.rows) return;
-  const int e0 = a.row_entry[row];
-  if (e0 < 0) return;
-  const int slot = a.entry_chunk[e0] / a.chunks_per_slot;
-  const float scale = a.scale[slot];
-  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-  for (int c = 0; c < a.nchunks[slot]; ++c) {
-    const T* A = static_cast<const T*>(a.a) + static_cast<size_t>(a.entry_chunk[e0 + c]) * kLoraChunk * a.in_pad;
-    float acc[kLoraChunk] = {};
-    for (int k = lane; k < a.in; k += 32) {
-      const float v = Num<T>::up(x[k]);
-#pragma unroll
-      for (int j = 0; j < kLoraChunk; ++j) acc[j] += v * Num<T>::up(A[static_cast<size_t>(j) * a.in_pad + k]);
+__global__ void __launch_bounds__(128, 1)
+    lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
+                       const LoraShrinkArgs a, const int splits) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kRingBytes);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* done = empty + kMaxStages;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int4 item = __ldg(a.item + blockIdx.x / splits);
+  const int n = item.z;
+  const int stage_bytes = kXBytes + a.group * kABytes;
+  const int stages = min(kMaxStages, kRingBytes / stage_bytes);
+  const int kb0 = static_cast<int>(rank) * a.num_kb / splits, kb1 = (static_cast<int>(rank) + 1) * a.num_kb / splits;
+  const uint32_t tmem_cols = a.group <= 2 ? 32 : 16 * a.group;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kMaxStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
-    T* u = static_cast<T*>(a.u) + (e0 + c) * kLoraEntryElems + static_cast<size_t>(row % kLoraBlock) * 2 * kLoraChunk;
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmA);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  grid_dep_wait();
+  grid_dep_trigger();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag)) {
+          ok = false;
+          break;
+        }
+        uint8_t* sx = smem + stage * stage_bytes;
+        mbar_arrive_expect_tx(&full[stage], kXBytes + n * kABytes);
+        tma_load_2d(sx, &tmX, kb * 64, item.x * kLoraItemRows, &full[stage]);
+        for (int i = 0; i < n; ++i)
+          tma_load_2d(sx + kXBytes + i * kABytes, &tmA, kb * 64,
+                      __ldg(a.entry_chunk + __ldg(a.item_entry + item.y + i)) * kLoraChunk, &full[stage]);
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok || *abort_flag) {
+        // loads in flight land before the CTA leaves
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 2000000ull) __nanosleep(1000);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = std::is_same<T, __nv_bfloat16>::value ? umma_idesc_bf16(kLoraItemRows, 16 * n)
+                                                                    : umma_idesc_f16(kLoraItemRows, 16 * n);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait_bounded(&full[stage], phase, a.err, kErrLoraWait, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t x_addr = smem_u32(smem + stage * stage_bytes), a_addr = x_addr + kXBytes;
 #pragma unroll
-    for (int j = 0; j < kLoraChunk; ++j) {
-      float v = acc[j];
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) split_value<T>(v * scale, u[j], u[kLoraChunk + j]);
+        for (int k = 0; k < 4; ++k)
+          umma_f16(tmem, umma_desc_sw128(x_addr + k * 32), umma_desc_sw128(a_addr + k * 32), idesc,
+                   (kb != kb0 || k != 0) ? 1u : 0u);
+        umma_commit(&empty[stage]);
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      umma_commit(done);
+    }
+    __syncwarp();
+  }
+  // this CTA's sums to shared memory (the ring is idle: every k-block was
+  // consumed), one row a thread; 4 floats of padding a row
+  float* part = reinterpret_cast<float*>(smem);
+  const int ld = 16 * a.group + 4;
+  bool ok = mbar_wait_bounded(done, 0, a.err, kErrLoraWait, nullptr) && !*abort_flag;
+  ok = __syncthreads_and(ok);
+  tc_fence_after();
+  if (ok) {
+    for (int i = 0; i < n; ++i) {
+      uint32_t v[16];
+      tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + i * 16, v);
+      tmem_ld_wait();
+      float4* dst = reinterpret_cast<float4*>(part + threadIdx.x * ld + i * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        dst[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
+                             __uint_as_float(v[4 * j + 3]));
     }
   }
+  tc_fence_before();
+  cluster_sync();
+  // `splits` threads a row, each every splits-th entry
+  const int r = static_cast<int>(rank) * (kLoraItemRows / splits) + threadIdx.x / splits;
+  const int row = item.x * kLoraItemRows + r;
+  const int e0 = ok && row < a.rows ? __ldg(a.row_entry + row) : -1;
+  if (e0 >= 0) {
+    const int slot = __ldg(a.entry_chunk + e0) / a.chunks_per_slot;
+    const float scale = __ldg(a.scale + slot);
+    for (int i = threadIdx.x % splits; i < n; i += splits) {
+      const int e = __ldg(a.item_entry + item.y + i);
+      if (__ldg(a.entry_chunk + e) / a.chunks_per_slot != slot) continue;
+      T hi[16], lo[16];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float4 s = ld_cluster_f4(part + r * ld + i * 16 + 4 * j, 0);
+        for (int c = 1; c < splits; ++c) {
+          const float4 t = ld_cluster_f4(part + r * ld + i * 16 + 4 * j, c);
+          s.x += t.x;
+          s.y += t.y;
+          s.z += t.z;
+          s.w += t.w;
+        }
+        split_value<T>(s.x * scale, hi[4 * j], lo[4 * j]);
+        split_value<T>(s.y * scale, hi[4 * j + 1], lo[4 * j + 1]);
+        split_value<T>(s.z * scale, hi[4 * j + 2], lo[4 * j + 2]);
+        split_value<T>(s.w * scale, hi[4 * j + 3], lo[4 * j + 3]);
+      }
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.u) + static_cast<size_t>(e) * kLoraEntryElems +
+                                            static_cast<size_t>(row % kLoraBlock) * 2 * kLoraChunk);
+      dst[0] = *reinterpret_cast<uint4*>(hi);
+      dst[1] = *reinterpret_cast<uint4*>(hi + 8);
+      dst[2] = *reinterpret_cast<uint4*>(lo);
+      dst[3] = *reinterpret_cast<uint4*>(lo + 8);
+    }
+  }
+  cluster_sync();  // no CTA leaves while another may still read its part
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+template <class T>
+cudaError_t launch_shrink(const CUtensorMap& x, const CUtensorMap& a_map, const LoraShrinkArgs& a, int splits, bool pdl,
+                          cudaStream_t s) {
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    e = cudaFuncSetAttribute(lora_shrink_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(kShrinkSmem));
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  const dim3 grid(a.items * splits);
+  if (pdl) return launch_pdl(lora_shrink_kernel<T>, grid, dim3(128), kShrinkSmem, s, attr, 1, x, a_map, a, splits);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = kShrinkSmem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, lora_shrink_kernel<T>, x, a_map, a, splits);
 }
 
 }  // namespace
 
-cudaError_t launch_lora_shrink(const LoraShrinkArgs& a, cudaStream_t s) {
-  if (a.rows <= 0) return cudaSuccess;
-  const int grid = (a.rows + 7) / 8;
-  if (a.bf16)
-    lora_shrink_rows<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
-  else
-    lora_shrink_rows<__half><<<grid, 256, 0, s>>>(a);
-  return cudaGetLastError();
+cudaError_t launch_lora_shrink(const CUtensorMap& x, const CUtensorMap& a_map, const LoraShrinkArgs& a, int num_sms,
+                               bool pdl, cudaStream_t s) {
+  if (a.items <= 0) return cudaSuccess;
+  if (a.num_kb < 1 || a.group < 1 || a.group > kLoraMaxGroup) return cudaErrorInvalidValue;
+  int splits = 1;
+  while (splits < 8 && 2 * splits * a.items <= num_sms && 4 * splits <= a.num_kb) splits *= 2;
+  return a.bf16 ? launch_shrink<__nv_bfloat16>(x, a_map, a, splits, pdl, s)
+                : launch_shrink<__half>(x, a_map, a, splits, pdl, s);
+}
+
+LoraItems lora_items(const LoraLayout& L, int num_sms) {
+  // the entries of each 128 rows, by the order of their first row
+  LoraItems it;
+  const int halves = (L.rows + kLoraItemRows - 1) / kLoraItemRows;
+  std::vector<std::vector<int>> need(halves);
+  for (int h = 0; h < halves; ++h) {
+    std::vector<int>& v = need[h];
+    int last = -1;
+    for (int m = h * kLoraItemRows; m < std::min(L.rows, (h + 1) * kLoraItemRows); ++m) {
+      const int e0 = L.row_entry[m];
+      if (e0 < 0 || e0 == last) continue;
+      last = e0;
+      if (std::find(v.begin(), v.end(), e0) != v.end()) continue;
+      for (int e = e0; e < static_cast<int>(L.chunk.size()) && (e == e0 || L.chunk[e].y > 0); ++e) v.push_back(e);
+    }
+  }
+  // the smallest group whose items still run at once
+  for (it.group = 1;; it.group *= 2) {
+    size_t items = 0;
+    for (const auto& v : need) items += (v.size() + it.group - 1) / it.group;
+    if (items <= static_cast<size_t>(num_sms) || it.group == kLoraMaxGroup) break;
+  }
+  for (int h = 0; h < halves; ++h)
+    for (size_t i = 0; i < need[h].size(); i += it.group) {
+      const int n = static_cast<int>(std::min<size_t>(it.group, need[h].size() - i));
+      it.item.push_back(make_int4(h, static_cast<int>(it.entry.size()), n, 0));
+      it.entry.insert(it.entry.end(), need[h].begin() + i, need[h].begin() + i + n);
+    }
+  return it;
 }
 
 LoraLayout lora_layout(const int32_t* rows, const int32_t* slot, int n, const std::vector<int>& chunks_of) {
@@ -157,7 +380,8 @@ struct Bank {
   long long ldw = 0;
   const float* bias = nullptr;
   std::vector<Slot> slot;
-  Buf a, b, scale, nchunks;
+  Buf a, b, scale;
+  CUtensorMap a_map;
   CUtensorMap b_map[2];  // B for 256- and 128-column tiles
   cudaStream_t stream = nullptr;  // uploads
   ~Bank() {
@@ -165,7 +389,7 @@ struct Bank {
     cudaGetDevice(&prev);
     cudaSetDevice(device);
     if (stream) cudaStreamDestroy(stream);
-    for (Buf* x : {&a, &b, &scale, &nchunks}) {
+    for (Buf* x : {&a, &b, &scale}) {
       if (x->p) cudaFree(x->p);
       x->p = nullptr;
     }
@@ -183,6 +407,9 @@ struct Plan {
   LoraLayout lay;
   std::vector<std::pair<int, int>> used;  // (slot, chunks)
   Buf dev, u;
+  int items = 0, group = 0;
+  const int4* d_item = nullptr;
+  const int* d_item_entry = nullptr;
   const int* d_row_entry = nullptr;
   const int* d_entry_chunk = nullptr;
   const int* d_off = nullptr;
@@ -286,13 +513,12 @@ int laya_lora_create(int device, int type, int64_t in, int64_t out, const void* 
     k->a.alloc(chunks * kLoraChunk * in_pad * 2, "lora adapters");
     k->b.alloc(chunks * kLoraChunk * out_pad * 2, "lora adapters");
     k->scale.alloc(sizeof(float) * slots, "lora scales");
-    k->nchunks.alloc(sizeof(int) * slots, "lora ranks");
     op_check(cudaMemsetAsync(k->a.p, 0, chunks * kLoraChunk * in_pad * 2, k->stream), "lora clear");
     op_check(cudaMemsetAsync(k->b.p, 0, chunks * kLoraChunk * out_pad * 2, k->stream), "lora clear");
     op_check(cudaMemsetAsync(k->scale.p, 0, sizeof(float) * slots, k->stream), "lora clear");
-    op_check(cudaMemsetAsync(k->nchunks.p, 0, sizeof(int) * slots, k->stream), "lora clear");
     op_check(cudaStreamSynchronize(k->stream), "lora clear");
-    if (make_tmap_lora(&k->b_map[0], k->b.p, k->bf16, chunks * out_pad, kLoraChunk, kGemmBBoxRows) ||
+    if (make_tmap_pitched(&k->a_map, k->a.p, k->bf16, chunks * kLoraChunk, in_pad, in_pad, kLoraChunk) ||
+        make_tmap_lora(&k->b_map[0], k->b.p, k->bf16, chunks * out_pad, kLoraChunk, kGemmBBoxRows) ||
         make_tmap_lora(&k->b_map[1], k->b.p, k->bf16, chunks * out_pad, kLoraChunk, kGemmBBoxRowsNarrow))
       throw OpError(LAYA_E_CUDA, "lora_create: tensor map encode failed");
     *lora = new laya_lora{k};
@@ -317,13 +543,11 @@ int laya_lora_set(laya_lora* lora, int slot, int rank, const void* a, const void
         hb[(static_cast<size_t>(r / kLoraChunk) * k.out_pad + n) * kLoraChunk + r % kLoraChunk] =
             store_host(load_host(b, host_type, static_cast<size_t>(n) * rank + r), k.bf16);
     DeviceScope scope(k.device);
-    const int nc = lora_chunks(rank);
     // runs already queued on the caller's streams may still read the slot
     op_check(cudaDeviceSynchronize(), "lora_set");
     op_check(cudaMemcpyAsync(k.a.as<uint16_t>() + ha.size() * slot, ha.data(), ha.size() * 2, cudaMemcpyHostToDevice, k.stream), "lora upload");
     op_check(cudaMemcpyAsync(k.b.as<uint16_t>() + hb.size() * slot, hb.data(), hb.size() * 2, cudaMemcpyHostToDevice, k.stream), "lora upload");
     op_check(cudaMemcpyAsync(k.scale.as<float>() + slot, &scale, 4, cudaMemcpyHostToDevice, k.stream), "lora upload");
-    op_check(cudaMemcpyAsync(k.nchunks.as<int>() + slot, &nc, 4, cudaMemcpyHostToDevice, k.stream), "lora upload");
     op_check(cudaStreamSynchronize(k.stream), "lora upload");
     k.slot[slot].rank = rank;
   });
@@ -358,10 +582,17 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     std::sort(q.used.begin(), q.used.end());
     q.used.erase(std::unique(q.used.begin(), q.used.end()), q.used.end());
     DeviceScope scope(k.device);
-    // [error word | off | row entries | entry chunks], each 256-byte aligned
+    const LoraItems it = lora_items(L, k.num_sms);
+    q.items = static_cast<int>(it.item.size());
+    q.group = it.group;
+    // [error word | off | row entries | entry chunks | items | their entries],
+    // each 256-byte aligned
     auto up = [](size_t v) { return (v + 63) / 64 * 64; };
     const size_t o_off = 64, o_row = o_off + up(L.off.size()), o_ent = o_row + up(L.row_entry.size());
-    std::vector<int> h(o_ent + up(entry_chunk.size()));
+    const size_t o_item = o_ent + up(entry_chunk.size()), o_ie = o_item + up(4 * it.item.size());
+    std::vector<int> h(o_ie + up(it.entry.size()));
+    if (!it.item.empty()) memcpy(h.data() + o_item, it.item.data(), it.item.size() * sizeof(int4));
+    std::copy(it.entry.begin(), it.entry.end(), h.begin() + o_ie);
     std::copy(L.off.begin(), L.off.end(), h.begin() + o_off);
     std::copy(L.row_entry.begin(), L.row_entry.end(), h.begin() + o_row);
     std::copy(entry_chunk.begin(), entry_chunk.end(), h.begin() + o_ent);
@@ -379,6 +610,8 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     q.d_off = q.dev.as<int>() + o_off;
     q.d_row_entry = q.dev.as<int>() + o_row;
     q.d_entry_chunk = q.dev.as<int>() + o_ent;
+    q.d_item = reinterpret_cast<const int4*>(q.dev.as<int>() + o_item);
+    q.d_item_entry = q.dev.as<int>() + o_ie;
     *plan = p.release();
   });
 }
@@ -405,21 +638,6 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     require_device_ptr(x, k.device, "lora_run: x");
     require_device_ptr(y, k.device, "lora_run: y");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    LoraShrinkArgs s{};
-    s.x = x;
-    s.ldx = ldx;
-    s.a = k.a.p;
-    s.row_entry = q.d_row_entry;
-    s.entry_chunk = q.d_entry_chunk;
-    s.scale = k.scale.as<float>();
-    s.u = q.u.p;
-    s.rows = q.lay.rows;
-    s.in = k.in;
-    s.in_pad = k.in_pad;
-    s.chunks_per_slot = k.cps;
-    s.nchunks = k.nchunks.as<int>();
-    s.bf16 = k.bf16;
-    if (!q.used.empty()) op_check(launch_lora_shrink(s, st), "lora launch");
     // x W^T and u B^T in one accumulator.  256 x 128 tiles where 256 x 256 ones
     // would fill at most half the clusters, as in the engine.
     const int tiles = (q.lay.rows + kGemmBM - 1) / kGemmBM * (k.out_pad / kGemmBN);
@@ -430,6 +648,23 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
         make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, bn / 2) ||
         make_tmap_pitched(&my, y, k.bf16, q.lay.rows, std::max(k.out & ~7, 8), ldy, kGemmOutBoxRows))
       throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
+    if (q.items > 0) {
+      LoraShrinkArgs s{};
+      s.item = q.d_item;
+      s.item_entry = q.d_item_entry;
+      s.items = q.items;
+      s.group = q.group;
+      s.row_entry = q.d_row_entry;
+      s.entry_chunk = q.d_entry_chunk;
+      s.scale = k.scale.as<float>();
+      s.u = q.u.p;
+      s.rows = q.lay.rows;
+      s.num_kb = k.in_pad / 64;
+      s.chunks_per_slot = k.cps;
+      s.bf16 = k.bf16;
+      s.err = q.d_err;
+      op_check(launch_lora_shrink(mx, k.a_map, s, k.num_sms, false, st), "lora launch");
+    }
     GemmArgs g{};
     g.M = q.lay.rows;
     g.N = (k.out + bn - 1) / bn * bn;
@@ -439,7 +674,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     g.ldo = static_cast<int>(ldy);
     g.bias = k.bias;
     g.n_valid = k.out;
-    const GemmExt ext{&q.u_map, &k.b_map[narrow], q.d_off, q.d_entry_chunk, k.out_pad};
+    const GemmExt ext{&q.u_map, &k.b_map[narrow], q.d_off, q.d_entry_chunk, k.out_pad, q.items > 0};
     op_check(launch_gemm(k.bf16 ? kEpiPlainBf16 : kEpiPlainF16, GemmMaps{&mx, &mw, &my}, g, k.num_sms, st, bn, &ext),
              "lora launch");
   });

@@ -1,6 +1,7 @@
 // Low-rank adapters beside a shared projection: the host plan of a batch and
 // the device kernels' launchers.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -37,20 +38,34 @@ LoraLayout lora_layout(const int32_t* rows, const int32_t* slot, int n, const st
 
 constexpr size_t kLoraEntryElems = static_cast<size_t>(kLoraBlock) * 2 * kLoraChunk;
 
+// The work of the rank-space product: item i computes entries
+// entry[item.y .. item.y + item.z) for rows [128 item.x, 128 item.x + 128).
+// Only entries some row of those 128 has are listed.
+constexpr int kLoraItemRows = 128;
+constexpr int kLoraMaxGroup = 8;  // entries per item
+struct LoraItems {
+  int group = 1;            // most entries of an item: 1, 2, 4 or 8
+  std::vector<int4> item;
+  std::vector<int> entry;
+};
+LoraItems lora_items(const LoraLayout& L, int num_sms);
+
 struct LoraShrinkArgs {
-  const void* x;          // [rows, in], pitch ldx
-  long long ldx;
-  const void* a;          // the bank's A
+  const int4* item;
+  const int* item_entry;
+  int items, group;
   const int* row_entry;   // [rows]
   const int* entry_chunk; // [entries]: chunk in the bank
   const float* scale;     // per slot
   void* u;
-  int rows, in, in_pad;
+  int rows, num_kb;       // num_kb: in / 64, rounded up
   int chunks_per_slot;
-  const int* nchunks;     // [slots]
   bool bf16;
+  int* err;
 };
 // u entries of every row with an adapter: scale * (x A^T) as value + remainder.
-cudaError_t launch_lora_shrink(const LoraShrinkArgs& a, cudaStream_t s);
+// x: box 64 x 128, A (make_tmap_pitched, [chunks * 16, in_pad]): box 64 x 16.
+cudaError_t launch_lora_shrink(const CUtensorMap& x, const CUtensorMap& a_map, const LoraShrinkArgs& a, int num_sms,
+                               bool pdl, cudaStream_t s);
 
 }  // namespace laya
