@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <exception>
 #include <new>
 #include <stdexcept>
@@ -49,13 +50,31 @@ int op_guard(F&& f) {
   }
 }
 
+// The number of devices, asked once it is known (a failed query is repeated).
+inline int device_count() {
+  static std::atomic<int> known{0};
+  int n = known.load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  op_check(cudaGetDeviceCount(&n), "cudaGetDeviceCount");
+  known.store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// SMs of a device (one that exists), asked once.
+inline int device_sms(int device) {
+  static std::atomic<int> known[64] = {};
+  int n = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  op_check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device), "device query");
+  if (device < 64) known[device].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 // Makes `device` current and restores the caller's device on the way out.
 struct DeviceScope {
   int prev = -1;
   explicit DeviceScope(int device) {
-    int n = 0;
-    op_check(cudaGetDeviceCount(&n), "cudaGetDeviceCount");
-    if (device < 0 || device >= n) throw OpError(LAYA_E_INVALID, "device out of range");
+    if (device < 0 || device >= device_count()) throw OpError(LAYA_E_INVALID, "device out of range");
     op_check(cudaGetDevice(&prev), "cudaGetDevice");
     if (prev == device) {
       prev = -1;

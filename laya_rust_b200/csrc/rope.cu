@@ -11,7 +11,11 @@
 // as an integer, so the f32 sine and cosine see a reduced argument whose
 // conversion rounds relative to itself.
 //
-// Simple form: one thread per (token, head, pair or copied element).
+// Bound by memory: every element is read and written once.  A thread owns one
+// 16-byte piece of a head (for the half layout the piece and its partner
+// rot / 2 further), computes the sines and cosines of its pairs once, and
+// turns the same piece of several heads with them, so the angles cost little
+// beside the copies.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -34,12 +38,14 @@ struct RopeTensorArg {
   void* out;
   long long x_token, x_head, out_token, out_head;
   int heads;
+  int group0;  // first head group of this tensor (heads_per_thread heads each)
 };
 
 struct RopeArgs {
   RopeTensorArg t[kMaxTensors];
   int count;
   int dim, rot;
+  int heads_per_thread;
   long long tokens;
   const int* pos;
   long long pos0;
@@ -78,31 +84,83 @@ __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v);
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 
-template <class T, bool HALF>
+// V elements moved as one access of sizeof(T) * V bytes.
+template <class T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T v[V];
+};
+
+constexpr int kHeadsAtOnce = 4;  // loads in flight a thread
+
+// VEC elements a piece; rot / 2 (half) or rot (interleaved), dim - rot, every
+// stride and address are multiples of it.
+template <class T, int VEC, bool HALF>
 __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeArgs a) {
-  const int half = a.rot / 2, copied = a.dim - a.rot, units = half + copied;
-  const RopeTensorArg& t = a.t[blockIdx.z];
-  const long long n = a.tokens * t.heads * units;
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
-       i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const int u = static_cast<int>(i % units);
-    const long long th = i / units;
-    const int h = static_cast<int>(th % t.heads);
-    const long long tok = th / t.heads;
-    const T* x = static_cast<const T*>(t.x) + tok * t.x_token + h * t.x_head;
-    T* o = static_cast<T*>(t.out) + tok * t.out_token + h * t.out_head;
-    if (u >= half) {
-      o[a.rot + u - half] = x[a.rot + u - half];
+  using P = Vec<T, VEC>;
+  constexpr int kPairs = HALF ? VEC : (VEC + 1) / 2;
+  constexpr int kPieces = HALF || VEC == 1 ? 2 : 1;  // pieces a unit turns
+  const int turned = HALF ? a.rot / 2 / VEC : a.rot / (kPieces * VEC);
+  const int units = turned + (a.dim - a.rot) / VEC;
+  int ti = 0;
+  while (ti + 1 < a.count && static_cast<int>(blockIdx.y) >= a.t[ti + 1].group0) ++ti;
+  const RopeTensorArg& t = a.t[ti];
+  const int h0 = (static_cast<int>(blockIdx.y) - t.group0) * a.heads_per_thread;
+  const int h1 = min(t.heads, h0 + a.heads_per_thread);
+  const long long n = a.tokens * units;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n;
+       i += static_cast<long long>(gridDim.x) * 256) {
+    const long long tok = n < (1ll << 31) ? static_cast<int>(i) / units : i / units;
+    const int u = static_cast<int>(i - tok * units);
+    const T* x = static_cast<const T*>(t.x) + tok * t.x_token;
+    T* o = static_cast<T*>(t.out) + tok * t.out_token;
+    if (u >= turned) {
+      if (t.x == t.out) continue;
+      const int at = a.rot + (u - turned) * VEC;
+      for (int h = h0; h < h1; h += kHeadsAtOnce) {
+        P p[kHeadsAtOnce];
+#pragma unroll
+        for (int k = 0; k < kHeadsAtOnce; ++k)
+          if (h + k < h1) p[k] = *reinterpret_cast<const P*>(x + (h + k) * t.x_head + at);
+#pragma unroll
+        for (int k = 0; k < kHeadsAtOnce; ++k)
+          if (h + k < h1) *reinterpret_cast<P*>(o + (h + k) * t.out_head + at) = p[k];
+      }
       continue;
     }
-    float c, s;
-    rope_angle(a.turns[u], a.pos ? a.pos[tok] : a.pos0 + tok, c, s);
-    c *= a.mscale;
-    s *= a.mscale * a.sign;
-    const int i0 = HALF ? u : 2 * u, i1 = HALF ? u + half : 2 * u + 1;
-    const float v0 = to_f32(x[i0]), v1 = to_f32(x[i1]);
-    o[i0] = from_f32<T>(v0 * c - v1 * s);
-    o[i1] = from_f32<T>(v1 * c + v0 * s);
+    const long long p0 = a.pos ? __ldg(a.pos + tok) : a.pos0 + tok;
+    float c[kPairs], s[kPairs];
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      rope_angle(a.turns[u * kPairs + j], p0, c[j], s[j]);
+      c[j] *= a.mscale;
+      s[j] *= a.mscale * a.sign;
+    }
+    // where the unit's pieces start: pairs are (first[j], second[j]) across
+    // two pieces, or neighbours within one
+    const int at0 = HALF ? u * VEC : u * kPieces * VEC, at1 = HALF ? a.rot / 2 + u * VEC : at0 + VEC;
+    for (int h = h0; h < h1; h += kHeadsAtOnce) {
+      P p[kHeadsAtOnce], q[kHeadsAtOnce];
+#pragma unroll
+      for (int k = 0; k < kHeadsAtOnce; ++k)
+        if (h + k < h1) {
+          p[k] = *reinterpret_cast<const P*>(x + (h + k) * t.x_head + at0);
+          if (kPieces == 2) q[k] = *reinterpret_cast<const P*>(x + (h + k) * t.x_head + at1);
+        }
+#pragma unroll
+      for (int k = 0; k < kHeadsAtOnce; ++k)
+        if (h + k < h1) {
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) {
+            T& e0 = kPieces == 2 ? p[k].v[j] : p[k].v[(2 * j) % VEC];
+            T& e1 = kPieces == 2 ? q[k].v[j] : p[k].v[(2 * j + 1) % VEC];
+            const float v0 = to_f32(e0), v1 = to_f32(e1);
+            e0 = from_f32<T>(v0 * c[j] - v1 * s[j]);
+            e1 = from_f32<T>(v1 * c[j] + v0 * s[j]);
+          }
+          *reinterpret_cast<P*>(o + (h + k) * t.out_head + at0) = p[k];
+          if (kPieces == 2) *reinterpret_cast<P*>(o + (h + k) * t.out_head + at1) = q[k];
+        }
+    }
   }
 }
 
@@ -123,18 +181,52 @@ __global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__
   a.sinb[i] = a.mscale * s;
 }
 
-template <class T>
-cudaError_t launch_rope(const RopeArgs& a, bool half, cudaStream_t st) {
-  long long n = 0;
-  for (int i = 0; i < a.count; ++i)
-    n = std::max(n, a.tokens * a.t[i].heads * (a.rot / 2 + a.dim - a.rot));
-  if (n == 0) return cudaSuccess;
-  const dim3 grid(static_cast<unsigned>(std::min<long long>((n + 255) / 256, 1 << 20)), 1, a.count);
+template <class T, int VEC>
+cudaError_t launch_vec(const RopeArgs& a, bool half, dim3 grid, cudaStream_t st) {
   if (half)
-    rope_kernel<T, true><<<grid, 256, 0, st>>>(a);
+    rope_kernel<T, VEC, true><<<grid, 256, 0, st>>>(a);
   else
-    rope_kernel<T, false><<<grid, 256, 0, st>>>(a);
+    rope_kernel<T, VEC, false><<<grid, 256, 0, st>>>(a);
   return cudaGetLastError();
+}
+
+// Whether pieces of `v` elements of `es` bytes fit the head, every stride and
+// every address.
+bool pieces_fit(const RopeArgs& a, bool half, int es, int v) {
+  if ((half ? a.rot / 2 : a.rot) % v || (a.dim - a.rot) % v) return false;
+  for (int i = 0; i < a.count; ++i) {
+    const RopeTensorArg& t = a.t[i];
+    if ((reinterpret_cast<uintptr_t>(t.x) | reinterpret_cast<uintptr_t>(t.out)) % (es * v)) return false;
+    if ((t.x_token | t.x_head | t.out_token | t.out_head) % v) return false;
+  }
+  return true;
+}
+
+template <class T>
+cudaError_t launch_rope(RopeArgs& a, bool half, int num_sms, cudaStream_t st) {
+  constexpr int es = sizeof(T), kMaxVec = 16 / es;
+  int v = kMaxVec;
+  while (v > 1 && !pieces_fit(a, half, es, v)) v /= 2;
+  const int units = (half ? a.rot / 2 / v : v == 1 ? a.rot / 2 : a.rot / v) + (a.dim - a.rot) / v;
+  const long long n = a.tokens * units;
+  // heads a thread: as many as 8, while there are still two full waves of threads
+  int heads = 0;
+  for (int i = 0; i < a.count; ++i) heads += a.t[i].heads;
+  a.heads_per_thread = 8;
+  while (a.heads_per_thread > 1 && n * heads < 2ll * 2048 * num_sms * a.heads_per_thread) a.heads_per_thread /= 2;
+  int groups = 0;
+  for (int i = 0; i < a.count; ++i) {
+    a.t[i].group0 = groups;
+    groups += (a.t[i].heads + a.heads_per_thread - 1) / a.heads_per_thread;
+  }
+  if (groups > 65535) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(std::min<long long>((n + 255) / 256, 1 << 22)), groups);
+  switch (v) {
+    case 8: return launch_vec<T, kMaxVec>(a, half, grid, st);
+    case 4: return launch_vec<T, 4>(a, half, grid, st);
+    case 2: return launch_vec<T, 2>(a, half, grid, st);
+    default: return launch_vec<T, 1>(a, half, grid, st);
+  }
 }
 
 bool finite_positive(double v) { return std::isfinite(v) && v > 0; }
@@ -169,12 +261,12 @@ float rope_stretch(double* f, int rot, const laya_rope_scaling* s) {
 }
 
 uint64_t rope_turns(double f) {
-  // 2 pi to the 64 bits of a long double
-  const long double two_pi = 6.283185307179586476925286766559L;
-  long double t = static_cast<long double>(f) / two_pi;
-  t -= floorl(t);
-  t = roundl(t * 18446744073709551616.0L);
-  return t >= 18446744073709551616.0L ? 0ull : static_cast<uint64_t>(t);
+  // f / (2 pi) as the product with 1 / (2 pi) in two doubles: the leading
+  // product, its exact error, and the constant's tail
+  constexpr double kInvHi = 0.15915494309189535, kInvLo = -9.839338337591243e-18;
+  const double hi = f * kInvHi, lo = std::fma(f, kInvHi, -hi) + f * kInvLo;
+  const double frac = hi - std::floor(hi);  // exact
+  return static_cast<uint64_t>(frac * 18446744073709551616.0) + static_cast<uint64_t>(static_cast<int64_t>(lo * 18446744073709551616.0));
 }
 
 cudaError_t launch_rope_table(const double* freqs, int n, float mscale, int positions, float* cosb, float* sinb,
@@ -275,9 +367,10 @@ extern "C" int laya_rope(int device, const laya_rope_spec* spec, const laya_rope
     a.sign = spec->inverse ? -1.0f : 1.0f;
     const bool half = spec->layout == LAYA_ROPE_HALF;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e = spec->type == LAYA_F16    ? launch_rope<__half>(a, half, st)
-                    : spec->type == LAYA_BF16 ? launch_rope<__nv_bfloat16>(a, half, st)
-                                              : launch_rope<float>(a, half, st);
+    const int sms = device_sms(device);
+    cudaError_t e = spec->type == LAYA_F16    ? launch_rope<__half>(a, half, sms, st)
+                    : spec->type == LAYA_BF16 ? launch_rope<__nv_bfloat16>(a, half, sms, st)
+                                              : launch_rope<float>(a, half, sms, st);
     op_check(e, "rope launch");
   });
 }

@@ -9,6 +9,7 @@ enqueue work and return; errors raise :class:`LayaError`.
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -37,10 +38,7 @@ class _CRopeSpec(ctypes.Structure):
                 ("dim", ctypes.c_int32), ("rot", ctypes.c_int32), ("mscale", ctypes.c_float), ("freqs", _f64p)]
 
 
-class _CRopeTensor(ctypes.Structure):
-    _fields_ = [("x", ctypes.c_void_p), ("out", ctypes.c_void_p), ("x_token", ctypes.c_int64),
-                ("x_head", ctypes.c_int64), ("out_token", ctypes.c_int64), ("out_head", ctypes.c_int64),
-                ("heads", ctypes.c_int64)]
+_rope_tensor = struct.Struct("=7q")  # laya_rope_tensor: seven 64-bit fields
 
 
 _bound = False
@@ -52,7 +50,7 @@ def lib():
     if not _bound:
         vp, i64, sc = ctypes.c_void_p, ctypes.c_int64, ctypes.POINTER(_CRopeScaling)
         L.laya_rope_freqs.argtypes = [ctypes.c_double, ctypes.c_int, sc, _f64p, ctypes.POINTER(ctypes.c_float)]
-        L.laya_rope.argtypes = [ctypes.c_int, ctypes.POINTER(_CRopeSpec), ctypes.POINTER(_CRopeTensor), ctypes.c_int,
+        L.laya_rope.argtypes = [ctypes.c_int, vp, ctypes.c_char_p, ctypes.c_int,
                                 i64, vp, i64, vp]
         L.laya_set_rope_scaling.argtypes = [vp, sc, sc]
         ci, i32p, i64p = ctypes.c_int, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(i64)
@@ -107,9 +105,10 @@ class RopeSpec:
         if self.freqs.size != max(rot, 0) // 2:
             raise ValueError(f"RopeSpec: {self.freqs.size} frequencies for rot {rot}")
         self._c = _CRopeSpec(type, layout, 1 if inverse else 0, dim, rot, mscale, self.freqs.ctypes.data_as(_f64p))
+        self._at = ctypes.addressof(self._c)
 
 
-@dataclass
+@dataclass(slots=True)
 class RopeTensor:
     """A [tokens, heads, dim] view at device address `x`, rotated into `out`."""
     x: int
@@ -124,10 +123,9 @@ class RopeTensor:
 def rope(spec: RopeSpec, tensors, tokens: int, pos: int = 0, pos0: int = 0, device: int = 0, stream: int = 0) -> None:
     """laya_rope: rotates 1 to 4 tensors (e.g. q and k) over the same tokens in
     one launch.  pos: device address of int32 [tokens], or 0 for pos0, pos0 + 1, ..."""
-    arr = (_CRopeTensor * max(1, len(tensors)))(*[_CRopeTensor(t.x or None, t.out or None, t.x_token, t.x_head,
-                                                               t.out_token, t.out_head, t.heads) for t in tensors])
-    _check(lib().laya_rope(device, ctypes.byref(spec._c), arr, len(tensors), tokens, pos or None, pos0,
-                           stream or None))
+    arr = b"".join([_rope_tensor.pack(t.x, t.out, t.x_token, t.x_head, t.out_token, t.out_head, t.heads)
+                    for t in tensors])
+    _check(lib().laya_rope(device, spec._at, arr, len(tensors), tokens, pos or None, pos0, stream or None))
 
 
 def set_rope_scaling(engine: Engine, full: RopeScaling | None = None, sliding: RopeScaling | None = None) -> None:
