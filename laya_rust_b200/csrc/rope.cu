@@ -11,13 +11,15 @@
 // as an integer, so the f32 sine and cosine see a reduced argument whose
 // conversion rounds relative to itself.
 //
-// Bound by memory: every element is read and written once.  A thread owns one
-// 16-byte piece of a head (for the half layout the piece and its partner
-// rot / 2 further), computes the sines and cosines of its pairs once, and
-// turns the same piece of several heads with them, so the angles cost little
-// beside the copies.
+// Bound by memory: every element is read and written once.  A block takes a few
+// tokens and all their heads (up to 256 pieces of 16 bytes times 4 heads), so
+// a sine and cosine is computed once for all heads and passed through shared
+// memory, and a thread turns one piece (for the half layout the piece and its
+// partner rot / 2 further) of up to 4 heads, all loaded before the angles are
+// computed.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "common.cuh"
@@ -45,7 +47,8 @@ struct RopeArgs {
   RopeTensorArg t[kMaxTensors];
   int count;
   int dim, rot;
-  int heads_per_thread;
+  int heads_per_thread, groups;       // groups: of heads, over all tensors
+  int block_tokens, block_groups;
   long long tokens;
   const int* pos;
   long long pos0;
@@ -84,83 +87,198 @@ __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v);
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 
-// V elements moved as one access of sizeof(T) * V bytes.
+// V elements moved as one access of sizeof(T) * V bytes: 32-bit words, or one
+// 16-bit element.
 template <class T, int V>
 struct alignas(sizeof(T) * V) Vec {
-  T v[V];
+  using Word = std::conditional_t<(sizeof(T) * V >= 4), uint32_t, T>;
+  static constexpr int kWords = sizeof(T) * V >= 4 ? sizeof(T) * V / 4 : 1;
+  Word w[kWords];
 };
 
-constexpr int kHeadsAtOnce = 4;  // loads in flight a thread
+// The two elements of a word, and back (one rounding each).
+template <class T>
+__device__ __forceinline__ float2 unpack(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
-// VEC elements a piece; rot / 2 (half) or rot (interleaved), dim - rot, every
-// stride and address are multiples of it.
+constexpr int kThreads = 256;
+constexpr int kBlocksPerSm = 3;              // at most 80 registers a thread
+constexpr int kMaxHeads = 4;                 // heads a thread turns, all loaded before the first is turned
+
+// (a c - b s, b c + a s), a pair of pairs an instruction (packed f32 pairs, each
+// rounded as the scalar operation).
+__device__ __forceinline__ void turn2(uint64_t a, uint64_t b, uint64_t c, uint64_t s, float (&x)[2], float (&y)[2]) {
+  f2_get(f2_sub(f2_mul(a, c), f2_mul(b, s)), x[0], x[1]);
+  f2_get(f2_fma(a, s, f2_mul(b, c)), y[0], y[1]);
+}
+
+// Turns the pairs across two pieces (half layout): pair j is (p[j], q[j]).
+template <class T, int VEC>
+__device__ __forceinline__ void turn_across(Vec<T, VEC>& p, Vec<T, VEC>& q, const float (&c)[VEC], const float (&s)[VEC]) {
+  if constexpr (VEC == 1) {
+    const T* pe = reinterpret_cast<const T*>(p.w);
+    const T* qe = reinterpret_cast<const T*>(q.w);
+    const float v0 = to_f32(*pe), v1 = to_f32(*qe);
+    *reinterpret_cast<T*>(p.w) = from_f32<T>(v0 * c[0] - v1 * s[0]);
+    *reinterpret_cast<T*>(q.w) = from_f32<T>(v1 * c[0] + v0 * s[0]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      float x[2], y[2];
+      turn2(f2(__uint_as_float(p.w[j]), __uint_as_float(p.w[j + 1])), f2(__uint_as_float(q.w[j]), __uint_as_float(q.w[j + 1])),
+            f2(c[j], c[j + 1]), f2(s[j], s[j + 1]), x, y);
+      p.w[j] = __float_as_uint(x[0]);
+      p.w[j + 1] = __float_as_uint(x[1]);
+      q.w[j] = __float_as_uint(y[0]);
+      q.w[j + 1] = __float_as_uint(y[1]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) {
+      const float2 a = unpack<T>(p.w[j]), b = unpack<T>(q.w[j]);
+      float x[2], y[2];
+      turn2(f2(a.x, a.y), f2(b.x, b.y), f2(c[2 * j], c[2 * j + 1]), f2(s[2 * j], s[2 * j + 1]), x, y);
+      p.w[j] = pack<T>(x[0], x[1]);
+      q.w[j] = pack<T>(y[0], y[1]);
+    }
+  }
+}
+
+// Turns the neighbours within one piece (interleaved layout).
+template <class T, int VEC>
+__device__ __forceinline__ void turn_within(Vec<T, VEC>& p, const float (&c)[VEC / 2], const float (&s)[VEC / 2]) {
+#pragma unroll
+  for (int j = 0; j < VEC / 2; ++j) {
+    float2 v;
+    if constexpr (sizeof(T) == 4)
+      v = make_float2(__uint_as_float(p.w[2 * j]), __uint_as_float(p.w[2 * j + 1]));
+    else
+      v = unpack<T>(p.w[j]);
+    const float x = v.x * c[j] - v.y * s[j], y = v.y * c[j] + v.x * s[j];
+    if constexpr (sizeof(T) == 4) {
+      p.w[2 * j] = __float_as_uint(x);
+      p.w[2 * j + 1] = __float_as_uint(y);
+    } else {
+      p.w[j] = pack<T>(x, y);
+    }
+  }
+}
+
+// A block turns tiles of a.block_tokens tokens by a.block_groups groups of
+// heads, one tile after another; a thread keeps its place in the tile (piece,
+// then group, then token), so its index arithmetic is done once.  The angles of
+// the next tile go to the other half of the shared buffer while this tile's
+// loads are in flight.  Pieces of VEC elements: rot / 2 (half) or rot
+// (interleaved), dim - rot, every stride and address are multiples of VEC.
 template <class T, int VEC, bool HALF>
-__global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __grid_constant__ RopeArgs a) {
   using P = Vec<T, VEC>;
   constexpr int kPairs = HALF ? VEC : (VEC + 1) / 2;
   constexpr int kPieces = HALF || VEC == 1 ? 2 : 1;  // pieces a unit turns
-  const int turned = HALF ? a.rot / 2 / VEC : a.rot / (kPieces * VEC);
+  extern __shared__ __align__(16) float angles[];    // [2][cos | sin][block_tokens * half]
+  const int half = a.rot / 2;
+  const int turned = half / kPairs;
   const int units = turned + (a.dim - a.rot) / VEC;
+  const int block_units = min(units, kThreads);  // heads of more pieces: grid.z parts of them
+  const int per_tok = a.block_groups * block_units;
+  const int n_angles = a.block_tokens * half;
+  const long long tiles = (a.tokens + a.block_tokens - 1) / a.block_tokens;
+
+  // this thread's place (a tile has at most kThreads of them)
+  const int tl = static_cast<int>(threadIdx.x) / per_tok, gu = static_cast<int>(threadIdx.x) - tl * per_tok;
+  const int group = static_cast<int>(blockIdx.y) * a.block_groups + gu / block_units;
+  const int u = static_cast<int>(blockIdx.z) * block_units + gu % block_units;
   int ti = 0;
-  while (ti + 1 < a.count && static_cast<int>(blockIdx.y) >= a.t[ti + 1].group0) ++ti;
-  const RopeTensorArg& t = a.t[ti];
-  const int h0 = (static_cast<int>(blockIdx.y) - t.group0) * a.heads_per_thread;
-  const int h1 = min(t.heads, h0 + a.heads_per_thread);
-  const long long n = a.tokens * units;
-  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n;
-       i += static_cast<long long>(gridDim.x) * 256) {
-    const long long tok = n < (1ll << 31) ? static_cast<int>(i) / units : i / units;
-    const int u = static_cast<int>(i - tok * units);
-    const T* x = static_cast<const T*>(t.x) + tok * t.x_token;
-    T* o = static_cast<T*>(t.out) + tok * t.out_token;
-    if (u >= turned) {
-      if (t.x == t.out) continue;
-      const int at = a.rot + (u - turned) * VEC;
-      for (int h = h0; h < h1; h += kHeadsAtOnce) {
-        P p[kHeadsAtOnce];
-#pragma unroll
-        for (int k = 0; k < kHeadsAtOnce; ++k)
-          if (h + k < h1) p[k] = *reinterpret_cast<const P*>(x + (h + k) * t.x_head + at);
-#pragma unroll
-        for (int k = 0; k < kHeadsAtOnce; ++k)
-          if (h + k < h1) *reinterpret_cast<P*>(o + (h + k) * t.out_head + at) = p[k];
+  while (ti + 1 < a.count && group >= a.t[ti + 1].group0) ++ti;
+  const RopeTensorArg t = a.t[ti];
+  const int h0 = (group - t.group0) * a.heads_per_thread;
+  const bool turn = u < turned;
+  int nh = tl < a.block_tokens && group < a.groups && u < units ? min(a.heads_per_thread, t.heads - h0) : 0;
+  if (!turn && t.x == t.out) nh = 0;
+  const int at0 = turn ? (HALF ? u * VEC : u * kPieces * VEC) : a.rot + (u - turned) * VEC;
+  const int at1 = HALF ? half + u * VEC : at0 + VEC;
+  const T* const x0 = static_cast<const T*>(t.x) + h0 * t.x_head;
+  T* const o0 = static_cast<T*>(t.out) + h0 * t.out_head;
+  // the first of the angles it computes
+  const int my_at = static_cast<int>(threadIdx.x) / half, my_j = static_cast<int>(threadIdx.x) - my_at * half;
+
+  auto compute_angles = [&](long long tile, float* buf) {
+    int at = my_at, j = my_j;
+    for (int i = threadIdx.x; i < n_angles; i += kThreads) {
+      const long long tok = tile * a.block_tokens + at;
+      if (tok < a.tokens) {
+        const long long pos = a.pos ? __ldg(a.pos + tok) : a.pos0 + tok;
+        float c, s;
+        rope_angle(a.turns[j], pos, c, s);
+        buf[i] = c * a.mscale;
+        buf[n_angles + i] = s * (a.mscale * a.sign);
       }
-      continue;
+      if (i + kThreads < n_angles) {
+        at = (i + kThreads) / half;
+        j = i + kThreads - at * half;
+      }
     }
-    const long long p0 = a.pos ? __ldg(a.pos + tok) : a.pos0 + tok;
-    float c[kPairs], s[kPairs];
+  };
+
+  long long tile = blockIdx.x;
+  if (tile < tiles) compute_angles(tile, angles);
+  int parity = 0;
+  for (; tile < tiles; tile += gridDim.x, parity ^= 1) {
+    const long long tok = tile * a.block_tokens + tl;
+    const int n = tok < a.tokens ? nh : 0;
+    const T* x = x0 + tok * t.x_token;
+    T* o = o0 + tok * t.out_token;
+    P p[kMaxHeads], q[kMaxHeads];
 #pragma unroll
-    for (int j = 0; j < kPairs; ++j) {
-      rope_angle(a.turns[u * kPairs + j], p0, c[j], s[j]);
-      c[j] *= a.mscale;
-      s[j] *= a.mscale * a.sign;
+    for (int k = 0; k < kMaxHeads; ++k)
+      if (k < n) {
+        p[k] = *reinterpret_cast<const P*>(x + k * t.x_head + at0);
+        if (kPieces == 2 && turn) q[k] = *reinterpret_cast<const P*>(x + k * t.x_head + at1);
+      }
+    __syncthreads();  // this tile's angles are there; the other buffer was read
+    if (tile + gridDim.x < tiles) compute_angles(tile + gridDim.x, angles + (parity ^ 1) * 2 * n_angles);
+    if (n <= 0) continue;
+    if (turn) {
+      float c[kPairs], s[kPairs];
+      const float* cs = angles + parity * 2 * n_angles + tl * half + u * kPairs;
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        c[j] = cs[j];
+        s[j] = cs[n_angles + j];
+      }
+#pragma unroll
+      for (int k = 0; k < kMaxHeads; ++k) {
+        if constexpr (kPieces == 2)
+          turn_across<T, VEC>(p[k], q[k], c, s);
+        else
+          turn_within<T, VEC>(p[k], c, s);
+      }
     }
-    // where the unit's pieces start: pairs are (first[j], second[j]) across
-    // two pieces, or neighbours within one
-    const int at0 = HALF ? u * VEC : u * kPieces * VEC, at1 = HALF ? a.rot / 2 + u * VEC : at0 + VEC;
-    for (int h = h0; h < h1; h += kHeadsAtOnce) {
-      P p[kHeadsAtOnce], q[kHeadsAtOnce];
 #pragma unroll
-      for (int k = 0; k < kHeadsAtOnce; ++k)
-        if (h + k < h1) {
-          p[k] = *reinterpret_cast<const P*>(x + (h + k) * t.x_head + at0);
-          if (kPieces == 2) q[k] = *reinterpret_cast<const P*>(x + (h + k) * t.x_head + at1);
-        }
-#pragma unroll
-      for (int k = 0; k < kHeadsAtOnce; ++k)
-        if (h + k < h1) {
-#pragma unroll
-          for (int j = 0; j < kPairs; ++j) {
-            T& e0 = kPieces == 2 ? p[k].v[j] : p[k].v[(2 * j) % VEC];
-            T& e1 = kPieces == 2 ? q[k].v[j] : p[k].v[(2 * j + 1) % VEC];
-            const float v0 = to_f32(e0), v1 = to_f32(e1);
-            e0 = from_f32<T>(v0 * c[j] - v1 * s[j]);
-            e1 = from_f32<T>(v1 * c[j] + v0 * s[j]);
-          }
-          *reinterpret_cast<P*>(o + (h + k) * t.out_head + at0) = p[k];
-          if (kPieces == 2) *reinterpret_cast<P*>(o + (h + k) * t.out_head + at1) = q[k];
-        }
-    }
+    for (int k = 0; k < kMaxHeads; ++k)
+      if (k < n) {
+        *reinterpret_cast<P*>(o + k * t.out_head + at0) = p[k];
+        if (kPieces == 2 && turn) *reinterpret_cast<P*>(o + k * t.out_head + at1) = q[k];
+      }
   }
 }
 
@@ -183,10 +301,11 @@ __global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__
 
 template <class T, int VEC>
 cudaError_t launch_vec(const RopeArgs& a, bool half, dim3 grid, cudaStream_t st) {
+  const size_t smem = 4 * sizeof(float) * a.block_tokens * (a.rot / 2);
   if (half)
-    rope_kernel<T, VEC, true><<<grid, 256, 0, st>>>(a);
+    rope_kernel<T, VEC, true><<<grid, kThreads, smem, st>>>(a);
   else
-    rope_kernel<T, VEC, false><<<grid, 256, 0, st>>>(a);
+    rope_kernel<T, VEC, false><<<grid, kThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -208,19 +327,26 @@ cudaError_t launch_rope(RopeArgs& a, bool half, int num_sms, cudaStream_t st) {
   int v = kMaxVec;
   while (v > 1 && !pieces_fit(a, half, es, v)) v /= 2;
   const int units = (half ? a.rot / 2 / v : v == 1 ? a.rot / 2 : a.rot / v) + (a.dim - a.rot) / v;
-  const long long n = a.tokens * units;
-  // heads a thread: as many as 8, while there are still two full waves of threads
+  // heads a thread: 4, fewer while the call would not fill the SMs
   int heads = 0;
   for (int i = 0; i < a.count; ++i) heads += a.t[i].heads;
-  a.heads_per_thread = 8;
-  while (a.heads_per_thread > 1 && n * heads < 2ll * 2048 * num_sms * a.heads_per_thread) a.heads_per_thread /= 2;
-  int groups = 0;
+  a.heads_per_thread = kMaxHeads;
+  while (a.heads_per_thread > 1 && a.tokens * units * heads < 1024ll * num_sms * a.heads_per_thread)
+    a.heads_per_thread /= 2;
+  a.groups = 0;
   for (int i = 0; i < a.count; ++i) {
-    a.t[i].group0 = groups;
-    groups += (a.t[i].heads + a.heads_per_thread - 1) / a.heads_per_thread;
+    a.t[i].group0 = a.groups;
+    a.groups += (a.t[i].heads + a.heads_per_thread - 1) / a.heads_per_thread;
   }
-  if (groups > 65535) return cudaErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>(std::min<long long>((n + 255) / 256, 1 << 22)), groups);
+  a.block_groups = std::min(a.groups, std::max(1, kThreads / units));
+  a.block_tokens = std::max(1, kThreads / (a.block_groups * units));
+  const unsigned gz = (units + kThreads - 1) / kThreads;
+  const unsigned gy = (a.groups + a.block_groups - 1) / a.block_groups;
+  if (gy > 65535) return cudaErrorInvalidValue;
+  // the resident blocks, each walking over its share of the tiles
+  const long long tiles = (a.tokens + a.block_tokens - 1) / a.block_tokens;
+  const long long want = std::max<long long>(1, static_cast<long long>(kBlocksPerSm) * num_sms / (gy * gz));
+  const dim3 grid(static_cast<unsigned>(std::min(tiles, want)), gy, gz);
   switch (v) {
     case 8: return launch_vec<T, kMaxVec>(a, half, grid, st);
     case 4: return launch_vec<T, 4>(a, half, grid, st);

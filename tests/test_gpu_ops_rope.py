@@ -59,7 +59,7 @@ def stream():
 @pytest.mark.parametrize("layout", [ops.ROPE_HALF, ops.ROPE_INTERLEAVED])
 @pytest.mark.parametrize("tokens,heads,dim,rot", [(1, 1, 64, 64), (1, 32, 64, 64), (5, 3, 64, 32), (33, 16, 64, 64),
                                                   (7, 2, 80, 20), (9, 5, 18, 6), (3, 1, 2, 2), (300, 12, 128, 128),
-                                                  (2, 3, 512, 512), (17, 4, 96, 48), (130, 40, 128, 64), (11, 7, 37, 36)])
+                                                  (2, 3, 512, 512), (17, 4, 96, 48), (3, 2, 511, 2), (40, 2, 510, 300), (1000, 40, 256, 256), (700, 70, 64, 64), (130, 40, 128, 64), (11, 7, 37, 36)])
 def test_against_64_bits(type, layout, tokens, heads, dim, rot):
     g = torch.Generator(device="cuda").manual_seed(tokens * 1000 + dim + rot)
     x = torch.randn(tokens, heads, dim, generator=g, device="cuda").to(DT[type])
