@@ -125,6 +125,11 @@ __global__ void __launch_bounds__(128, 1)
   grid_dep_trigger();
 
   if (warp == 0) {
+    // lane i holds entry i's row of A
+    const int a_row = lane < n ? __ldg(a.item_chunk + item.y + lane) * kLoraChunk : 0;
+    int a_rows[kLoraMaxGroup];
+#pragma unroll
+    for (int i = 0; i < kLoraMaxGroup; ++i) a_rows[i] = __shfl_sync(0xffffffffu, a_row, i);
     if (lane == 0) {
       bool ok = true;
       int stage = 0;
@@ -137,9 +142,9 @@ __global__ void __launch_bounds__(128, 1)
         uint8_t* sx = smem + stage * stage_bytes;
         mbar_arrive_expect_tx(&full[stage], kXBytes + n * kABytes);
         tma_load_2d(sx, &tmX, kb * 64, item.x * kLoraItemRows, &full[stage]);
-        for (int i = 0; i < n; ++i)
-          tma_load_2d(sx + kXBytes + i * kABytes, &tmA, kb * 64,
-                      __ldg(a.entry_chunk + __ldg(a.item_entry + item.y + i)) * kLoraChunk, &full[stage]);
+#pragma unroll
+        for (int i = 0; i < kLoraMaxGroup; ++i)
+          if (i < n) tma_load_2d(sx + kXBytes + i * kABytes, &tmA, kb * 64, a_rows[i], &full[stage]);
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
@@ -205,8 +210,8 @@ __global__ void __launch_bounds__(128, 1)
     const int slot = __ldg(a.entry_chunk + e0) / a.chunks_per_slot;
     const float scale = __ldg(a.scale + slot);
     for (int i = threadIdx.x % splits; i < n; i += splits) {
+      if (__ldg(a.item_chunk + item.y + i) / a.chunks_per_slot != slot) continue;
       const int e = __ldg(a.item_entry + item.y + i);
-      if (__ldg(a.entry_chunk + e) / a.chunks_per_slot != slot) continue;
       T hi[16], lo[16];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -235,6 +240,55 @@ __global__ void __launch_bounds__(128, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+// u = scale (x A^T) for one (row, chunk) pair a block: a warp takes two of the
+// chunk's 16 rows of A over all of K, so no sum leaves its warp.
+template <class T>
+__global__ void __launch_bounds__(256) lora_pairs_kernel(const LoraPairsArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 p = __ldg(a.pair + blockIdx.x);
+  grid_dep_wait();
+  grid_dep_trigger();
+  const float scale = __ldg(a.scale + p.w);
+  const T* x = static_cast<const T*>(a.x) + p.x * a.ldx;
+  const T* A0 = static_cast<const T*>(a.a) + (static_cast<size_t>(p.z) * kLoraChunk + 2 * warp) * a.in_pad;
+  const T* A1 = A0 + a.in_pad;
+  float s0 = 0.0f, s1 = 0.0f;
+  const int whole = a.in & ~7;  // the rest of a row of x may hold anything
+#pragma unroll 4
+  for (int k = 8 * lane; k < whole; k += 256) {
+    const uint4 xv = *reinterpret_cast<const uint4*>(x + k);
+    const uint4 av = __ldg(reinterpret_cast<const uint4*>(A0 + k)), bv = __ldg(reinterpret_cast<const uint4*>(A1 + k));
+    const T* xe = reinterpret_cast<const T*>(&xv);
+    const T* ae = reinterpret_cast<const T*>(&av);
+    const T* be = reinterpret_cast<const T*>(&bv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = Num<T>::up(xe[j]);
+      s0 += v * Num<T>::up(ae[j]);
+      s1 += v * Num<T>::up(be[j]);
+    }
+  }
+  if (lane < a.in - whole) {
+    const float v = Num<T>::up(x[whole + lane]);
+    s0 += v * Num<T>::up(A0[whole + lane]);
+    s1 += v * Num<T>::up(A1[whole + lane]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+  }
+  if (lane == 0) {
+    T hi[2], lo[2];
+    split_value<T>(s0 * scale, hi[0], lo[0]);
+    split_value<T>(s1 * scale, hi[1], lo[1]);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.u) + static_cast<size_t>(p.y) * kLoraEntryElems +
+                                                static_cast<size_t>(p.x % kLoraBlock) * 2 * kLoraChunk + 2 * warp);
+    dst[0] = *reinterpret_cast<uint32_t*>(hi);
+    dst[kLoraChunk / 2] = *reinterpret_cast<uint32_t*>(lo);
   }
 }
 
@@ -279,6 +333,14 @@ cudaError_t launch_lora_shrink(const CUtensorMap& x, const CUtensorMap& a_map, c
   while (splits < 8 && 2 * splits * a.items <= num_sms && 4 * splits <= a.num_kb) splits *= 2;
   return a.bf16 ? launch_shrink<__nv_bfloat16>(x, a_map, a, splits, pdl, s)
                 : launch_shrink<__half>(x, a_map, a, splits, pdl, s);
+}
+
+cudaError_t launch_lora_pairs(const LoraPairsArgs& a, bool pdl, cudaStream_t s) {
+  if (a.pairs <= 0) return cudaSuccess;
+  auto* kernel = a.bf16 ? &lora_pairs_kernel<__nv_bfloat16> : &lora_pairs_kernel<__half>;
+  if (pdl) return launch_pdl(kernel, dim3(a.pairs), dim3(256), 0, s, nullptr, 0, a);
+  kernel<<<a.pairs, 256, 0, s>>>(a);
+  return cudaGetLastError();
 }
 
 LoraItems lora_items(const LoraLayout& L, int num_sms) {
@@ -407,9 +469,13 @@ struct Plan {
   LoraLayout lay;
   std::vector<std::pair<int, int>> used;  // (slot, chunks)
   Buf dev, u;
+  bool small = false;  // lora_small.cu, not the GEMM
   int items = 0, group = 0;
   const int4* d_item = nullptr;
   const int* d_item_entry = nullptr;
+  const int* d_item_chunk = nullptr;
+  const int4* d_pair = nullptr;
+  int pairs = 0;  // > 0: the rank-space product goes by pairs, not items
   const int* d_row_entry = nullptr;
   const int* d_entry_chunk = nullptr;
   const int* d_off = nullptr;
@@ -454,6 +520,12 @@ uint16_t store_host(float v, bool bf16) {
   }
   return b;
 }
+
+// Few (row, chunk) pairs take a block each, reading 16 rows of A from L2.
+constexpr size_t kLoraMaxPairs = 512;
+
+// The rows lora_small.cu takes.
+bool lora_use_small(int rows) { return rows >= 1 && rows <= kLoraBlock; }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -582,15 +654,34 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     std::sort(q.used.begin(), q.used.end());
     q.used.erase(std::unique(q.used.begin(), q.used.end()), q.used.end());
     DeviceScope scope(k.device);
-    const LoraItems it = lora_items(L, k.num_sms);
+    // few (row, chunk) pairs: one block each; else items of 128 rows
+    std::vector<int4> pair;
+    for (int m = 0; m < L.rows && pair.size() <= kLoraMaxPairs; ++m) {
+      const int e0 = L.row_entry[m];
+      if (e0 < 0) continue;
+      for (int e = e0; e < static_cast<int>(L.chunk.size()) && (e == e0 || L.chunk[e].y > 0); ++e)
+        pair.push_back(make_int4(m, e, entry_chunk[e], L.chunk[e].x));
+    }
+    LoraItems it;
+    if (pair.size() <= kLoraMaxPairs) {
+      q.pairs = static_cast<int>(pair.size());
+    } else {
+      pair.clear();
+      it = lora_items(L, k.num_sms);
+    }
+    std::vector<int> item_chunk;
+    for (int e : it.entry) item_chunk.push_back(entry_chunk[e]);
     q.items = static_cast<int>(it.item.size());
     q.group = it.group;
-    // [error word | off | row entries | entry chunks | items | their entries],
-    // each 256-byte aligned
+    // [error word | off | row entries | entry chunks | items | their entries |
+    // their chunks | pairs], each 256-byte aligned
     auto up = [](size_t v) { return (v + 63) / 64 * 64; };
     const size_t o_off = 64, o_row = o_off + up(L.off.size()), o_ent = o_row + up(L.row_entry.size());
     const size_t o_item = o_ent + up(entry_chunk.size()), o_ie = o_item + up(4 * it.item.size());
-    std::vector<int> h(o_ie + up(it.entry.size()));
+    const size_t o_ic = o_ie + up(it.entry.size()), o_pair = o_ic + up(item_chunk.size());
+    std::vector<int> h(o_pair + up(4 * pair.size()));
+    if (!pair.empty()) memcpy(h.data() + o_pair, pair.data(), pair.size() * sizeof(int4));
+    std::copy(item_chunk.begin(), item_chunk.end(), h.begin() + o_ic);
     if (!it.item.empty()) memcpy(h.data() + o_item, it.item.data(), it.item.size() * sizeof(int4));
     std::copy(it.entry.begin(), it.entry.end(), h.begin() + o_ie);
     std::copy(L.off.begin(), L.off.end(), h.begin() + o_off);
@@ -599,7 +690,9 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     q.dev.alloc(h.size() * 4, "lora plan");
     const size_t entries = std::max<size_t>(1, L.chunk.size());
     q.u.alloc(entries * kLoraEntryElems * 2, "lora workspace");
-    if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock, 2 * kLoraChunk, kGemmABoxRows))
+    q.small = lora_use_small(L.rows);
+    if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock, 2 * kLoraChunk,
+                       q.small ? (L.rows + 15) / 16 * 16 : kGemmABoxRows))
       throw OpError(LAYA_E_CUDA, "lora_plan_create: tensor map encode failed");
     op_check(cudaMemcpyAsync(q.dev.p, h.data(), h.size() * 4, cudaMemcpyHostToDevice, k.stream), "lora plan upload");
     // rows of other adapters are zero in an entry, and stay zero: every run
@@ -612,6 +705,8 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     q.d_entry_chunk = q.dev.as<int>() + o_ent;
     q.d_item = reinterpret_cast<const int4*>(q.dev.as<int>() + o_item);
     q.d_item_entry = q.dev.as<int>() + o_ie;
+    q.d_item_chunk = q.dev.as<int>() + o_ic;
+    q.d_pair = reinterpret_cast<const int4*>(q.dev.as<int>() + o_pair);
     *plan = p.release();
   });
 }
@@ -638,20 +733,31 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     require_device_ptr(x, k.device, "lora_run: x");
     require_device_ptr(y, k.device, "lora_run: y");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // x W^T and u B^T in one accumulator.  256 x 128 tiles where 256 x 256 ones
-    // would fill at most half the clusters, as in the engine.
-    const int tiles = (q.lay.rows + kGemmBM - 1) / kGemmBM * (k.out_pad / kGemmBN);
-    const bool narrow = tiles * 2 <= k.num_sms / 2;
-    const int bn = narrow ? kGemmBNNarrow : kGemmBN;
+    const uint32_t xbox = q.small ? (q.lay.rows + 15) / 16 * 16 : kGemmABoxRows;
     CUtensorMap mx, mw, my;
-    if (make_tmap_pitched(&mx, x, k.bf16, q.lay.rows, k.in, ldx, kGemmABoxRows) ||
-        make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, bn / 2) ||
-        make_tmap_pitched(&my, y, k.bf16, q.lay.rows, std::max(k.out & ~7, 8), ldy, kGemmOutBoxRows))
+    if (make_tmap_pitched(&mx, x, k.bf16, q.lay.rows, k.in, ldx, xbox))
       throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
-    if (q.items > 0) {
+    if (q.pairs > 0) {
+      LoraPairsArgs s{};
+      s.pair = q.d_pair;
+      s.pairs = q.pairs;
+      s.x = x;
+      s.ldx = ldx;
+      s.a = k.a.p;
+      s.scale = k.scale.as<float>();
+      s.u = q.u.p;
+      s.in = k.in;
+      s.in_pad = k.in_pad;
+      s.bf16 = k.bf16;
+      op_check(launch_lora_pairs(s, false, st), "lora launch");
+    } else if (q.items > 0) {
+      CUtensorMap mxi = mx;
+      if (xbox != kLoraItemRows && make_tmap_pitched(&mxi, x, k.bf16, q.lay.rows, k.in, ldx, kLoraItemRows))
+        throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
       LoraShrinkArgs s{};
       s.item = q.d_item;
       s.item_entry = q.d_item_entry;
+      s.item_chunk = q.d_item_chunk;
       s.items = q.items;
       s.group = q.group;
       s.row_entry = q.d_row_entry;
@@ -663,8 +769,37 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       s.chunks_per_slot = k.cps;
       s.bf16 = k.bf16;
       s.err = q.d_err;
-      op_check(launch_lora_shrink(mx, k.a_map, s, k.num_sms, false, st), "lora launch");
+      op_check(launch_lora_shrink(mxi, k.a_map, s, k.num_sms, false, st), "lora launch");
     }
+    // x W^T and u B^T in one accumulator
+    const bool early = q.pairs > 0 || q.items > 0;
+    if (q.small) {
+      if (make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, 128))
+        throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
+      LoraSmallArgs g{};
+      g.entry_chunk = q.d_entry_chunk;
+      g.entries = static_cast<int>(q.lay.chunk.size());
+      g.b_rows = k.out_pad;
+      g.bias = k.bias;
+      g.y = y;
+      g.ldy = ldy;
+      g.rows = q.lay.rows;
+      g.out = k.out;
+      g.num_kb = k.in_pad / 64;
+      g.bf16 = k.bf16;
+      g.early = early;
+      g.err = q.d_err;
+      op_check(launch_lora_small(mx, mw, q.u_map, k.b_map[0], g, k.num_sms, st), "lora launch");
+      return;
+    }
+    // 256 x 128 tiles where 256 x 256 ones would fill at most half the
+    // clusters, as in the engine
+    const int tiles = (q.lay.rows + kGemmBM - 1) / kGemmBM * (k.out_pad / kGemmBN);
+    const bool narrow = tiles * 2 <= k.num_sms / 2;
+    const int bn = narrow ? kGemmBNNarrow : kGemmBN;
+    if (make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, bn / 2) ||
+        make_tmap_pitched(&my, y, k.bf16, q.lay.rows, std::max(k.out & ~7, 8), ldy, kGemmOutBoxRows))
+      throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
     GemmArgs g{};
     g.M = q.lay.rows;
     g.N = (k.out + bn - 1) / bn * bn;
@@ -674,7 +809,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     g.ldo = static_cast<int>(ldy);
     g.bias = k.bias;
     g.n_valid = k.out;
-    const GemmExt ext{&q.u_map, &k.b_map[narrow], q.d_off, q.d_entry_chunk, k.out_pad, q.items > 0};
+    const GemmExt ext{&q.u_map, &k.b_map[narrow], q.d_off, q.d_entry_chunk, k.out_pad, early};
     op_check(launch_gemm(k.bf16 ? kEpiPlainBf16 : kEpiPlainF16, GemmMaps{&mx, &mw, &my}, g, k.num_sms, st, bn, &ext),
              "lora launch");
   });

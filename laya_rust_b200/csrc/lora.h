@@ -53,6 +53,7 @@ LoraItems lora_items(const LoraLayout& L, int num_sms);
 struct LoraShrinkArgs {
   const int4* item;
   const int* item_entry;
+  const int* item_chunk;  // the entries' chunks in the bank, same order
   int items, group;
   const int* row_entry;   // [rows]
   const int* entry_chunk; // [entries]: chunk in the bank
@@ -67,5 +68,38 @@ struct LoraShrinkArgs {
 // x: box 64 x 128, A (make_tmap_pitched, [chunks * 16, in_pad]): box 64 x 16.
 cudaError_t launch_lora_shrink(const CUtensorMap& x, const CUtensorMap& a_map, const LoraShrinkArgs& a, int num_sms,
                                bool pdl, cudaStream_t s);
+
+// The same for few (row, chunk) pairs: pair p is (row, entry, chunk in the
+// bank, slot).
+struct LoraPairsArgs {
+  const int4* pair;
+  int pairs;
+  const void* x;          // pitch ldx, 16-byte aligned
+  long long ldx;
+  const void* a;          // the bank's A
+  const float* scale;
+  void* u;
+  int in, in_pad;
+  bool bf16;
+};
+cudaError_t launch_lora_pairs(const LoraPairsArgs& a, bool pdl, cudaStream_t s);
+
+// The whole projection of at most kLoraBlock rows (one block, so entries
+// 0 .. entries - 1): lora_small.cu.  Maps: x [rows, in] box 64 x up16(rows), W
+// box 64 x 128, u box 16 x up16(rows), B box 16 x 128.
+struct LoraSmallArgs {
+  const int* entry_chunk;
+  int entries;
+  int b_rows;
+  const float* bias;
+  void* y;
+  long long ldy;
+  int rows, out, num_kb;
+  bool bf16;
+  int early;              // see GemmExt
+  int* err;
+};
+cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const CUtensorMap& b,
+                              const LoraSmallArgs& a, int num_sms, cudaStream_t s);
 
 }  // namespace laya
