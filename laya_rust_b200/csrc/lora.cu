@@ -692,7 +692,7 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     q.u.alloc(entries * kLoraEntryElems * 2, "lora workspace");
     q.small = lora_use_small(L.rows);
     if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock, 2 * kLoraChunk,
-                       q.small ? (L.rows + 15) / 16 * 16 : kGemmABoxRows))
+                       q.small ? lora_small_tile(L.rows) : kGemmABoxRows))
       throw OpError(LAYA_E_CUDA, "lora_plan_create: tensor map encode failed");
     op_check(cudaMemcpyAsync(q.dev.p, h.data(), h.size() * 4, cudaMemcpyHostToDevice, k.stream), "lora plan upload");
     // rows of other adapters are zero in an entry, and stay zero: every run
@@ -733,11 +733,15 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     require_device_ptr(x, k.device, "lora_run: x");
     require_device_ptr(y, k.device, "lora_run: y");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const uint32_t xbox = q.small ? (q.lay.rows + 15) / 16 * 16 : kGemmABoxRows;
+    const uint32_t xbox = q.small ? lora_small_tile(q.lay.rows) : kGemmABoxRows;
+    const int entries = static_cast<int>(q.lay.chunk.size());
+    const bool fused = q.small && entries >= 1 && entries <= kLoraMaxGroup;
     CUtensorMap mx, mw, my;
     if (make_tmap_pitched(&mx, x, k.bf16, q.lay.rows, k.in, ldx, xbox))
       throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
-    if (q.pairs > 0) {
+    if (fused) {
+      // u comes with the projection
+    } else if (q.pairs > 0) {
       LoraPairsArgs s{};
       s.pair = q.d_pair;
       s.pairs = q.pairs;
@@ -772,13 +776,17 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       op_check(launch_lora_shrink(mxi, k.a_map, s, k.num_sms, false, st), "lora launch");
     }
     // x W^T and u B^T in one accumulator
-    const bool early = q.pairs > 0 || q.items > 0;
+    const bool early = !fused && (q.pairs > 0 || q.items > 0);
     if (q.small) {
       if (make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, 128))
         throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
       LoraSmallArgs g{};
       g.entry_chunk = q.d_entry_chunk;
-      g.entries = static_cast<int>(q.lay.chunk.size());
+      g.row_entry = q.d_row_entry;
+      g.scale = k.scale.as<float>();
+      g.entries = entries;
+      for (int i = 0; fused && i < entries; ++i) g.chunk[i] = q.lay.chunk[i].x * k.cps + q.lay.chunk[i].y;
+      g.chunks_per_slot = k.cps;
       g.b_rows = k.out_pad;
       g.bias = k.bias;
       g.y = y;
@@ -789,7 +797,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       g.bf16 = k.bf16;
       g.early = early;
       g.err = q.d_err;
-      op_check(launch_lora_small(mx, mw, q.u_map, k.b_map[0], g, k.num_sms, st), "lora launch");
+      op_check(launch_lora_small(mx, mw, q.u_map, k.b_map[0], k.a_map, g, fused, k.num_sms, st), "lora launch");
       return;
     }
     // 256 x 128 tiles where 256 x 256 ones would fill at most half the

@@ -84,22 +84,30 @@ struct LoraPairsArgs {
 };
 cudaError_t launch_lora_pairs(const LoraPairsArgs& a, bool pdl, cudaStream_t s);
 
-// The whole projection of at most kLoraBlock rows (one block, so entries
-// 0 .. entries - 1): lora_small.cu.  Maps: x [rows, in] box 64 x up16(rows), W
-// box 64 x 128, u box 16 x up16(rows), B box 16 x 128.
+// The projection of at most kLoraBlock rows (one block, so entries
+// 0 .. entries - 1): lora_small.cu.  `fused` (1 to kLoraMaxGroup entries): it
+// computes u too, otherwise u is there, or comes from the launch before it
+// (early).  Maps: x [rows, in] box 64 x lora_small_tile(rows), W box 64 x 128, u
+// box 16 x lora_small_tile(rows), B box 16 x 128, A box 64 x 16.
 struct LoraSmallArgs {
   const int* entry_chunk;
+  const int* row_entry;
+  const float* scale;
   int entries;
+  int chunk[kLoraMaxGroup];  // fused: the entries' chunks in the bank
+  int chunks_per_slot;
   int b_rows;
   const float* bias;
   void* y;
   long long ldy;
   int rows, out, num_kb;
   bool bf16;
-  int early;              // see GemmExt
+  int early;              // see GemmExt; not with fused
   int* err;
 };
+// Rows a tile of the small projection: a multiple of 16, at most 64.
+int lora_small_tile(int rows);
 cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const CUtensorMap& b,
-                              const LoraSmallArgs& a, int num_sms, cudaStream_t s);
+                              const CUtensorMap& a_map, const LoraSmallArgs& a, bool fused, int num_sms, cudaStream_t s);
 
 }  // namespace laya

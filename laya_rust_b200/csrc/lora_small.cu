@@ -2,16 +2,23 @@
 //
 // With few rows the product is a stream of W: what counts is how many SMs read
 // it at once and how short the chain behind the loads is.  So W takes the M
-// side of the MMA (128 output columns a tile) and the rows of x the N side
-// (16..256, no padding beyond 16), and K is cut over a cluster of up to 8 CTAs,
-// each with a few k-blocks that are all in flight together: 3072 outputs are
-// 24 tiles x 8 parts.  The adapter entries are dealt out over the cluster the
-// same way.  D is transposed (TMEM lane = output column, TMEM column = row), so
-// a CTA writes its f32 part to shared memory as [row][128 columns]; the CTAs
-// then each add a share of the rows over the cluster in rank order
-// (distributed shared memory) and store them 16 bytes a thread.
+// side of the MMA (128 output columns a tile) and a tile of 16..64 rows of x
+// the N side (no padding beyond 16), and K is cut over a cluster of up to 8
+// CTAs, each with a few k-blocks that are all in flight together: 3072 outputs
+// are 24 tiles x 8 parts.  The adapter entries are dealt out over the cluster
+// the same way.  D is transposed (TMEM lane = output column, TMEM column =
+// row), so a CTA leaves its f32 sums in shared memory as [row][128 columns].
+// Each CTA owns a share of the rows: the others send it their sums of those rows
+// with one bulk copy each (shared memory to shared memory; plain stores or loads
+// through the cluster measured 4 us for 16 KB), and it adds them in rank order
+// and stores 16 bytes a thread.
 //
-// Measured (one B200, whole call as a graph, L2 cold): see lora_use_small.
+// With at most 8 entries (FUSED) the same launch computes u as well: the A rows
+// of the entries ride along the K loop as a second M = 128 operand against the
+// same x, the cluster adds those sums first, and each CTA turns the entries it
+// owns into the two 16-bit operands of the adapter step in its own shared
+// memory.  Every cluster repeats u for its rows (16 rows of A per entry from
+// L2), which costs less than a launch of its own.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -28,13 +35,24 @@ namespace {
 constexpr int kCols = 128;                    // output columns of a tile
 constexpr int kWBytes = kCols * 64 * 2;       // W operand of a k-block
 constexpr int kBBytes = kCols * 32;           // one entry's B operand
+constexpr int kABytes = kLoraChunk * 64 * 2;  // one entry's A operand of a k-block
 constexpr int kMaxStages = 8;
 constexpr int kThreads = 128;
-constexpr int kPartLd = kCols + 4;            // floats a row of the f32 part
-constexpr size_t kSmemLimit = 232448;
+constexpr int kMaxRows = 64;                  // rows a tile
+constexpr int kPartLd = kCols + 4;            // floats a row of the f32 parts
+constexpr int kPartULd = kLoraChunk + 4;      // and of the rank-space parts
+constexpr size_t kSmemLimit = 232448 - 1024;  // dynamic, beside the static barriers
 
 struct SmallMaps {
-  CUtensorMap x, w, u, b;
+  CUtensorMap x, w, u, b, a;
+};
+
+// What the launch decides.
+struct SmallShape {
+  int xrows;   // rows a tile (N of the MMA): 16..64
+  int stages;
+  int own;     // FUSED: most entries a CTA owns
+  int ring_bytes;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -42,18 +60,40 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float4 ld_cluster_f4(const float* p, uint32_t rank) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The address in CTA `rank`'s shared memory that `p` has in this CTA's.
+__device__ __forceinline__ uint32_t map_to_rank(const void* p, uint32_t rank) {
   uint32_t r;
-  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(r)
+  return r;
+}
+// Copies `bytes` (a multiple of 16) to shared memory of CTA `rank`, at the
+// address `dst` has there, counted on that CTA's `bar`.
+__device__ __forceinline__ void bulk_to_rank(const void* dst, uint64_t* bar, const void* src, uint32_t bytes, uint32_t rank) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   map_to_rank(dst, rank)),
+               "r"(smem_u32(src)), "r"(bytes), "r"(map_to_rank(bar, rank))
                : "memory");
-  return v;
+}
+
+// Eight consecutive floats of every CTA's part, added in rank order: this CTA's
+// own at `own`, those it was sent `step` floats apart from `in` (rank c at place
+// c, or c - 1 past its own rank).
+template <int SPLITS>
+__device__ __forceinline__ void sum_parts(const float* own, const float* in, int step, int rank, float (&v)[8]) {
+#pragma unroll
+  for (int c = 0; c < SPLITS; ++c) {
+    const float* p = c == rank ? own : in + (c < rank ? c : c - 1) * step;
+    const float4 s = *reinterpret_cast<const float4*>(p), t = *reinterpret_cast<const float4*>(p + 4);
+    if (c == 0) {
+      v[0] = s.x, v[1] = s.y, v[2] = s.z, v[3] = s.w;
+      v[4] = t.x, v[5] = t.y, v[6] = t.z, v[7] = t.w;
+    } else {
+      v[0] += s.x, v[1] += s.y, v[2] += s.z, v[3] += s.w;
+      v[4] += t.x, v[5] += t.y, v[6] += t.z, v[7] += t.w;
+    }
+  }
 }
 
 template <class T>
@@ -67,79 +107,131 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// (a, b) as packed values and packed remainders (0 where a value is not finite).
 template <class T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<T>(a, b);
+  float2 h;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    h = make_float2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u));
+  else
+    h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  lo = pack2<T>(isfinite(h.x) ? a - h.x : 0.0f, isfinite(h.y) ? b - h.y : 0.0f);
+}
+
+template <class T, int SPLITS, bool FUSED>
 __global__ void __launch_bounds__(kThreads)
-    lora_small_kernel(const __grid_constant__ SmallMaps maps, const LoraSmallArgs a, const int splits, const int stages) {
+    lora_small_kernel(const __grid_constant__ SmallMaps maps, const __grid_constant__ LoraSmallArgs a, const SmallShape sh) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, b_full, done2, in_full, in_u_full;
+  __shared__ int row_slot[kMaxRows];
+  __shared__ float row_scale[kMaxRows];
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(cluster_rank());
-  const int n0 = static_cast<int>(blockIdx.x) / splits * kCols;
-  const int xrows = (a.rows + 15) & ~15;              // N of the MMA
+  const int rank = SPLITS > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int n0 = static_cast<int>(blockIdx.x) / SPLITS * kCols;
+  const int xrows = sh.xrows, m0 = static_cast<int>(blockIdx.y) * xrows;
+  const int rows = min(xrows, a.rows - m0);
   const int x_bytes = xrows * 128, u_bytes = xrows * 32;
-  const int stage_bytes = kWBytes + ((x_bytes + 1023) & ~1023);
-  const int kb0 = rank * a.num_kb / splits, kb1 = (rank + 1) * a.num_kb / splits;
-  const int e0 = rank * a.entries / splits, e1 = (rank + 1) * a.entries / splits;
-  const uint32_t tmem_cols = xrows <= 32 ? 32 : xrows <= 64 ? 64 : xrows <= 128 ? 128 : 256;
-
+  const int a_bytes = FUSED ? a.entries * kABytes : 0;
+  const int stage_bytes = kWBytes + x_bytes + a_bytes;
+  const int kb0 = rank * a.num_kb / SPLITS, kb1 = (rank + 1) * a.num_kb / SPLITS;
+  const int e0 = rank * a.entries / SPLITS, e1 = (rank + 1) * a.entries / SPLITS;
+  const int need_cols = FUSED ? 2 * xrows : xrows;
+  const uint32_t tmem_cols = need_cols <= 32 ? 32 : need_cols <= 64 ? 64 : 128;
+  // [FUSED: owned B operands | owned u operands] [ring] [part] [parts sent here]
+  // [FUSED: rank-space part] [parts sent here]; apart from the ring, which this
+  // CTA may still be using when another one's sums arrive
+  uint8_t* own_b = smem;
+  uint8_t* own_u = own_b + sh.own * kBBytes;
+  uint8_t* ring = own_u + sh.own * 2 * u_bytes;
+  const int own_rows = xrows / SPLITS;                            // rows rank * own_rows ..
+  float* part = reinterpret_cast<float*>(ring + sh.ring_bytes);   // [xrows][kPartLd]
+  float* part_in = part + xrows * kPartLd;                        // [SPLITS - 1][own_rows][kPartLd]
+  float* part_u = part_in + (SPLITS - 1) * own_rows * kPartLd;    // [entries][xrows][kPartULd]
+  const int u_entry = xrows * kPartULd;
+  float* part_u_in = part_u + a.entries * u_entry;                // [SPLITS - 1][e1 - e0][xrows][kPartULd]
   if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) {
+    for (int s = 0; s < sh.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(&done, 1);
+    mbar_init(&b_full, 1);
+    mbar_init(&done2, 1);
+    mbar_init(&in_full, 1);
+    mbar_init(&in_u_full, 1);
     abort_word = 0;
     fence_mbar_init();
+    if (SPLITS > 1) {
+      mbar_arrive_expect_tx(&in_full, (SPLITS - 1) * own_rows * kPartLd * 4);
+      if (FUSED && e0 < e1) mbar_arrive_expect_tx(&in_u_full, (SPLITS - 1) * (e1 - e0) * u_entry * 4);
+    }
   }
   if (warp == 1) {
     tmem_alloc(&tmem_holder, tmem_cols);
     tmem_relinquish();
   }
+  __syncwarp();
+  if (SPLITS > 1) cluster_arrive();  // this CTA's shared memory exists
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_holder;
+  const uint32_t tmem = tmem_holder, tmem_u = tmem + xrows;
   if (!a.early) grid_dep_wait();
   grid_dep_trigger();
 
+  const uint32_t idesc = std::is_same<T, __nv_bfloat16>::value ? umma_idesc_bf16(kCols, xrows) : umma_idesc_f16(kCols, xrows);
   if (warp == 0) {
     if (lane == 0) {
       bool ok = true;
       int stage = 0;
       uint32_t phase = 0;
       auto next = [&]() {
-        if (++stage == stages) {
+        if (++stage == sh.stages) {
           stage = 0;
           phase ^= 1u;
         }
       };
-      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag);
         if (!ok) break;
-        uint8_t* sw = smem + stage * stage_bytes;
-        mbar_arrive_expect_tx(&full[stage], kWBytes + x_bytes);
+        uint8_t* sw = ring + stage * stage_bytes;
+        mbar_arrive_expect_tx(&full[stage], stage_bytes);
         tma_load_2d(sw, &maps.w, kb * 64, n0, &full[stage]);
-        tma_load_2d(sw + kWBytes, &maps.x, kb * 64, 0, &full[stage]);
+        tma_load_2d(sw + kWBytes, &maps.x, kb * 64, m0, &full[stage]);
+        if constexpr (FUSED) {
+#pragma unroll
+          for (int i = 0; i < kLoraMaxGroup; ++i)
+            if (i < a.entries)
+              tma_load_2d(sw + kWBytes + x_bytes + i * kABytes, &maps.a, kb * 64, a.chunk[i] * kLoraChunk, &full[stage]);
+        }
         next();
       }
-      if (e0 < e1 && ok) {
+      if constexpr (FUSED) {
+        if (e0 < e1 && ok) {
+          mbar_arrive_expect_tx(&b_full, (e1 - e0) * kBBytes);
+#pragma unroll
+          for (int i = 0; i < kLoraMaxGroup; ++i)
+            if (i >= e0 && i < e1) tma_load_2d(own_b + (i - e0) * kBBytes, &maps.b, 0, a.chunk[i] * a.b_rows + n0, &b_full);
+        }
+      } else if (e0 < e1 && ok) {
         int chunk = __ldg(a.entry_chunk + e0);
         grid_dep_wait();  // u is complete
         for (int e = e0; e < e1; e += 2) {
           const int n = min(2, e1 - e);
           ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag);
           if (!ok) break;
-          uint8_t* sb = smem + stage * stage_bytes;
+          uint8_t* sb = ring + stage * stage_bytes;
           mbar_arrive_expect_tx(&full[stage], n * (kBBytes + 2 * u_bytes));
           for (int i = 0; i < n; ++i) {
             uint8_t* su = sb + kWBytes + i * 2 * u_bytes;
             tma_load_2d(sb + i * kBBytes, &maps.b, 0, chunk * a.b_rows + n0, &full[stage]);
-            tma_load_2d(su, &maps.u, 0, (e + i) * kLoraBlock, &full[stage]);
-            tma_load_2d(su + u_bytes, &maps.u, 16, (e + i) * kLoraBlock, &full[stage]);
+            tma_load_2d(su, &maps.u, 0, (e + i) * kLoraBlock + m0, &full[stage]);
+            tma_load_2d(su + u_bytes, &maps.u, 16, (e + i) * kLoraBlock + m0, &full[stage]);
             if (e + i + 1 < e1) chunk = __ldg(a.entry_chunk + e + i + 1);
           }
           next();
@@ -154,78 +246,166 @@ __global__ void __launch_bounds__(kThreads)
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc =
-          std::is_same<T, __nv_bfloat16>::value ? umma_idesc_bf16(kCols, xrows) : umma_idesc_f16(kCols, xrows);
       bool ok = true;
       int stage = 0;
       uint32_t phase = 0;
       auto next = [&]() {
         umma_commit(&empty[stage]);
-        if (++stage == stages) {
+        if (++stage == sh.stages) {
           stage = 0;
           phase ^= 1u;
         }
       };
-      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         ok = mbar_wait_bounded(&full[stage], phase, a.err, kErrLoraWait, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t w_addr = smem_u32(smem + stage * stage_bytes), x_addr = w_addr + kWBytes;
+        const uint32_t w_addr = smem_u32(ring + stage * stage_bytes), x_addr = w_addr + kWBytes;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           umma_f16(tmem, umma_desc_sw128(w_addr + k * 32), umma_desc_sw128(x_addr + k * 32), idesc,
                    (kb != kb0 || k != 0) ? 1u : 0u);
-        next();
-      }
-      for (int e = e0; e < e1 && ok; e += 2) {
-        ok = mbar_wait_bounded(&full[stage], phase, a.err, kErrLoraWait, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t b_addr = smem_u32(smem + stage * stage_bytes);
-        for (int i = 0; i < min(2, e1 - e); ++i) {
-          const uint64_t db = umma_desc_sw32(b_addr + i * kBBytes);
-          const uint32_t su = b_addr + kWBytes + i * 2 * u_bytes;
-          umma_f16(tmem, db, umma_desc_sw32(su), idesc, 1u);
-          umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
+        if constexpr (FUSED) {
+          // 128 rows from the A operand on: past the entries' they are whatever
+          // follows in shared memory, and their sums are never read
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tmem_u, umma_desc_sw128(x_addr + x_bytes + k * 32), umma_desc_sw128(x_addr + k * 32), idesc,
+                     (kb != kb0 || k != 0) ? 1u : 0u);
         }
         next();
+      }
+      if constexpr (!FUSED) {
+        for (int e = e0; e < e1 && ok; e += 2) {
+          ok = mbar_wait_bounded(&full[stage], phase, a.err, kErrLoraWait, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t b_addr = smem_u32(ring + stage * stage_bytes);
+          for (int i = 0; i < min(2, e1 - e); ++i) {
+            const uint64_t db = umma_desc_sw32(b_addr + i * kBBytes);
+            const uint32_t su = b_addr + kWBytes + i * 2 * u_bytes;
+            umma_f16(tmem, db, umma_desc_sw32(su), idesc, 1u);
+            umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
+          }
+          next();
+        }
       }
       umma_commit(&done);
     }
     __syncwarp();
+  } else if (FUSED) {
+    // whose adapter each row has, while the other warps load and multiply
+    const int m = static_cast<int>(threadIdx.x) - 64;
+    if (m < xrows) {
+      const int re = m < rows ? __ldg(a.row_entry + m0 + m) : -1;
+      const int slot = re >= 0 ? __ldg(a.entry_chunk + re) / a.chunks_per_slot : -1;
+      row_slot[m] = slot;
+      row_scale[m] = slot >= 0 ? __ldg(a.scale + slot) : 0.0f;
+    }
   }
-  // this CTA's f32 part to shared memory (the ring is idle: every stage was
-  // consumed): thread = output column, 16 rows at a time
-  float* part = reinterpret_cast<float*>(smem);
+  const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
   bool ok = mbar_wait_bounded(&done, 0, a.err, kErrLoraWait, nullptr) && !*abort_flag;
   ok = __syncthreads_and(ok);
   tc_fence_after();
-  if (ok) {
-    for (int m = 0; m < xrows; m += 16) {
-      uint32_t v[16];
-      tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + m, v);
-      tmem_ld_wait();
+  if (SPLITS > 1) cluster_wait();  // every CTA of the cluster has started
+  if constexpr (FUSED) {
+    // thread = row of A
+    if (warp * 32 < a.entries * kLoraChunk) {
+      float* dst = part_u + (static_cast<int>(threadIdx.x) / kLoraChunk) * u_entry + threadIdx.x % kLoraChunk;
+      for (int m = 0; m < rows; m += 16) {
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(tmem_u + lane_base + m, v);
+        tmem_ld_wait();
+        if (static_cast<int>(threadIdx.x) < a.entries * kLoraChunk) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) part[(m + j) * kPartLd + threadIdx.x] = __uint_as_float(v[j]);
+          for (int j = 0; j < 16; ++j) dst[(m + j) * kPartULd] = __uint_as_float(v[j]);
+        }
+      }
     }
+    fence_proxy_async_smem();
+    __syncthreads();
+    if (SPLITS > 1) {
+      // each owner's entries, to the owner
+      const int to = static_cast<int>(threadIdx.x);
+      if (to < SPLITS && to != rank) {
+        const int f0 = to * a.entries / SPLITS, f1 = (to + 1) * a.entries / SPLITS;
+        if (f0 < f1)
+          bulk_to_rank(part_u_in + (rank < to ? rank : rank - 1) * (f1 - f0) * u_entry, &in_u_full, part_u + f0 * u_entry,
+                       (f1 - f0) * u_entry * 4, to);
+      }
+      if (e0 < e1 && !mbar_wait_bounded(&in_u_full, 0, a.err, kErrLoraWait, nullptr)) ok = false;
+    }
+    for (int e = e0; e < e1; ++e) {
+      // thread: half (8 of 16 rank values) of row threadIdx.x / 2
+      const int slot = a.chunk[e] / a.chunks_per_slot;
+      uint8_t* hi_op = own_u + (e - e0) * 2 * u_bytes;
+      const int m = static_cast<int>(threadIdx.x >> 1), h = threadIdx.x & 1;
+      if (m >= xrows) continue;
+      uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+      if (row_slot[m] == slot) {
+        float v[8];
+        sum_parts<SPLITS>(part_u + e * u_entry + m * kPartULd + 8 * h,
+                          part_u_in + (e - e0) * u_entry + m * kPartULd + 8 * h, (e1 - e0) * u_entry, rank, v);
+        const float scale = row_scale[m];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split2<T>(v[2 * j] * scale, v[2 * j + 1] * scale, hi[j], lo[j]);
+      }
+      // 32-byte swizzle: 16-byte piece h of row m at piece h ^ (m / 4 % 2)
+      const int at = m * 32 + ((h ^ ((m >> 2) & 1)) << 4);
+      *reinterpret_cast<uint4*>(hi_op + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(hi_op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    tc_fence_before();
+    fence_proxy_async_smem();
+    __syncthreads();
+    if (e0 < e1 && ok) {
+      if (threadIdx.x == 32) {
+        if (mbar_wait_bounded(&b_full, 0, a.err, kErrLoraWait, abort_flag)) {
+          tc_fence_after();
+          for (int i = 0; i < e1 - e0; ++i) {
+            const uint64_t db = umma_desc_sw32(smem_u32(own_b + i * kBBytes));
+            const uint32_t su = smem_u32(own_u + i * 2 * u_bytes);
+            umma_f16(tmem, db, umma_desc_sw32(su), idesc, 1u);
+            umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
+          }
+        }
+        umma_commit(&done2);
+      }
+      ok = mbar_wait_bounded(&done2, 0, a.err, kErrLoraWait, nullptr) && !*abort_flag;
+    }
+    ok = __syncthreads_and(ok);
+    tc_fence_after();
+  }
+  // thread = output column
+  for (int m = 0; m < rows; m += 16) {
+    uint32_t v[16];
+    tmem_ld_32x32b_x16(tmem + lane_base + m, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) part[(m + j) * kPartLd + threadIdx.x] = __uint_as_float(v[j]);
   }
   tc_fence_before();
-  if (splits > 1)
-    cluster_sync();
-  else
-    __syncthreads();
-  // rows rank, rank + splits, ...: 16 threads a row, 8 columns each
+  fence_proxy_async_smem();
+  __syncthreads();
+  if (SPLITS > 1) {
+    // each owner's rows, to the owner
+    const int to = static_cast<int>(threadIdx.x);
+    if (to < SPLITS && to != rank)
+      bulk_to_rank(part_in + (rank < to ? rank : rank - 1) * own_rows * kPartLd, &in_full, part + to * own_rows * kPartLd,
+                   own_rows * kPartLd * 4, to);
+    if (!mbar_wait_bounded(&in_full, 0, a.err, kErrLoraWait, nullptr)) ok = false;
+    __syncwarp();
+    cluster_arrive();  // what this CTA was sent has landed
+  }
+  // the owned rows: 16 threads a row, 8 columns each
   const int col = n0 + static_cast<int>(threadIdx.x & 15) * 8;
   const int left = a.out - col;  // columns of this thread that exist
-  for (int m = rank + static_cast<int>(threadIdx.x >> 4) * splits; m < a.rows && left > 0 && ok; m += 8 * splits) {
-    const float* p = part + m * kPartLd + (threadIdx.x & 15) * 8;
-    float4 s = ld_cluster_f4(p, 0), t = ld_cluster_f4(p + 4, 0);
-    for (int c = 1; c < splits; ++c) {
-      const float4 s1 = ld_cluster_f4(p, c), t1 = ld_cluster_f4(p + 4, c);
-      s.x += s1.x, s.y += s1.y, s.z += s1.z, s.w += s1.w;
-      t.x += t1.x, t.y += t1.y, t.z += t1.z, t.w += t1.w;
-    }
-    float v[8] = {s.x, s.y, s.z, s.w, t.x, t.y, t.z, t.w};
+  for (int i = static_cast<int>(threadIdx.x >> 4); i < own_rows && left > 0 && ok; i += 8) {
+    const int m = rank * own_rows + i;
+    if (m >= rows) break;
+    float v[8];
+    sum_parts<SPLITS>(part + m * kPartLd + (threadIdx.x & 15) * 8, part_in + i * kPartLd + (threadIdx.x & 15) * 8,
+                      own_rows * kPartLd, rank, v);
     if (a.bias) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -234,7 +414,7 @@ __global__ void __launch_bounds__(kThreads)
     uint32_t o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
-    uint16_t* dst = static_cast<uint16_t*>(a.y) + static_cast<size_t>(m) * a.ldy + col;
+    uint16_t* dst = static_cast<uint16_t*>(a.y) + static_cast<size_t>(m0 + m) * a.ldy + col;
     if (left >= 8) {
       *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
     } else {
@@ -243,62 +423,96 @@ __global__ void __launch_bounds__(kThreads)
         if (j < left) dst[j] = static_cast<uint16_t>(o[j / 2] >> (16 * (j & 1)));
     }
   }
-  grid_dep_wait();  // this grid does not complete before the one that computes u
-  if (splits > 1)
-    cluster_sync();  // no CTA leaves while another may still read its part
-  else
-    __syncthreads();
+  __syncwarp();
+  if constexpr (!FUSED) grid_dep_wait();  // this grid does not complete before the one that computes u
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, tmem_cols);
   }
+  __syncwarp();
+  if (SPLITS > 1) cluster_wait();  // no CTA leaves while a copy may still read its part
 }
 
-template <class T>
-cudaError_t launch(const SmallMaps& maps, const LoraSmallArgs& a, int splits, int stages, size_t smem, cudaStream_t s) {
+template <class T, int SPLITS, bool FUSED>
+cudaError_t launch(const SmallMaps& maps, const LoraSmallArgs& a, const SmallShape& sh, size_t smem, cudaStream_t s) {
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(lora_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(kSmemLimit - 1024));
+    e = cudaFuncSetAttribute(lora_small_kernel<T, SPLITS, FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(kSmemLimit));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.x = SPLITS;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  const dim3 grid((a.out + kCols - 1) / kCols * splits);
-  return launch_pdl(lora_small_kernel<T>, grid, dim3(kThreads), smem, s, attr, 1, maps, a, splits, stages);
+  const dim3 grid((a.out + kCols - 1) / kCols * SPLITS, (a.rows + sh.xrows - 1) / sh.xrows);
+  return launch_pdl(lora_small_kernel<T, SPLITS, FUSED>, grid, dim3(kThreads), smem, s, attr, 1, maps, a, sh);
+}
+
+template <class T, bool FUSED>
+cudaError_t launch_splits(int splits, const SmallMaps& maps, const LoraSmallArgs& a, const SmallShape& sh, size_t smem,
+                          cudaStream_t s) {
+  switch (splits) {
+    case 1: return launch<T, 1, FUSED>(maps, a, sh, smem, s);
+    case 2: return launch<T, 2, FUSED>(maps, a, sh, smem, s);
+    case 4: return launch<T, 4, FUSED>(maps, a, sh, smem, s);
+    default: return launch<T, 8, FUSED>(maps, a, sh, smem, s);
+  }
 }
 
 }  // namespace
 
+int lora_small_tile(int rows) {
+  // row tiles of at most 64, of equal size
+  const int tiles = (rows + kMaxRows - 1) / kMaxRows;
+  return ((rows + tiles - 1) / tiles + 15) / 16 * 16;
+}
+
 cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const CUtensorMap& b,
-                              const LoraSmallArgs& a, int num_sms, cudaStream_t s) {
+                              const CUtensorMap& a_map, const LoraSmallArgs& a, bool fused, int num_sms, cudaStream_t s) {
   if (a.rows <= 0) return cudaSuccess;
-  if (a.rows > kLoraBlock || a.num_kb < 1) return cudaErrorInvalidValue;
-  const int tiles = (a.out + kCols - 1) / kCols, xrows = (a.rows + 15) / 16 * 16;
+  if (a.rows > kLoraBlock || a.num_kb < 1 || (fused && (a.entries < 1 || a.entries > kLoraMaxGroup)))
+    return cudaErrorInvalidValue;
+  SmallShape sh{};
+  sh.xrows = lora_small_tile(a.rows);
+  const int tiles = (a.out + kCols - 1) / kCols * ((a.rows + sh.xrows - 1) / sh.xrows);
+  // K parts: as many as still run at once, one CTA an SM (measured at 64 rows,
+  // 1024 -> 3072: 4 parts, 96 CTAs, 5.7 us; 8 parts, in two rounds, 10.3 us), two
+  // for tiles of 16 rows, whose CTAs are small (1 row: 4 parts 4.2 us, 8 parts
+  // 3.7 us)
+  const int room_ctas = sh.xrows <= 16 ? 2 * num_sms : num_sms;
   int splits = 1;
-  while (splits < 8 && 2 * splits <= a.num_kb && tiles * splits < num_sms) splits *= 2;
-  const int stage_bytes = kWBytes + (xrows * 128 + 1023) / 1024 * 1024;
-  const int steps = (a.num_kb + splits - 1) / splits + ((a.entries + splits - 1) / splits + 1) / 2;
-  const int room = static_cast<int>((kSmemLimit - 4096) / stage_bytes);
-  const int stages = std::max(1, std::min(std::min(kMaxStages, steps), room));
+  while (splits < 8 && 2 * splits <= a.num_kb && 2 * splits * tiles <= room_ctas) splits *= 2;
+  sh.own = fused ? (a.entries + splits - 1) / splits : 0;
+  const int stage_bytes = kWBytes + sh.xrows * 128 + (fused ? a.entries * kABytes : 0);
+  const int steps = (a.num_kb + splits - 1) / splits + (fused ? 0 : ((a.entries + splits - 1) / splits + 1) / 2);
+  const size_t parts =
+      sizeof(float) * sh.xrows * (2 * kPartLd + (fused ? (a.entries + (splits - 1) * sh.own) * kPartULd : 0));
+  // fused: the last stage's A operand is read as 128 rows; what follows is the
+  // parts, long enough with the padding here
+  const size_t fixed = 1024 + static_cast<size_t>(sh.own) * (kBBytes + sh.xrows * 64) + std::max<size_t>(parts, fused ? 128 * 128 : 0);
+  const int room = static_cast<int>((kSmemLimit - fixed) / stage_bytes);
+  sh.stages = std::max(1, std::min(std::min(kMaxStages, steps), room));
+  sh.ring_bytes = sh.stages * stage_bytes;
   // A CTA waits for its cluster, so no CTA may be left waiting for TMEM that a
   // waiting one holds: shared memory in proportion to the TMEM columns (456 of
   // an SM's 233472 bytes a column, of its 512) keeps the columns of the CTAs
   // on an SM, of this kernel and the other clustered ones, within 512.
-  const int cols = xrows <= 32 ? 32 : xrows <= 64 ? 64 : xrows <= 128 ? 128 : 256;
-  const size_t smem = std::max(1024 + std::max(static_cast<size_t>(stages) * stage_bytes, sizeof(float) * xrows * kPartLd),
-                               static_cast<size_t>(cols) * 456 - 1024);
-  const SmallMaps maps{x, w, u, b};
-  return a.bf16 ? launch<__nv_bfloat16>(maps, a, splits, stages, smem, s)
-                : launch<__half>(maps, a, splits, stages, smem, s);
+  const int need = fused ? 2 * sh.xrows : sh.xrows;
+  const int cols = need <= 32 ? 32 : need <= 64 ? 64 : 128;
+  const size_t smem = std::max(fixed + static_cast<size_t>(sh.ring_bytes), static_cast<size_t>(cols) * 456 - 1024);
+  const SmallMaps maps{x, w, u, b, a_map};
+  if (a.bf16)
+    return fused ? launch_splits<__nv_bfloat16, true>(splits, maps, a, sh, smem, s)
+                 : launch_splits<__nv_bfloat16, false>(splits, maps, a, sh, smem, s);
+  return fused ? launch_splits<__half, true>(splits, maps, a, sh, smem, s)
+               : launch_splits<__half, false>(splits, maps, a, sh, smem, s);
 }
 
 }  // namespace laya

@@ -164,6 +164,7 @@ class LoraPlan:
         _check(lib().laya_lora_plan_create(lora._h, r.ctypes.data_as(_i32p), s.ctypes.data_as(_i32p), r.size,
                                            ctypes.byref(h)))
         self._h = h
+        self._destroy = lib().laya_lora_plan_destroy
 
     def status(self) -> None:
         """Waits for the device; raises if a bounded wait expired in a run."""
@@ -171,7 +172,7 @@ class LoraPlan:
 
     def close(self) -> None:
         if getattr(self, "_h", None):
-            lib().laya_lora_plan_destroy(self._h)
+            self._destroy(self._h)
             self._h = None
 
     def __del__(self):
@@ -188,6 +189,7 @@ class Lora:
         _check(lib().laya_lora_create(device, type, inn, out, w or None, ldw, bias or None, slots, max_rank,
                                       ctypes.byref(h)))
         self._h = h
+        self._destroy = lib().laya_lora_destroy
         self.inn, self.out = inn, out
 
     def set(self, slot: int, a, b, scale: float = 1.0) -> None:
@@ -213,7 +215,7 @@ class Lora:
 
     def close(self) -> None:
         if getattr(self, "_h", None):
-            lib().laya_lora_destroy(self._h)
+            self._destroy(self._h)
             self._h = None
 
     def __del__(self):
