@@ -96,12 +96,12 @@ int laya_rope(int device, const laya_rope_spec *spec, const laya_rope_tensor *te
  *   y[m] = x[m] W^T + bias + scale_a (x[m] A_a^T) B_a^T
  * for row m of a segment with adapter a, without the last term for a segment
  * that has none.  W [out, in], A_a [rank_a, in], B_a [out, rank_a]; x, W, A, B
- * and y of one 16-bit type (LAYA_F16 or LAYA_BF16), bias f32.  Sums are f32 and
- * y is rounded once: the rank-space vector x A^T passes between the two
- * products as a pair of 16-bit values (value and remainder), not one.  With
- * LAYA_F16 its magnitude times scale must stay below 65504, as every f16
- * activation must.  The sum order depends on the number of rows of the whole
- * call, not on the other rows' values or adapters; equal calls give equal bits.
+ * and y of one 16-bit type (LAYA_F16 or LAYA_BF16), bias f32.  Sums are f32.
+ * The rank-space vector scale x A^T is rounded once between the two products:
+ * to f16, or to a pair of bf16 (value and remainder); y is rounded once.  With
+ * LAYA_F16 the magnitude of scale x A^T must stay below 65504, as every f16
+ * activation must.  A row's sums never meet another row's values; equal calls
+ * give equal bits.
  *
  * A laya_lora holds the adapters of one projection; W and bias stay the
  * caller's (read at every run).  A laya_lora_plan holds the segments of one

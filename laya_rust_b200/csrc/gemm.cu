@@ -32,10 +32,10 @@
 // With EXT (rows that have low-rank adapters), a tile's K loop goes on over the
 // adapters its row block needs: entry e multiplies 16 columns of rank-space
 // vectors u (zero in rows of other adapters) with 16 columns of that adapter's
-// B.  A stage then holds two entries, each u's values and remainders (two
-// 128-row operands of 32 bytes a row, 32-byte swizzle) against one B operand:
-// four K = 16 MMAs, as many as a stage of the K loop.  So adapters cost a tile
-// entries / 2 more k-blocks and no pass of their own over the output.
+// B (operands of 32 bytes a row, 32-byte swizzle).  A stage holds four entries,
+// or two of bf16, whose u is a value and a remainder: four K = 16 MMAs, as many
+// as a stage of the K loop.  So adapters cost a tile entries / 4 (bf16: / 2) more
+// k-blocks and no pass of their own over the output.
 // No TMA load in this kernel uses multicast; every CTA loads its own operand
 // halves.  The MMA completion signal is delivered to both CTAs of the pair
 // with tcgen05.commit's cluster-multicast form.
@@ -70,10 +70,13 @@ constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int STAGING_BYTES = 4096;    // 32 rows x 128 B
 constexpr int BAR_BYTES = 256;
 constexpr size_t SMEM_LIMIT = 232448;
-// EXT: one adapter operand of a CTA's rows, 16 columns (32 bytes) a row; a
-// stage takes two entries of two such operands
+// EXT: one adapter operand of a CTA's rows, 16 columns (32 bytes) a row; four
+// fill a stage's A operand
 constexpr int EXT_A_BYTES = CTA_ROWS * 32;
-static_assert(4 * EXT_A_BYTES == CTA_ROWS * BK * 2, "two entries fill a stage's A operand");
+static_assert(4 * EXT_A_BYTES == CTA_ROWS * BK * 2, "four operands to a stage");
+// 16-column operands of u an entry has
+template <int EPI>
+constexpr int kExtParts = EPI == kEpiPlainBf16 ? 2 : 1;
 
 template <int BN>
 struct Cfg {
@@ -607,23 +610,32 @@ __global__ void __launch_bounds__(THREADS, 1)
             grid_dep_wait();  // u is complete
             early = false;
           }
-          for (int e = __ldg(ext.off + mb); e < e1; e += 2) {
-            const int n = min(2, e1 - e);
-            const int chunk[2] = {__ldg(ext.chunk + e), n > 1 ? __ldg(ext.chunk + e + 1) : 0};
+          constexpr int kParts = kExtParts<EPI>, kPerStage = 4 / kParts;
+          int e = __ldg(ext.off + mb);
+          int chunk[kPerStage];
+#pragma unroll
+          for (int i = 0; i < kPerStage; ++i) chunk[i] = e + i < e1 ? __ldg(ext.chunk + e + i) : 0;
+          for (; e < e1; e += kPerStage) {
+            const int n = min(kPerStage, e1 - e);
             if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, args.err, kErrGemmProducerWait, abort_flag,
                                    args.wait_limit_ns)) {
               ok = false;
               break;
             }
             const uint32_t fb = map_to_rank(smem_u32(&full[stage]), 0);
-            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * n * (2 * EXT_A_BYTES + BN / 2 * 32));
-            for (int i = 0; i < n; ++i) {
-              uint8_t* sa = sA + stage * C::A_BYTES + i * 2 * EXT_A_BYTES;
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * n * (kParts * EXT_A_BYTES + BN / 2 * 32));
+#pragma unroll
+            for (int i = 0; i < kPerStage; ++i) {
+              if (i >= n) break;
+              uint8_t* sa = sA + stage * C::A_BYTES + i * kParts * EXT_A_BYTES;
               const int y = (e + i) * BM + static_cast<int>(rank) * CTA_ROWS;
               tma_load_2d_pair(sa, &ext.u, 0, y, fb);
-              tma_load_2d_pair(sa + EXT_A_BYTES, &ext.u, 16, y, fb);
+              if (kParts == 2) tma_load_2d_pair(sa + EXT_A_BYTES, &ext.u, 16, y, fb);
               tma_load_2d_pair(sB + stage * C::B_BYTES + i * (BN / 2 * 32), &ext.b, 0, chunk[i] * ext.b_rows + n0, fb);
             }
+#pragma unroll
+            for (int i = 0; i < kPerStage; ++i)
+              chunk[i] = e + kPerStage + i < e1 ? __ldg(ext.chunk + e + kPerStage + i) : 0;
             if (++stage == C::STAGES) {
               stage = 0;
               phase ^= 1u;
@@ -678,7 +690,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (kb1 == num_kb) {
             const int mb = w.tile / num_n;
             const int e1 = __ldg(ext.off + mb + 1);
-            for (int e = __ldg(ext.off + mb); e < e1; e += 2) {
+            constexpr int kParts = kExtParts<EPI>, kPerStage = 4 / kParts;
+            for (int e = __ldg(ext.off + mb); e < e1; e += kPerStage) {
               if (!mbar_wait_bounded(&full[stage], phase, args.err, kErrGemmMmaWait, abort_flag, args.wait_limit_ns)) {
                 ok = false;
                 break;
@@ -686,11 +699,11 @@ __global__ void __launch_bounds__(THREADS, 1)
               tc_fence_after();
               const uint32_t a_addr = smem_u32(sA + stage * C::A_BYTES);
               const uint32_t b_addr = smem_u32(sB + stage * C::B_BYTES);
-              for (int i = 0; i < min(2, e1 - e); ++i) {
+              for (int i = 0; i < min(kPerStage, e1 - e); ++i) {
                 const uint64_t db = umma_desc_sw32(b_addr + i * (BN / 2 * 32));
-                const uint32_t sa = a_addr + i * 2 * EXT_A_BYTES;
+                const uint32_t sa = a_addr + i * kParts * EXT_A_BYTES;
                 umma2_f16(d_tmem, umma_desc_sw32(sa), db, idesc, 1u);
-                umma2_f16(d_tmem, umma_desc_sw32(sa + EXT_A_BYTES), db, idesc, 1u);
+                if (kParts == 2) umma2_f16(d_tmem, umma_desc_sw32(sa + EXT_A_BYTES), db, idesc, 1u);
               }
               umma2_commit_both(&empty[stage]);
               if (++stage == C::STAGES) {

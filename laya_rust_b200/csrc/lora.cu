@@ -3,11 +3,9 @@
 //
 //   y[m] = x[m] W^T + bias + s_a (x[m] A_a^T) B_a^T
 //
-// Two launches.  The first computes u = s_a (x A_a^T) in rank space, f32, and
-// leaves it as a pair of 16-bit values (value and remainder, together 16 bits
-// more than one), so the second product's operands are 16-bit and the pair's
-// rounding stays far below that of y.  The second computes x W^T + u B^T in one f32
-// accumulator and rounds once: the tcgen05 GEMM of gemm.cu, whose K loop goes on
+// Two launches.  The first computes u = s_a (x A_a^T) in rank space, in f32, and
+// rounds it to the 16-bit operand of the second product (lora.h says how).
+// The second computes x W^T + u B^T in one f32 accumulator and rounds once: the tcgen05 GEMM of gemm.cu, whose K loop goes on
 // over the adapters of its row block (GemmExt).  It is launched with programmatic
 // serialization and waits for u only before its adapter steps, so its K loop
 // runs beside the first launch.
@@ -42,64 +40,98 @@ struct Num<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 };
 
-// v as a 16-bit value and the 16-bit remainder; a value that is not finite has
-// remainder 0 (inf - inf would be NaN).
+// Two rank values into u: packed values, and for bf16 the packed remainders
+// (0 where a value is not finite: inf - inf would be NaN) 16 elements further.
 template <class T>
-__device__ __forceinline__ void split_value(float v, T& hi, T& lo) {
-  hi = Num<T>::down(v);
-  const float h = Num<T>::up(hi);
-  lo = Num<T>::down(isfinite(h) ? v - h : 0.0f);
+__device__ __forceinline__ void store_u2(T* dst, float a, float b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 hi = __floats2bfloat162_rn(a, b);
+    const float2 h = __bfloat1622float2(hi);
+    *reinterpret_cast<__nv_bfloat162*>(dst) = hi;
+    *reinterpret_cast<__nv_bfloat162*>(dst + kLoraChunk) =
+        __floats2bfloat162_rn(isfinite(h.x) ? a - h.x : 0.0f, isfinite(h.y) ? b - h.y : 0.0f);
+  } else {
+    *reinterpret_cast<__half2*>(dst) = __floats2half2_rn(a, b);
+  }
+}
+template <class T>
+__device__ __forceinline__ T* u_row(void* u, int entry, int row) {
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  return static_cast<T*>(u) + static_cast<size_t>(entry) * lora_entry_elems(bf16) +
+         static_cast<size_t>(row % kLoraBlock) * lora_u_width(bf16);
+}
+// 16 rank values, as 16-byte stores.
+template <class T>
+__device__ __forceinline__ void store_u16(T* dst, const float (&v)[16]) {
+  __align__(16) T t[2 * kLoraChunk];
+#pragma unroll
+  for (int j = 0; j < 16; j += 2) store_u2<T>(t + j, v[j], v[j + 1]);
+  const uint4* src = reinterpret_cast<const uint4*>(t);
+  uint4* d = reinterpret_cast<uint4*>(dst);
+  d[0] = src[0];
+  d[1] = src[1];
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    d[2] = src[2];
+    d[3] = src[3];
+  }
 }
 
 constexpr int kXBytes = kLoraItemRows * 64 * 2;   // x operand of a k-block: 16 KB
 constexpr int kABytes = kLoraChunk * 64 * 2;      // one entry's A operand: 2 KB
 constexpr int kRingBytes = 192 * 1024;
 constexpr int kMaxStages = 8;
-constexpr size_t kShrinkSmem = 1024 + kRingBytes + 256;
+constexpr size_t kShrinkSmem = 1024 + kRingBytes;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float4 ld_cluster_f4(const float* p, uint32_t rank) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t map_to_rank(const void* p, uint32_t rank) {
   uint32_t r;
-  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(r)
+  return r;
+}
+__device__ __forceinline__ void bulk_to_rank(const void* dst, uint64_t* bar, const void* src, uint32_t bytes, uint32_t rank) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   map_to_rank(dst, rank)),
+               "r"(smem_u32(src)), "r"(bytes), "r"(map_to_rank(bar, rank))
                : "memory");
-  return v;
 }
 
 // u = scale (x A^T) for one item: 128 rows against up to 8 entries (M = 128,
 // N = 16 entries), K cut over the CTAs of a cluster.  Per CTA: warp 0 loads
-// (TMA ring of x and A k-blocks), warp 1 issues the MMAs, then all four warps
-// take the f32 sums from TMEM to shared memory, the CTAs of the cluster add
-// each other's parts in rank order (distributed shared memory, rows dealt out
-// over the CTAs) and store the entries each row owns.
-template <class T>
+// (TMA ring of x and A k-blocks), warp 1 issues the MMAs, warps 2 and 3 look up
+// the rows' adapters.  Then a thread has its row's sums in TMEM: alone it stores
+// them; in a cluster each CTA owns a share of the rows, the others send it
+// their sums with one bulk copy each, and it adds them in rank order.
+template <class T, int SPLITS>
 __global__ void __launch_bounds__(128, 1)
     lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
-                       const LoraShrinkArgs a, const int splits) {
+                       const LoraShrinkArgs a) {
   extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, in_full;
+  __shared__ uint32_t tmem_holder;
+  __shared__ int abort_word;
+  __shared__ int row_slot[kLoraItemRows];
+  __shared__ float row_scale[kLoraItemRows];
+  __shared__ int item_entry[kLoraMaxGroup], item_slot[kLoraMaxGroup];
+  volatile int* abort_flag = &abort_word;
   uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kRingBytes);
-  uint64_t* empty = full + kMaxStages;
-  uint64_t* done = empty + kMaxStages;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
-  const int4 item = __ldg(a.item + blockIdx.x / splits);
+  const int rank = SPLITS > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int4 item = __ldg(a.item + blockIdx.x / SPLITS);
   const int n = item.z;
   const int stage_bytes = kXBytes + a.group * kABytes;
-  const int stages = min(kMaxStages, kRingBytes / stage_bytes);
-  const int kb0 = static_cast<int>(rank) * a.num_kb / splits, kb1 = (static_cast<int>(rank) + 1) * a.num_kb / splits;
+  // the sums, apart from the ring: [128][ld] and, sent here, [SPLITS - 1][own rows][ld]
+  const int ld = 16 * a.group + 4, own_rows = kLoraItemRows / SPLITS;
+  const int part_bytes = SPLITS > 1 ? 2 * kLoraItemRows * ld * 4 : 0;
+  const int stages = min(kMaxStages, (kRingBytes - part_bytes) / stage_bytes);
+  float* part = reinterpret_cast<float*>(smem + kRingBytes - part_bytes);
+  float* part_in = part + kLoraItemRows * ld;
+  const int kb0 = rank * a.num_kb / SPLITS, kb1 = (rank + 1) * a.num_kb / SPLITS;
   const uint32_t tmem_cols = a.group <= 2 ? 32 : 16 * a.group;
 
   if (threadIdx.x == 0) {
@@ -107,26 +139,31 @@ __global__ void __launch_bounds__(128, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(done, 1);
-    *abort_flag = 0;
+    mbar_init(&done, 1);
+    mbar_init(&in_full, 1);
+    abort_word = 0;
     fence_mbar_init();
+    if (SPLITS > 1) mbar_arrive_expect_tx(&in_full, (SPLITS - 1) * own_rows * ld * 4);
     tma_prefetch_desc(&tmX);
     tma_prefetch_desc(&tmA);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_holder, tmem_cols);
+    tmem_alloc(&tmem_holder, tmem_cols);
     tmem_relinquish();
   }
+  // lane i of warp 0 holds entry i's row of A
+  const int a_row = warp == 0 && lane < n ? __ldg(a.item_chunk + item.y + lane) * kLoraChunk : 0;
+  __syncwarp();
+  if (SPLITS > 1) cluster_arrive();  // this CTA's shared memory exists
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_holder;
+  const uint32_t tmem = tmem_holder;
+  // everything above reads only the plan
   grid_dep_wait();
   grid_dep_trigger();
 
   if (warp == 0) {
-    // lane i holds entry i's row of A
-    const int a_row = lane < n ? __ldg(a.item_chunk + item.y + lane) * kLoraChunk : 0;
     int a_rows[kLoraMaxGroup];
 #pragma unroll
     for (int i = 0; i < kLoraMaxGroup; ++i) a_rows[i] = __shfl_sync(0xffffffffu, a_row, i);
@@ -135,10 +172,8 @@ __global__ void __launch_bounds__(128, 1)
       int stage = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag)) {
-          ok = false;
-          break;
-        }
+        ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag);
+        if (!ok) break;
         uint8_t* sx = smem + stage * stage_bytes;
         mbar_arrive_expect_tx(&full[stage], kXBytes + n * kABytes);
         tma_load_2d(sx, &tmX, kb * 64, item.x * kLoraItemRows, &full[stage]);
@@ -177,70 +212,86 @@ __global__ void __launch_bounds__(128, 1)
           phase ^= 1u;
         }
       }
-      umma_commit(done);
+      umma_commit(&done);
     }
     __syncwarp();
+  } else {
+    for (int r = static_cast<int>(threadIdx.x) - 64; r < kLoraItemRows; r += 64) {
+      const int row = item.x * kLoraItemRows + r;
+      const int e0 = row < a.rows ? __ldg(a.row_entry + row) : -1;
+      const int slot = e0 >= 0 ? __ldg(a.entry_chunk + e0) / a.chunks_per_slot : -1;
+      row_slot[r] = slot;
+      row_scale[r] = slot >= 0 ? __ldg(a.scale + slot) : 0.0f;
+    }
+    const int i = static_cast<int>(threadIdx.x) - 64;
+    if (i < n) {
+      item_entry[i] = __ldg(a.item_entry + item.y + i);
+      item_slot[i] = __ldg(a.item_chunk + item.y + i) / a.chunks_per_slot;
+    }
   }
-  // this CTA's sums to shared memory (the ring is idle: every k-block was
-  // consumed), one row a thread; 4 floats of padding a row
-  float* part = reinterpret_cast<float*>(smem);
-  const int ld = 16 * a.group + 4;
-  bool ok = mbar_wait_bounded(done, 0, a.err, kErrLoraWait, nullptr) && !*abort_flag;
+  bool ok = mbar_wait_bounded(&done, 0, a.err, kErrLoraWait, nullptr) && !*abort_flag;
   ok = __syncthreads_and(ok);
   tc_fence_after();
-  if (ok) {
+  const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+  if constexpr (SPLITS == 1) {
+    const int r = threadIdx.x;
+    const int slot = ok ? row_slot[r] : -1;
+    const float scale = row_scale[r];
     for (int i = 0; i < n; ++i) {
       uint32_t v[16];
-      tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + i * 16, v);
+      tmem_ld_32x32b_x16(tmem + lane_base + i * 16, v);
       tmem_ld_wait();
-      float4* dst = reinterpret_cast<float4*>(part + threadIdx.x * ld + i * 16);
+      if (item_slot[i] != slot) continue;
+      float f[16];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        dst[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
-                             __uint_as_float(v[4 * j + 3]));
+      for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[j]) * scale;
+      store_u16<T>(u_row<T>(a.u, item_entry[i], item.x * kLoraItemRows + r), f);
     }
-  }
-  tc_fence_before();
-  cluster_sync();
-  // `splits` threads a row, each every splits-th entry
-  const int r = static_cast<int>(rank) * (kLoraItemRows / splits) + threadIdx.x / splits;
-  const int row = item.x * kLoraItemRows + r;
-  const int e0 = ok && row < a.rows ? __ldg(a.row_entry + row) : -1;
-  if (e0 >= 0) {
-    const int slot = __ldg(a.entry_chunk + e0) / a.chunks_per_slot;
-    const float scale = __ldg(a.scale + slot);
-    for (int i = threadIdx.x % splits; i < n; i += splits) {
-      if (__ldg(a.item_chunk + item.y + i) / a.chunks_per_slot != slot) continue;
-      const int e = __ldg(a.item_entry + item.y + i);
-      T hi[16], lo[16];
+    tc_fence_before();
+    __syncthreads();
+  } else {
+    cluster_wait();  // every CTA of the cluster has started
+    for (int i = 0; i < n; ++i) {
+      uint32_t v[16];
+      tmem_ld_32x32b_x16(tmem + lane_base + i * 16, v);
+      tmem_ld_wait();
+      uint4* dst = reinterpret_cast<uint4*>(part + threadIdx.x * ld + i * 16);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float4 s = ld_cluster_f4(part + r * ld + i * 16 + 4 * j, 0);
-        for (int c = 1; c < splits; ++c) {
-          const float4 t = ld_cluster_f4(part + r * ld + i * 16 + 4 * j, c);
-          s.x += t.x;
-          s.y += t.y;
-          s.z += t.z;
-          s.w += t.w;
-        }
-        split_value<T>(s.x * scale, hi[4 * j], lo[4 * j]);
-        split_value<T>(s.y * scale, hi[4 * j + 1], lo[4 * j + 1]);
-        split_value<T>(s.z * scale, hi[4 * j + 2], lo[4 * j + 2]);
-        split_value<T>(s.w * scale, hi[4 * j + 3], lo[4 * j + 3]);
+      for (int j = 0; j < 4; ++j) dst[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+    tc_fence_before();
+    fence_proxy_async_smem();
+    __syncthreads();
+    const int to = static_cast<int>(threadIdx.x);
+    if (to < SPLITS && to != rank)
+      bulk_to_rank(part_in + (rank < to ? rank : rank - 1) * own_rows * ld, &in_full, part + to * own_rows * ld,
+                   own_rows * ld * 4, to);
+    if (!mbar_wait_bounded(&in_full, 0, a.err, kErrLoraWait, nullptr)) ok = false;
+    __syncwarp();
+    cluster_arrive();  // what this CTA was sent has landed
+    // SPLITS threads a row, each every SPLITS-th entry
+    const int q = static_cast<int>(threadIdx.x) / SPLITS, r = rank * own_rows + q;
+    const int slot = ok ? row_slot[r] : -1;
+    for (int i = static_cast<int>(threadIdx.x) % SPLITS; i < n && slot >= 0; i += SPLITS) {
+      if (item_slot[i] != slot) continue;
+      float f[16];
+#pragma unroll
+      for (int c = 0; c < SPLITS; ++c) {
+        const float* p = (c == rank ? part + r * ld : part_in + ((c < rank ? c : c - 1) * own_rows + q) * ld) + i * 16;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) f[j] = c == 0 ? p[j] : f[j] + p[j];
       }
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.u) + static_cast<size_t>(e) * kLoraEntryElems +
-                                            static_cast<size_t>(row % kLoraBlock) * 2 * kLoraChunk);
-      dst[0] = *reinterpret_cast<uint4*>(hi);
-      dst[1] = *reinterpret_cast<uint4*>(hi + 8);
-      dst[2] = *reinterpret_cast<uint4*>(lo);
-      dst[3] = *reinterpret_cast<uint4*>(lo + 8);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) f[j] *= row_scale[r];
+      store_u16<T>(u_row<T>(a.u, item_entry[i], item.x * kLoraItemRows + r), f);
     }
   }
-  cluster_sync();  // no CTA leaves while another may still read its part
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, tmem_cols);
   }
+  __syncwarp();
+  if (SPLITS > 1) cluster_wait();  // no CTA leaves while a copy may still read its part
 }
 
 // u = scale (x A^T) for one (row, chunk) pair a block: a warp takes two of the
@@ -282,65 +333,57 @@ __global__ void __launch_bounds__(256) lora_pairs_kernel(const LoraPairsArgs a) 
     s1 += __shfl_xor_sync(0xffffffffu, s1, o);
   }
   if (lane == 0) {
-    T hi[2], lo[2];
-    split_value<T>(s0 * scale, hi[0], lo[0]);
-    split_value<T>(s1 * scale, hi[1], lo[1]);
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.u) + static_cast<size_t>(p.y) * kLoraEntryElems +
-                                                static_cast<size_t>(p.x % kLoraBlock) * 2 * kLoraChunk + 2 * warp);
-    dst[0] = *reinterpret_cast<uint32_t*>(hi);
-    dst[kLoraChunk / 2] = *reinterpret_cast<uint32_t*>(lo);
+    store_u2<T>(u_row<T>(a.u, p.y, p.x) + 2 * warp, s0 * scale, s1 * scale);
   }
 }
 
-template <class T>
-cudaError_t launch_shrink(const CUtensorMap& x, const CUtensorMap& a_map, const LoraShrinkArgs& a, int splits, bool pdl,
-                          cudaStream_t s) {
+template <class T, int SPLITS>
+cudaError_t launch_shrink(const CUtensorMap& x, const CUtensorMap& a_map, const LoraShrinkArgs& a, cudaStream_t s) {
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(lora_shrink_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(lora_shrink_kernel<T, SPLITS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(kShrinkSmem));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.x = SPLITS;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  const dim3 grid(a.items * splits);
-  if (pdl) return launch_pdl(lora_shrink_kernel<T>, grid, dim3(128), kShrinkSmem, s, attr, 1, x, a_map, a, splits);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = kShrinkSmem;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, lora_shrink_kernel<T>, x, a_map, a, splits);
+  return launch_pdl(lora_shrink_kernel<T, SPLITS>, dim3(a.items * SPLITS), dim3(128), kShrinkSmem, s, attr, 1, x, a_map, a);
+}
+
+template <class T>
+cudaError_t launch_shrink(int splits, const CUtensorMap& x, const CUtensorMap& a_map, const LoraShrinkArgs& a,
+                          cudaStream_t s) {
+  switch (splits) {
+    case 1: return launch_shrink<T, 1>(x, a_map, a, s);
+    case 2: return launch_shrink<T, 2>(x, a_map, a, s);
+    case 4: return launch_shrink<T, 4>(x, a_map, a, s);
+    default: return launch_shrink<T, 8>(x, a_map, a, s);
+  }
 }
 
 }  // namespace
 
 cudaError_t launch_lora_shrink(const CUtensorMap& x, const CUtensorMap& a_map, const LoraShrinkArgs& a, int num_sms,
-                               bool pdl, cudaStream_t s) {
+                               cudaStream_t s) {
   if (a.items <= 0) return cudaSuccess;
   if (a.num_kb < 1 || a.group < 1 || a.group > kLoraMaxGroup) return cudaErrorInvalidValue;
   int splits = 1;
   while (splits < 8 && 2 * splits * a.items <= num_sms && 4 * splits <= a.num_kb) splits *= 2;
-  return a.bf16 ? launch_shrink<__nv_bfloat16>(x, a_map, a, splits, pdl, s)
-                : launch_shrink<__half>(x, a_map, a, splits, pdl, s);
+  return a.bf16 ? launch_shrink<__nv_bfloat16>(splits, x, a_map, a, s) : launch_shrink<__half>(splits, x, a_map, a, s);
 }
 
-cudaError_t launch_lora_pairs(const LoraPairsArgs& a, bool pdl, cudaStream_t s) {
+cudaError_t launch_lora_pairs(const LoraPairsArgs& a, cudaStream_t s) {
   if (a.pairs <= 0) return cudaSuccess;
   auto* kernel = a.bf16 ? &lora_pairs_kernel<__nv_bfloat16> : &lora_pairs_kernel<__half>;
-  if (pdl) return launch_pdl(kernel, dim3(a.pairs), dim3(256), 0, s, nullptr, 0, a);
-  kernel<<<a.pairs, 256, 0, s>>>(a);
-  return cudaGetLastError();
+  return launch_pdl(kernel, dim3(a.pairs), dim3(256), 0, s, nullptr, 0, a);
 }
 
 LoraItems lora_items(const LoraLayout& L, int num_sms) {
@@ -689,15 +732,15 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     std::copy(entry_chunk.begin(), entry_chunk.end(), h.begin() + o_ent);
     q.dev.alloc(h.size() * 4, "lora plan");
     const size_t entries = std::max<size_t>(1, L.chunk.size());
-    q.u.alloc(entries * kLoraEntryElems * 2, "lora workspace");
+    q.u.alloc(entries * lora_entry_elems(k.bf16) * 2, "lora workspace");
     q.small = lora_use_small(L.rows);
-    if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock, 2 * kLoraChunk,
+    if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock, lora_u_width(k.bf16),
                        q.small ? lora_small_tile(L.rows) : kGemmABoxRows))
       throw OpError(LAYA_E_CUDA, "lora_plan_create: tensor map encode failed");
     op_check(cudaMemcpyAsync(q.dev.p, h.data(), h.size() * 4, cudaMemcpyHostToDevice, k.stream), "lora plan upload");
     // rows of other adapters are zero in an entry, and stay zero: every run
     // writes the same rows of each entry
-    op_check(cudaMemsetAsync(q.u.p, 0, entries * kLoraEntryElems * 2, k.stream), "lora workspace clear");
+    op_check(cudaMemsetAsync(q.u.p, 0, entries * lora_entry_elems(k.bf16) * 2, k.stream), "lora workspace clear");
     op_check(cudaStreamSynchronize(k.stream), "lora plan upload");
     q.d_err = q.dev.as<int>();
     q.d_off = q.dev.as<int>() + o_off;
@@ -753,7 +796,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       s.in = k.in;
       s.in_pad = k.in_pad;
       s.bf16 = k.bf16;
-      op_check(launch_lora_pairs(s, false, st), "lora launch");
+      op_check(launch_lora_pairs(s, st), "lora launch");
     } else if (q.items > 0) {
       CUtensorMap mxi = mx;
       if (xbox != kLoraItemRows && make_tmap_pitched(&mxi, x, k.bf16, q.lay.rows, k.in, ldx, kLoraItemRows))
@@ -773,7 +816,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       s.chunks_per_slot = k.cps;
       s.bf16 = k.bf16;
       s.err = q.d_err;
-      op_check(launch_lora_shrink(mxi, k.a_map, s, k.num_sms, false, st), "lora launch");
+      op_check(launch_lora_shrink(mxi, k.a_map, s, k.num_sms, st), "lora launch");
     }
     // x W^T and u B^T in one accumulator
     const bool early = !fused && (q.pairs > 0 || q.items > 0);

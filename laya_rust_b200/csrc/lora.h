@@ -24,9 +24,15 @@ inline int lora_chunks(int rank) { return (rank + kLoraChunk - 1) / kLoraChunk; 
 // The adapters each block of 256 rows needs.  Entry e in [off[b], off[b + 1])
 // is one chunk of one adapter that some row of block b has; a slot's chunks
 // are consecutive entries, slots in order of first use.  row_entry[m]: the
-// first entry of row m's adapter, or -1.  u, the rank-space vectors, is
-// [entries][256 rows][16 values | 16 remainders] in the 16-bit type, zero for
-// rows of other adapters.
+// first entry of row m's adapter, or -1.  u, the rank-space vectors scale *
+// (x A^T), is [entries][256 rows][16 values], in bf16 [16 values | 16
+// remainders], zero for rows of other adapters.
+//
+// u passes between the two products in the 16-bit type.  In f16 one value: half a
+// step is 2^-11 of it, so what it adds to y's error is at most 2^-11 of the
+// adapter's part of y (the errors of its rank values average out), beside the
+// 2^-11 of all of y that rounding y costs.  In bf16 half a step is 2^-8, and a
+// second bf16 with the remainder leaves 2^-16.
 struct LoraLayout {
   int rows = 0;
   std::vector<int> off;
@@ -36,7 +42,9 @@ struct LoraLayout {
 // Throws OpError; chunks_of(slot) is the slot's chunk count, 0 if it is empty.
 LoraLayout lora_layout(const int32_t* rows, const int32_t* slot, int n, const std::vector<int>& chunks_of);
 
-constexpr size_t kLoraEntryElems = static_cast<size_t>(kLoraBlock) * 2 * kLoraChunk;
+// Values a row of an entry.
+constexpr int lora_u_width(bool bf16) { return bf16 ? 2 * kLoraChunk : kLoraChunk; }
+constexpr size_t lora_entry_elems(bool bf16) { return static_cast<size_t>(kLoraBlock) * lora_u_width(bf16); }
 
 // The work of the rank-space product: item i computes entries
 // entry[item.y .. item.y + item.z) for rows [128 item.x, 128 item.x + 128).
@@ -64,10 +72,12 @@ struct LoraShrinkArgs {
   bool bf16;
   int* err;
 };
-// u entries of every row with an adapter: scale * (x A^T) as value + remainder.
+// u entries of every row with an adapter.
 // x: box 64 x 128, A (make_tmap_pitched, [chunks * 16, in_pad]): box 64 x 16.
+// Both launches of u pass grid_dep_wait() before grid_dep_trigger(), so a GEMM
+// behind them may start early.
 cudaError_t launch_lora_shrink(const CUtensorMap& x, const CUtensorMap& a_map, const LoraShrinkArgs& a, int num_sms,
-                               bool pdl, cudaStream_t s);
+                               cudaStream_t s);
 
 // The same for few (row, chunk) pairs: pair p is (row, entry, chunk in the
 // bank, slot).
@@ -82,7 +92,7 @@ struct LoraPairsArgs {
   int in, in_pad;
   bool bf16;
 };
-cudaError_t launch_lora_pairs(const LoraPairsArgs& a, bool pdl, cudaStream_t s);
+cudaError_t launch_lora_pairs(const LoraPairsArgs& a, cudaStream_t s);
 
 // The projection of at most kLoraBlock rows (one block, so entries
 // 0 .. entries - 1): lora_small.cu.  `fused` (1 to kLoraMaxGroup entries): it

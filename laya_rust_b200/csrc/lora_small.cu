@@ -16,8 +16,7 @@
 // With at most 8 entries (FUSED) the same launch computes u as well: the A rows
 // of the entries ride along the K loop as a second M = 128 operand against the
 // same x, the cluster adds those sums first, and each CTA turns the entries it
-// owns into the two 16-bit operands of the adapter step in its own shared
-// memory.  Every cluster repeats u for its rows (16 rows of A per entry from
+// owns into 16-bit operands of the adapter step in its own shared memory.  Every cluster repeats u for its rows (16 rows of A per entry from
 // L2), which costs less than a launch of its own.
 #include <cuda_bf16.h>
 
@@ -107,16 +106,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// (a, b) as packed values and packed remainders (0 where a value is not finite).
+// (a, b) as packed values and, for bf16, packed remainders (0 where a value is
+// not finite).
 template <class T>
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = pack2<T>(a, b);
-  float2 h;
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    h = make_float2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u));
-  else
-    h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  lo = pack2<T>(isfinite(h.x) ? a - h.x : 0.0f, isfinite(h.y) ? b - h.y : 0.0f);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const float x = __uint_as_float(hi << 16), y = __uint_as_float(hi & 0xffff0000u);
+    lo = pack2<T>(isfinite(x) ? a - x : 0.0f, isfinite(y) ? b - y : 0.0f);
+  }
 }
 
 template <class T, int SPLITS, bool FUSED>
@@ -135,6 +133,8 @@ __global__ void __launch_bounds__(kThreads)
   const int n0 = static_cast<int>(blockIdx.x) / SPLITS * kCols;
   const int xrows = sh.xrows, m0 = static_cast<int>(blockIdx.y) * xrows;
   const int rows = min(xrows, a.rows - m0);
+  constexpr int kParts = std::is_same<T, __nv_bfloat16>::value ? 2 : 1;  // operands of u an entry has
+  constexpr int kPerStage = 4 / kParts;                                    // entries a stage
   const int x_bytes = xrows * 128, u_bytes = xrows * 32;
   const int a_bytes = FUSED ? a.entries * kABytes : 0;
   const int stage_bytes = kWBytes + x_bytes + a_bytes;
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads)
   // CTA may still be using when another one's sums arrive
   uint8_t* own_b = smem;
   uint8_t* own_u = own_b + sh.own * kBBytes;
-  uint8_t* ring = own_u + sh.own * 2 * u_bytes;
+  uint8_t* ring = own_u + sh.own * kParts * u_bytes;
   const int own_rows = xrows / SPLITS;                            // rows rank * own_rows ..
   float* part = reinterpret_cast<float*>(ring + sh.ring_bytes);   // [xrows][kPartLd]
   float* part_in = part + xrows * kPartLd;                        // [SPLITS - 1][own_rows][kPartLd]
@@ -221,17 +221,17 @@ __global__ void __launch_bounds__(kThreads)
       } else if (e0 < e1 && ok) {
         int chunk = __ldg(a.entry_chunk + e0);
         grid_dep_wait();  // u is complete
-        for (int e = e0; e < e1; e += 2) {
-          const int n = min(2, e1 - e);
+        for (int e = e0; e < e1; e += kPerStage) {
+          const int n = min(kPerStage, e1 - e);
           ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag);
           if (!ok) break;
           uint8_t* sb = ring + stage * stage_bytes;
-          mbar_arrive_expect_tx(&full[stage], n * (kBBytes + 2 * u_bytes));
+          mbar_arrive_expect_tx(&full[stage], n * (kBBytes + kParts * u_bytes));
           for (int i = 0; i < n; ++i) {
-            uint8_t* su = sb + kWBytes + i * 2 * u_bytes;
+            uint8_t* su = sb + kWBytes + i * kParts * u_bytes;
             tma_load_2d(sb + i * kBBytes, &maps.b, 0, chunk * a.b_rows + n0, &full[stage]);
             tma_load_2d(su, &maps.u, 0, (e + i) * kLoraBlock + m0, &full[stage]);
-            tma_load_2d(su + u_bytes, &maps.u, 16, (e + i) * kLoraBlock + m0, &full[stage]);
+            if (kParts == 2) tma_load_2d(su + u_bytes, &maps.u, 16, (e + i) * kLoraBlock + m0, &full[stage]);
             if (e + i + 1 < e1) chunk = __ldg(a.entry_chunk + e + i + 1);
           }
           next();
@@ -276,16 +276,16 @@ __global__ void __launch_bounds__(kThreads)
         next();
       }
       if constexpr (!FUSED) {
-        for (int e = e0; e < e1 && ok; e += 2) {
+        for (int e = e0; e < e1 && ok; e += kPerStage) {
           ok = mbar_wait_bounded(&full[stage], phase, a.err, kErrLoraWait, abort_flag);
           if (!ok) break;
           tc_fence_after();
           const uint32_t b_addr = smem_u32(ring + stage * stage_bytes);
-          for (int i = 0; i < min(2, e1 - e); ++i) {
+          for (int i = 0; i < min(kPerStage, e1 - e); ++i) {
             const uint64_t db = umma_desc_sw32(b_addr + i * kBBytes);
-            const uint32_t su = b_addr + kWBytes + i * 2 * u_bytes;
+            const uint32_t su = b_addr + kWBytes + i * kParts * u_bytes;
             umma_f16(tmem, db, umma_desc_sw32(su), idesc, 1u);
-            umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
+            if (kParts == 2) umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
           }
           next();
         }
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int e = e0; e < e1; ++e) {
       // thread: half (8 of 16 rank values) of row threadIdx.x / 2
       const int slot = a.chunk[e] / a.chunks_per_slot;
-      uint8_t* hi_op = own_u + (e - e0) * 2 * u_bytes;
+      uint8_t* hi_op = own_u + (e - e0) * kParts * u_bytes;
       const int m = static_cast<int>(threadIdx.x >> 1), h = threadIdx.x & 1;
       if (m >= xrows) continue;
       uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads)
       // 32-byte swizzle: 16-byte piece h of row m at piece h ^ (m / 4 % 2)
       const int at = m * 32 + ((h ^ ((m >> 2) & 1)) << 4);
       *reinterpret_cast<uint4*>(hi_op + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(hi_op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      if (kParts == 2) *reinterpret_cast<uint4*>(hi_op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     tc_fence_before();
     fence_proxy_async_smem();
@@ -364,9 +364,9 @@ __global__ void __launch_bounds__(kThreads)
           tc_fence_after();
           for (int i = 0; i < e1 - e0; ++i) {
             const uint64_t db = umma_desc_sw32(smem_u32(own_b + i * kBBytes));
-            const uint32_t su = smem_u32(own_u + i * 2 * u_bytes);
+            const uint32_t su = smem_u32(own_u + i * kParts * u_bytes);
             umma_f16(tmem, db, umma_desc_sw32(su), idesc, 1u);
-            umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
+            if (kParts == 2) umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
           }
         }
         umma_commit(&done2);
@@ -491,7 +491,8 @@ cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const 
   while (splits < 8 && 2 * splits <= a.num_kb && 2 * splits * tiles <= room_ctas) splits *= 2;
   sh.own = fused ? (a.entries + splits - 1) / splits : 0;
   const int stage_bytes = kWBytes + sh.xrows * 128 + (fused ? a.entries * kABytes : 0);
-  const int steps = (a.num_kb + splits - 1) / splits + (fused ? 0 : ((a.entries + splits - 1) / splits + 1) / 2);
+  const int per_stage = a.bf16 ? 2 : 4;
+  const int steps = (a.num_kb + splits - 1) / splits + (fused ? 0 : ((a.entries + splits - 1) / splits + per_stage - 1) / per_stage);
   const size_t parts =
       sizeof(float) * sh.xrows * (2 * kPartLd + (fused ? (a.entries + (splits - 1) * sh.own) * kPartULd : 0));
   // fused: the last stage's A operand is read as 128 rows; what follows is the

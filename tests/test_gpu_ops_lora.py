@@ -8,11 +8,12 @@ step (16 terms) after aligning them to the largest, keeping at least 2 bits
 below an f32 mantissa's, and truncates: under 2^-22 of the magnitudes for each
 of its in / 16 steps, so 2^-22 (in / 16 + 1) in all, which is no more than
 (in + 16) 2^-24 for in >= 3 * 16 and covered by the bound below with the
-factor 4.  The pair that carries x A^T keeps 2 eps^2 of it (eps: half a step
-of the type), the scale rounds once.  So
-  |error| <= 4 (in + rank + 32) 2^-24 (S1 + S2) + 2 eps^2 S2
+factor 4.  Between the products scale x A^T is rounded to one f16 (off by at
+most eps, half a step, of each value) or to a pair of bf16 (2 eps^2), and the
+scale rounds once.  So
+  |error| <= 4 (in + rank + 32) 2^-24 (S1 + S2) + r S2,  r = eps (f16), 2 eps^2 (bf16)
 and y rounds by at most eps |y| (2^-25 for f16 values below its normal range;
-remainders below f16's normal range add rank 2^-25 |B|).
+rank values below f16's normal range add 2^-25 sum_j |B_j|).
 """
 import numpy as np
 import pytest
@@ -82,7 +83,8 @@ class Case:
                 rank = max(rank, a.shape[0])
             row += r
         eps = torch.finfo(DT[self.type]).eps / 2
-        tol = 4 * (self.inn + rank + 32) * 2.0 ** -24 * (s1 + s2) + 2 * eps * eps * s2 + tiny
+        between = eps if self.type == ops.F16 else 2 * eps * eps
+        tol = 4 * (self.inn + rank + 32) * 2.0 ** -24 * (s1 + s2) + between * s2 + tiny
         return y, tol
 
     def check(self):
