@@ -9,7 +9,7 @@
  * Neither has a counterpart in the reference (zerodegress/laya-rust), whose
  * rotation exists only inside its attention (src/graph.rs:62-84,
  * src/backend/cuda/kernels.rs:135-163) and which has no adapters.  The engine
- * runs them too: laya_set_rope_scaling.
+ * runs them too: laya_forward_adapted, laya_set_rope_scaling.
  *
  * Conventions are those of laya_b200.h: LAYA_OK (0) or a nonzero status with
  * the message in laya_last_error(), nothing aborts.  Device buffers are the
@@ -155,7 +155,36 @@ int laya_lora_layout(const int32_t *rows, const int32_t *slot, int n, const int3
                      int64_t *blocks, int64_t *entries, int32_t *off, int64_t cap_blocks, int32_t *chunks,
                      int64_t cap_entries);
 
-/* ---- the engine -------------------------------------------------------------------- */
+/* ---- the engine --------------------------------------------------------------------
+ * Adapters of many tenants in one forward: each sequence of a request names its
+ * adapter, or none, and the encoder's four projections (Wqkv, Wo, Wi, mlp.Wo) add
+ * that adapter's part in their accumulator, before RoPE, GeGLU and the residual.
+ * All sequences still share every launch.
+ *
+ * laya_adapters_create: room for `slots` adapters of rank <= max_rank on every
+ * encoder projection (14.5 MB per slot and 16 ranks); replaces the slots there
+ * were.  laya_adapter_create empties a slot and gives it its rank and scale,
+ * with no matrices: it then changes nothing.  laya_adapter_upload sets the
+ * matrices of one projection, named like its weight
+ * ("encoder.layers.{i}.attn.Wqkv.weight", "...attn.Wo.weight",
+ * "...mlp.Wi.weight", "...mlp.Wo.weight"): a [rank, in] and b [out, rank] with
+ * in and out as the weight is stored, host arrays of `host_type`, rounded to f16
+ * (values must be finite in f16).  laya_adapter_drop empties the slot.  These
+ * wait for the engine's queued work and retire captured graphs, as a weight
+ * upload does. */
+int laya_adapters_create(laya_engine *e, int slots, int max_rank);
+int laya_adapter_create(laya_engine *e, int slot, int rank, float scale);
+int laya_adapter_upload(laya_engine *e, int slot, const char *name, const void *a, const void *b, int host_type);
+int laya_adapter_drop(laya_engine *e, int slot);
+/* laya_forward, sequence i with the adapter adapter[i] (a created slot) or
+ * LAYA_LORA_NONE; adapter [n], host.  A sequence's answer does not depend, not
+ * by a bit, on which adapters the other sequences of the request have; one
+ * without an adapter gets its answer of laya_forward on the same request. */
+int laya_forward_adapted(laya_engine *e, const laya_req *req, const int32_t *adapter, float *logits, float *act);
+/* laya_plan_create with adapters; run, capture, outputs and layers as for any
+ * plan.  LAYA_E_STATE from a run: one of its slots was dropped, or changed its
+ * up16(rank), since. */
+int laya_plan_create_adapted(laya_engine *e, const laya_req *req, const int32_t *adapter, laya_plan **out);
 /* The engine's rotation with stretched frequencies, for requests longer than
  * the model was trained on: `full` for the global layers' frequencies
  * (rope.freq_full), `sliding` for the windowed layers' (rope.freq_sliding);

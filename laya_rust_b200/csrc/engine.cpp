@@ -32,6 +32,7 @@
 #include "../../include/laya_b200.h"
 #include "gguf_reader.h"
 #include "kernels.h"
+#include "lora.h"
 #include "ops_common.h"
 #include "rope.h"
 
@@ -305,11 +306,19 @@ struct HostPlan {
   std::vector<RowGroup> groups;
   std::vector<uint8_t> rowtype;
   std::vector<int8_t> mmask;
+  // low-rank adapters of the sequences (adapted requests only)
+  bool adapted = false;
+  std::vector<std::pair<int, int>> slots;  // (slot, chunks) the batch uses
+  LoraLayout lora;
+  LoraItems lora_work;
+  std::vector<int> entry_chunk, item_chunk;
 };
 
 // Offsets of each array inside one packed device buffer.
 struct PlanLayout {
-  size_t tok, pos, seq_start, seq_len, cls_row, mk_row, tiles, items, rowtype, mmask, rowseq, total;
+  size_t tok, pos, seq_start, seq_len, cls_row, mk_row, tiles, items, rowtype, mmask, rowseq;
+  size_t lora_off, row_entry, entry_chunk, lora_item, item_entry, item_chunk;  // adapted requests
+  size_t total;
 };
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -333,6 +342,14 @@ PlanLayout layout_for(const HostPlan& p) {
   L.rowtype = take(p.R);
   L.mmask = take((size_t)p.n * p.k);
   L.rowseq = take(sizeof(int) * p.R);
+  if (p.adapted) {
+    L.lora_off = take(sizeof(int) * p.lora.off.size());
+    L.row_entry = take(sizeof(int) * p.R);
+    L.entry_chunk = take(sizeof(int) * p.entry_chunk.size());
+    L.lora_item = take(sizeof(int4) * p.lora_work.item.size());
+    L.item_entry = take(sizeof(int) * p.lora_work.entry.size());
+    L.item_chunk = take(sizeof(int) * p.item_chunk.size());
+  }
   L.total = o;
   return L;
 }
@@ -349,6 +366,17 @@ void pack(const HostPlan& p, const PlanLayout& L, uint8_t* dst) {
   memcpy(dst + L.rowtype, p.rowtype.data(), p.R);
   memcpy(dst + L.mmask, p.mmask.data(), (size_t)p.n * p.k);
   memcpy(dst + L.rowseq, p.rowseq.data(), sizeof(int) * p.R);
+  if (p.adapted) {
+    auto put = [&](size_t at, const auto& v) {
+      if (!v.empty()) memcpy(dst + at, v.data(), sizeof(v[0]) * v.size());
+    };
+    put(L.lora_off, p.lora.off);
+    put(L.row_entry, p.lora.row_entry);
+    put(L.entry_chunk, p.entry_chunk);
+    put(L.lora_item, p.lora_work.item);
+    put(L.item_entry, p.lora_work.entry);
+    put(L.item_chunk, p.item_chunk);
+  }
 }
 
 // Attention tiles for the sequences of at most kAttnTcQRows tokens among
@@ -394,7 +422,7 @@ void attention_items(const std::vector<int>& start, const std::vector<int>& len,
 // n, l, k > 0 (graph.rs:93) and indexes ids / mpos / qtype unchecked
 // (cpu/mod.rs:145-153, 372-398) -- out-of-range values panic there and are
 // rejected here.
-HostPlan make_plan(const laya_req* q) {
+HostPlan make_plan(const laya_req* q, bool one_group = false) {
   if (!q) throw Error(LAYA_E_INVALID, "null request");
   if (q->n <= 0 || q->l <= 0 || q->k <= 0)
     throw Error(LAYA_E_INVALID, fmt("request needs n, l, k > 0 (got %lld, %lld, %lld)", (long long)q->n,
@@ -443,7 +471,7 @@ HostPlan make_plan(const laya_req* q) {
   }
   // two row groups of about R/2 rows, split at a sequence boundary
   int split = p.n;
-  if (p.n >= 2 && R >= kSplitMinRows && row_groups_enabled()) {
+  if (p.n >= 2 && R >= kSplitMinRows && row_groups_enabled() && !one_group) {
     int best = R;
     for (int b = 1; b < p.n; ++b) {
       const int d = std::abs(2 * p.seq_start[b] - R);
@@ -505,6 +533,7 @@ struct PlanMaps {
   GroupMaps g[2];
   CUtensorMap a_mk;                                // scorer A operand (gathered marker rows)
   CUtensorMap qkv_rows;                            // attention: 64-column x 32-row boxes of qkv
+  CUtensorMap u;                                   // adapters: the rank-space vectors
   uint64_t gen = ~0ull;                            // arena generation encoded for
 };
 
@@ -524,6 +553,20 @@ struct DevicePlan {
   const T* at(size_t off) const {
     return reinterpret_cast<const T*>(base + off);
   }
+};
+
+// One encoder projection's adapters.
+struct AdapterBank {
+  DevBuf a, b;
+  CUtensorMap a_map, b_map, b_narrow;
+  std::vector<char> has;  // slot has matrices here
+};
+
+// The adapters of a projection's rows (a null bank: none).
+struct Adapted {
+  const DevicePlan* dp = nullptr;
+  const AdapterBank* bank = nullptr;
+  int rows = 0;  // of the bank's B, per chunk
 };
 
 struct Engine {
@@ -574,6 +617,163 @@ struct Engine {
   bool stuck_next = false;
   int stuck_kind = 0;  // 0: the first GEMM, 1: the first attention launch
   unsigned long long stuck_limit_ns = 0;
+
+  // Low-rank adapters on the encoder projections (laya_adapters_create): per
+  // projection the chunks of every slot (lora.h), and the rank-space vectors of
+  // the running batch, shared by all launches of the engine's stream.
+  enum Proj { kProjQkv, kProjWo, kProjWi, kProjWo2, kProjs };
+  using Bank = AdapterBank;
+  std::vector<Bank> banks;      // [layer * kProjs + projection]
+  int slots = 0, slot_chunks = 0;
+  std::vector<int> slot_rank;   // 0: empty
+  DevBuf slot_scale, u;
+
+  static int proj_in(int p) { return p == kProjWo2 ? INTER : H; }
+  static int proj_out(int p) { return p == kProjQkv ? 3 * H : p == kProjWi ? 2 * INTER : H; }
+  // rows of the projection's weight on the device
+  static int proj_rows(int p) { return p == kProjWi ? 2 * INTER_PAD : proj_out(p); }
+
+  void wait_idle() {
+    ck(cudaStreamSynchronize(stream), "sync");
+    ck(cudaStreamSynchronize(side), "sync");
+  }
+
+  void adapters_create(int n, int max_rank) {
+    if (!finalized) throw Error(LAYA_E_STATE, "engine has no weights (call laya_finalize)");
+    if (n < 1 || n > LAYA_LORA_MAX_SLOTS) throw Error(LAYA_E_INVALID, "adapters: slots must be 1..LAYA_LORA_MAX_SLOTS");
+    if (max_rank < 1 || max_rank > LAYA_LORA_MAX_RANK)
+      throw Error(LAYA_E_INVALID, "adapters: max_rank must be 1..LAYA_LORA_MAX_RANK");
+    const int cps = lora_chunks(max_rank);
+    const size_t chunks = (size_t)n * cps;
+    // chunks are addressed through 32-bit TMA row coordinates
+    if (chunks * (2 * INTER_PAD) >= ((size_t)1 << 31)) throw Error(LAYA_E_INVALID, "adapters: slots * max_rank is too large");
+    set_device();
+    wait_idle();
+    ++arena_gen;
+    banks.clear();
+    slots = 0;
+    try {
+      std::vector<Bank> v(NLAYER * kProjs);
+      for (int i = 0; i < NLAYER * kProjs; ++i) {
+        const int p = i % kProjs;
+        const size_t an = chunks * kLoraChunk * proj_in(p) * 2, bn = chunks * kLoraChunk * proj_rows(p) * 2;
+        v[i].a.alloc(an, "adapters");
+        v[i].b.alloc(bn, "adapters");
+        ck(cudaMemsetAsync(v[i].a.p, 0, an, stream), "adapters clear");
+        ck(cudaMemsetAsync(v[i].b.p, 0, bn, stream), "adapters clear");
+        if (make_tmap_pitched(&v[i].a_map, v[i].a.p, false, chunks * kLoraChunk, proj_in(p), proj_in(p), kLoraChunk) ||
+            make_tmap_lora(&v[i].b_map, v[i].b.p, false, chunks * proj_rows(p), kLoraChunk, kGemmBBoxRows) ||
+            make_tmap_lora(&v[i].b_narrow, v[i].b.p, false, chunks * proj_rows(p), kLoraChunk, kGemmBBoxRowsNarrow))
+          throw Error(LAYA_E_CUDA, "tensor map encode failed for the adapters");
+        v[i].has.assign(n, 0);
+      }
+      slot_scale.alloc(sizeof(float) * n, "adapters");
+      ck(cudaMemsetAsync(slot_scale.p, 0, sizeof(float) * n, stream), "adapters clear");
+      ck(cudaStreamSynchronize(stream), "adapters clear");
+      banks = std::move(v);
+    } catch (...) {
+      cudaGetLastError();
+      throw;
+    }
+    slots = n;
+    slot_chunks = cps;
+    slot_rank.assign(n, 0);
+  }
+
+  void require_slot(int slot) const {
+    if (slot < 0 || slot >= slots) throw Error(LAYA_E_INVALID, fmt("adapter slot %d out of range (%d slots)", slot, slots));
+  }
+
+  void adapter_create(int slot, int rank, float scale) {
+    require_slot(slot);
+    if (rank < 1 || lora_chunks(rank) > slot_chunks) throw Error(LAYA_E_INVALID, "adapter: rank must be 1..max_rank");
+    if (!std::isfinite(scale)) throw Error(LAYA_E_INVALID, "adapter: scale is not finite");
+    adapter_drop(slot);
+    upload_sync(slot_scale.as<float>() + slot, &scale, sizeof scale, "adapter scale");
+    slot_rank[slot] = rank;
+  }
+
+  void adapter_drop(int slot) {
+    require_slot(slot);
+    set_device();
+    wait_idle();
+    ++arena_gen;
+    slot_rank[slot] = 0;
+    for (int i = 0; i < NLAYER * kProjs; ++i) {
+      Bank& b = banks[i];
+      if (!b.has[slot]) continue;
+      const size_t an = (size_t)slot_chunks * kLoraChunk * proj_in(i % kProjs) * 2;
+      const size_t bn = (size_t)slot_chunks * kLoraChunk * proj_rows(i % kProjs) * 2;
+      ck(cudaMemsetAsync(b.a.as<uint8_t>() + an * slot, 0, an, stream), "adapter clear");
+      ck(cudaMemsetAsync(b.b.as<uint8_t>() + bn * slot, 0, bn, stream), "adapter clear");
+      b.has[slot] = 0;
+    }
+    ck(cudaStreamSynchronize(stream), "adapter clear");
+  }
+
+  void adapter_upload(int slot, const std::string& name, const void* a, const void* b, int type) {
+    require_slot(slot);
+    if (slot_rank[slot] == 0) throw Error(LAYA_E_STATE, fmt("adapter slot %d is empty (call laya_adapter_create)", slot));
+    if (type != LAYA_F16 && type != LAYA_BF16 && type != LAYA_F32) throw Error(LAYA_E_INVALID, "adapter: unknown type");
+    int which = -1;
+    static const char* const kNames[kProjs] = {"attn.Wqkv.weight", "attn.Wo.weight", "mlp.Wi.weight", "mlp.Wo.weight"};
+    for (int i = 0; i < NLAYER * kProjs && which < 0; ++i)
+      if (name == fmt("encoder.layers.%d.%s", i / kProjs, kNames[i % kProjs])) which = i;
+    if (which < 0) throw Error(LAYA_E_INVALID, "adapter: " + name + " is not an encoder projection");
+    const int p = which % kProjs, rank = slot_rank[slot];
+    std::vector<int> row_of;
+    if (p == kProjWi) {
+      // the weight's gate/up co-tiling (see upload)
+      row_of.resize(2 * INTER);
+      for (int g = 0; g < INTER; ++g) {
+        row_of[g] = 256 * (g / 128) + g % 128;
+        row_of[INTER + g] = row_of[g] + 128;
+      }
+    }
+    const std::vector<uint16_t> ha = lora_pack_a(a, type, rank, proj_in(p), proj_in(p), false);
+    const std::vector<uint16_t> hb = lora_pack_b(b, type, rank, proj_out(p), proj_rows(p), false, row_of);
+    set_device();
+    wait_idle();
+    ++arena_gen;
+    Bank& k = banks[which];
+    upload_sync(k.a.as<uint16_t>() + (size_t)slot * slot_chunks * kLoraChunk * proj_in(p), ha.data(), ha.size() * 2,
+                "adapter upload");
+    upload_sync(k.b.as<uint16_t>() + (size_t)slot * slot_chunks * kLoraChunk * proj_rows(p), hb.data(), hb.size() * 2,
+                "adapter upload");
+    k.has[slot] = 1;
+  }
+
+  // The request's plan with the adapters of its sequences.
+  HostPlan make_adapted_plan(const laya_req* q, const int32_t* adapter) {
+    if (!adapter) throw Error(LAYA_E_INVALID, "null adapter array");
+    HostPlan p = make_plan(q, true);
+    std::vector<int> chunks(slots);
+    for (int i = 0; i < slots; ++i) chunks[i] = lora_chunks(slot_rank[i]);
+    for (int b = 0; b < p.n; ++b)
+      if (adapter[b] != LAYA_LORA_NONE && (adapter[b] < 0 || adapter[b] >= slots || chunks[adapter[b]] == 0))
+        throw Error(LAYA_E_INVALID, fmt("row %d: adapter %d is not a created slot", b, adapter[b]));
+    p.lora = lora_layout(p.seq_len.data(), adapter, p.n, chunks);
+    p.lora_work = lora_items(p.lora, num_sms);
+    p.adapted = !p.lora.chunk.empty();
+    for (const int2& c : p.lora.chunk) {
+      p.entry_chunk.push_back(c.x * slot_chunks + c.y);
+      if (c.y == 0) p.slots.emplace_back(c.x, chunks[c.x]);
+    }
+    std::sort(p.slots.begin(), p.slots.end());
+    p.slots.erase(std::unique(p.slots.begin(), p.slots.end()), p.slots.end());
+    for (int e : p.lora_work.entry) p.item_chunk.push_back(p.entry_chunk[e]);
+    return p;
+  }
+
+  // A plan made earlier: its slots must be as they were.
+  void check_slots(const HostPlan& p) const {
+    for (const auto& s : p.slots)
+      if (s.first >= slots || lora_chunks(slot_rank[s.first]) != s.second)
+        throw Error(LAYA_E_STATE, fmt("adapter slot %d was dropped or changed its rank since the plan was made", s.first));
+    for (size_t i = 0; i < p.entry_chunk.size(); ++i)
+      if (p.entry_chunk[i] != p.lora.chunk[i].x * slot_chunks + p.lora.chunk[i].y)
+        throw Error(LAYA_E_STATE, "the adapter slots were created anew since the plan was made");
+  }
 
   // decision-tail weight pointers, looked up once (see tail_weights)
   TailWeights tail_cache{};
@@ -835,6 +1035,11 @@ struct Engine {
   void ensure_arena(const HostPlan& p) {
     ensure_rope(p.l);
     ensure_parts();
+    if (p.adapted && u.bytes < p.lora.chunk.size() * lora_entry_elems(false) * 2) {
+      wait_idle();
+      ++arena_gen;
+      u.alloc(p.lora.chunk.size() * lora_entry_elems(false) * 2 * 2, "adapter workspace");
+    }
     const int rows = (p.R + kGemmBM - 1) / kGemmBM * kGemmBM;
     const int mk = (p.n * p.k + kGemmBM - 1) / kGemmBM * kGemmBM;
     if (rows <= cap_rows && mk <= cap_mk && p.n <= cap_n) return;
@@ -926,13 +1131,46 @@ struct Engine {
             make_tmap_2d(&q.o_gate, gate.as<__half>() + r0 * INTER, false, rows, INTER, 64, ob) ||
             make_tmap_2d(&q.o_hmlp, hmlp.as<__half>() + r0 * HEAD_INTER, false, rows, HEAD_INTER, 64, ob);
     }
+    if (!bad && p.adapted)
+      bad = make_tmap_lora(&m.u, u.p, false, p.lora.chunk.size() * kLoraBlock, kLoraChunk, kGemmABoxRows) != 0;
     if (bad) throw Error(LAYA_E_CUDA, "tensor map encode failed for the arena");
     m.gen = arena_gen;
   }
 
   // ---- the forward ---------------------------------------------------------------
+  // The projection's adapters, if a slot of the batch has matrices there.
+  Adapted adapted(const DevicePlan& dp, int layer, int proj) const {
+    if (!dp.host.adapted) return {};
+    const Bank& b = banks[layer * kProjs + proj];
+    for (const auto& s : dp.host.slots)
+      if (b.has[s.first]) return {&dp, &b, proj_rows(proj)};
+    return {};
+  }
+
   void gemm(int epi, const CUtensorMap& A, const Weight& Wt, const CUtensorMap& Out, int M, int N, int K, GemmArgs a,
-            cudaStream_t s, int64_t& nl, int kind, const CUtensorMap* out2 = nullptr) {
+            cudaStream_t s, int64_t& nl, int kind, const CUtensorMap* out2 = nullptr, const Adapted& ad = Adapted()) {
+    if (ad.bank) {
+      // the rank-space product of the rows, from the same operand; the GEMM
+      // waits for it only before its adapter steps
+      const DevicePlan& dp = *ad.dp;
+      LoraShrinkArgs r{};
+      r.item = dp.at<int4>(dp.lay.lora_item);
+      r.item_entry = dp.at<int>(dp.lay.item_entry);
+      r.item_chunk = dp.at<int>(dp.lay.item_chunk);
+      r.items = (int)dp.host.lora_work.item.size();
+      r.group = dp.host.lora_work.group;
+      r.row_entry = dp.at<int>(dp.lay.row_entry);
+      r.entry_chunk = dp.at<int>(dp.lay.entry_chunk);
+      r.scale = slot_scale.as<float>();
+      r.u = u.p;
+      r.rows = M;
+      r.num_kb = K / kGemmBK;
+      r.chunks_per_slot = slot_chunks;
+      r.err = err.as<int>();
+      ck(launch_lora_shrink(A, ad.bank->a_map, r, num_sms, s), "adapter launch");
+      ++nl;
+      mark(kind);
+    }
     a.M = M;
     a.N = N;
     a.K = K;
@@ -951,8 +1189,12 @@ struct Engine {
     const int tiles256 = ((M + kGemmBM - 1) / kGemmBM) * (N / kGemmBN);
     const bool narrow = narrow_enabled() && tiles256 * 2 <= num_sms / 2 &&
                         (epi == kEpiQkvRope || epi == kEpiQkvBias || epi == kEpiGeglu || epi == kEpiBiasRelu);
+    GemmExt ext{};
+    if (ad.bank)
+      ext = GemmExt{&ad.dp->maps.u, narrow ? &ad.bank->b_narrow : &ad.bank->b_map, ad.dp->at<int>(ad.dp->lay.lora_off),
+                    ad.dp->at<int>(ad.dp->lay.entry_chunk), ad.rows, true};
     ck(launch_gemm(epi, GemmMaps{&A, narrow ? &Wt.tmap_narrow : &Wt.tmap, &Out, out2}, a, num_sms, s,
-                   narrow ? kGemmBNNarrow : kGemmBN),
+                   narrow ? kGemmBNNarrow : kGemmBN, ad.bank ? &ext : nullptr),
        "gemm launch");
     ++nl;
     mark(kind);
@@ -1021,7 +1263,7 @@ struct Engine {
   // (a LayerNorm of the same rows comes next) and a small M, the K loop is
   // split and the sums stay pending for that LayerNorm.
   void resid_gemm(int gi, const CUtensorMap& A, const Weight& Wt, const CUtensorMap& Out, int R, int K, cudaStream_t s,
-                  int64_t& nl, int kind, bool defer, const float* bias = nullptr) {
+                  int64_t& nl, int kind, bool defer, const float* bias = nullptr, const Adapted& ad = Adapted()) {
     GemmArgs r{};
     r.ldo = H;
     r.bias = bias;
@@ -1030,7 +1272,7 @@ struct Engine {
       int tail_rb = 0, ts = 0;
       if (defer) choose_tail(R, K, tail_rb, ts);
       if (ts < 2) {
-        gemm(kEpiResid, A, Wt, Out, R, H, K, r, s, nl, kind);
+        gemm(kEpiResid, A, Wt, Out, R, H, K, r, s, nl, kind, nullptr, ad);
         return;
       }
       if (pend[gi].nparts > 0) throw Error(LAYA_E_STATE, "split-K parts of an earlier GEMM were not consumed");
@@ -1039,14 +1281,14 @@ struct Engine {
       r.main_tiles = (num_m - tail_rb) * num_n;
       r.tail_row0 = (num_m - tail_rb) * kGemmBM;
       r.split_rows = tail_rb * kGemmBM;
-      gemm(kEpiResidTail, A, Wt, Out, R, H, K, r, s, nl, kind, &parts_map[gi]);
+      gemm(kEpiResidTail, A, Wt, Out, R, H, K, r, s, nl, kind, &parts_map[gi], ad);
       pend[gi] = PendingParts{parts[gi].as<float>(), ts, (size_t)r.split_rows * H, r.tail_row0};
       return;
     }
     if (pend[gi].nparts > 0) throw Error(LAYA_E_STATE, "split-K parts of an earlier GEMM were not consumed");
     r.splits = S;
     r.split_rows = (R + kGemmBM - 1) / kGemmBM * kGemmBM;
-    gemm(kEpiPartial, A, Wt, parts_map[gi], R, H, K, r, s, nl, kind);
+    gemm(kEpiPartial, A, Wt, parts_map[gi], R, H, K, r, s, nl, kind, nullptr, ad);
     pend[gi] = PendingParts{parts[gi].as<float>(), S, (size_t)r.split_rows * H};
   }
 
@@ -1080,17 +1322,18 @@ struct Engine {
     q.sinb = global ? sin_full.as<float>() : sin_slide.as<float>();
     q.scale = SCALE;
     gemm(kEpiQkvRope, M.a_t16, W(fmt("encoder.layers.%d.attn.Wqkv.weight", layer)), M.o_qkv, R, 3 * H, H, q, s, nl,
-         kProfQkv);
+         kProfQkv, nullptr, adapted(dp, layer, kProjQkv));
     attention(dp, gi, global ? -1 : WINDOW, s, nl);
-    resid_gemm(gi, M.a_ctx, W(fmt("encoder.layers.%d.attn.Wo.weight", layer)), M.o_x, R, H, s, nl, kProfWo, true);
+    resid_gemm(gi, M.a_ctx, W(fmt("encoder.layers.%d.attn.Wo.weight", layer)), M.o_x, R, H, s, nl, kProfWo, true, nullptr,
+               adapted(dp, layer, kProjWo));
     row_ln(gi, xg, fmt("encoder.layers.%d.mlp_norm.weight", layer), nullptr, tg, R, s, nl);
     GemmArgs gg{};
     gg.ldo = INTER;
     gg.n_valid = INTER;
     gemm(kEpiGeglu, M.a_t16, W(fmt("encoder.layers.%d.mlp.Wi.weight", layer)), M.o_gate, R, 2 * INTER_PAD, H, gg, s,
-         nl, kProfWi);
+         nl, kProfWi, nullptr, adapted(dp, layer, kProjWi));
     resid_gemm(gi, M.a_gate, W(fmt("encoder.layers.%d.mlp.Wo.weight", layer)), M.o_x, R, INTER, s, nl, kProfWo2,
-               true);
+               true, nullptr, adapted(dp, layer, kProjWo2));
   }
 
   // Adds row group gi's pending split-K parts to its residual rows.
@@ -1205,6 +1448,13 @@ struct Engine {
     ck(cudaStreamWaitEvent(stream, ev_join, 0), "join wait");
   }
 
+  // Rows of other adapters are zero in u's entries; every launch of the batch
+  // writes the same rows, so one clear per forward is enough.
+  void clear_u(const HostPlan& p) {
+    if (p.adapted)
+      ck(cudaMemsetAsync(u.p, 0, p.lora.chunk.size() * lora_entry_elems(false) * 2, stream), "adapter workspace clear");
+  }
+
   // Enqueues one forward of plan `dp` (graph.rs:86-186).
   int64_t enqueue(DevicePlan& dp, laya_tap_fn tap = nullptr, void* user = nullptr) {
     ensure_maps(dp);
@@ -1212,6 +1462,7 @@ struct Engine {
     const int G = (int)p.groups.size();
     const bool conc = G > 1 && !tap && !prof_ev;
     int64_t nl = 0;
+    clear_u(p);
     fork(conc);
     for (int gi = 0; gi < G; ++gi) {
       const RowGroup& g = p.groups[gi];
@@ -1256,6 +1507,7 @@ struct Engine {
     const int G = (int)dp.host.groups.size();
     const bool conc = G > 1 && !prof_ev;
     int64_t nl = 0;
+    clear_u(dp.host);
     fork(conc);
     pend[0] = pend[1] = PendingParts();
     for (int gi = 0; gi < G; ++gi) {
@@ -1379,6 +1631,15 @@ struct Engine {
                               (int64_t)L.seq_len, (int64_t)L.cls_row, (int64_t)L.mk_row, (int64_t)L.tiles,
                               (int64_t)L.items, (int64_t)L.rowtype, (int64_t)L.mmask, (int64_t)L.rowseq,
                               (int64_t)L.total, (int64_t)rope_len, parts_ready ? 1 : 0};
+    if (p.adapted) {
+      for (size_t v : {L.lora_off, L.row_entry, L.entry_chunk, L.lora_item, L.item_entry, L.item_chunk, p.lora.chunk.size(),
+                       p.lora_work.item.size(), (size_t)p.lora_work.group})
+        k.push_back((int64_t)v);
+      // which projections have launches of their own for adapters follows from
+      // the slots (and the bank, whose changes bump arena_gen)
+      for (const auto& s : p.slots) k.push_back(s.first);
+      k.push_back(-2);
+    }
     for (const RowGroup& g : p.groups) {
       k.push_back(g.row0);
       k.push_back(g.rows);
@@ -1433,12 +1694,13 @@ struct Engine {
     return exec;
   }
 
-  void forward(const laya_req* q, float* logits, float* act, laya_tap_fn tap, void* user) {
+  void forward(const laya_req* q, float* logits, float* act, laya_tap_fn tap, void* user,
+               const int32_t* adapter = nullptr) {
     if (!finalized) throw Error(LAYA_E_STATE, "engine has no weights (call laya_finalize)");
     if (!logits || !act) throw Error(LAYA_E_INVALID, "null output buffer");
     set_device();
     DevicePlan dp;
-    dp.host = make_plan(q);
+    dp.host = adapter ? make_adapted_plan(q, adapter) : make_plan(q);
     ensure_arena(dp.host);
     upload_plan(dp, true);
     // taps read the stream between layers and the timeout test needs its
@@ -1684,11 +1946,61 @@ int laya_plan_create(laya_engine* e, const laya_req* req, laya_plan** out) {
   });
 }
 
+int laya_adapters_create(laya_engine* e, int slots, int max_rank) {
+  return guard([&] {
+    if (!e) throw Error(LAYA_E_INVALID, "null engine");
+    e->e->adapters_create(slots, max_rank);
+  });
+}
+
+int laya_adapter_create(laya_engine* e, int slot, int rank, float scale) {
+  return guard([&] {
+    if (!e) throw Error(LAYA_E_INVALID, "null engine");
+    e->e->adapter_create(slot, rank, scale);
+  });
+}
+
+int laya_adapter_upload(laya_engine* e, int slot, const char* name, const void* a, const void* b, int host_type) {
+  return guard([&] {
+    if (!e || !name || !a || !b) throw Error(LAYA_E_INVALID, "null argument");
+    e->e->adapter_upload(slot, name, a, b, host_type);
+  });
+}
+
+int laya_adapter_drop(laya_engine* e, int slot) {
+  return guard([&] {
+    if (!e) throw Error(LAYA_E_INVALID, "null engine");
+    e->e->adapter_drop(slot);
+  });
+}
+
+int laya_forward_adapted(laya_engine* e, const laya_req* req, const int32_t* adapter, float* logits, float* act) {
+  return guard([&] {
+    if (!e || !adapter) throw Error(LAYA_E_INVALID, "null argument");
+    e->e->forward(req, logits, act, nullptr, nullptr, adapter);
+  });
+}
+
+int laya_plan_create_adapted(laya_engine* e, const laya_req* req, const int32_t* adapter, laya_plan** out) {
+  return guard([&] {
+    if (!e || !adapter || !out) throw Error(LAYA_E_INVALID, "null argument");
+    Engine& g = *e->e;
+    if (!g.finalized) throw Error(LAYA_E_STATE, "engine has no weights (call laya_finalize)");
+    g.set_device();
+    std::unique_ptr<laya_plan> p(new laya_plan());
+    p->dp.host = g.make_adapted_plan(req, adapter);
+    g.ensure_arena(p->dp.host);
+    g.upload_plan(p->dp, false);
+    *out = p.release();
+  });
+}
+
 int laya_plan_run(laya_engine* e, laya_plan* p) {
   return guard([&] {
     if (!e || !p) throw Error(LAYA_E_INVALID, "null argument");
     Engine& g = *e->e;
     g.set_device();
+    g.check_slots(p->dp.host);
     g.ensure_arena(p->dp.host);
     if (p->dp.graph && p->dp.graph_arena_gen != g.arena_gen) {
       // the arena moved since capture: the graph holds stale pointers
@@ -1708,6 +2020,7 @@ int laya_plan_capture(laya_engine* e, laya_plan* p) {
     if (!e || !p) throw Error(LAYA_E_INVALID, "null argument");
     Engine& g = *e->e;
     g.set_device();
+    g.check_slots(p->dp.host);
     g.ensure_arena(p->dp.host);
     // one eager run first: per-device kernel attributes are set outside capture
     g.enqueue(p->dp);
@@ -1756,6 +2069,7 @@ int laya_plan_profile(laya_engine* e, laya_plan* p, int steps, double* ms, int64
     if (!e || !p || !ms || !launches || steps <= 0) throw Error(LAYA_E_INVALID, "bad argument");
     Engine& g = *e->e;
     g.set_device();
+    g.check_slots(p->dp.host);
     g.ensure_arena(p->dp.host);
     g.profile(p->dp, steps, ms, launches);
     g.check_device_error();
@@ -1830,6 +2144,7 @@ int laya_plan_run_layer(laya_engine* e, laya_plan* p, int layer) {
     if (layer < 0 || layer >= laya::NLAYER) throw Error(LAYA_E_INVALID, "layer out of range (0..27)");
     Engine& g = *e->e;
     g.set_device();
+    g.check_slots(p->dp.host);
     g.ensure_arena(p->dp.host);
     g.enqueue_layer(p->dp, layer);
   });

@@ -375,8 +375,10 @@ cudaError_t launch_lora_shrink(const CUtensorMap& x, const CUtensorMap& a_map, c
                                cudaStream_t s) {
   if (a.items <= 0) return cudaSuccess;
   if (a.num_kb < 1 || a.group < 1 || a.group > kLoraMaxGroup) return cudaErrorInvalidValue;
-  int splits = 1;
-  while (splits < 8 && 2 * splits * a.items <= num_sms && 4 * splits <= a.num_kb) splits *= 2;
+  // by the rows and K alone: a row's sums keep their order whatever adapters
+  // the other rows have
+  int splits = lora_splits(a.rows, num_sms);
+  while (splits > 1 && 2 * splits > a.num_kb) splits /= 2;
   return a.bf16 ? launch_shrink<__nv_bfloat16>(splits, x, a_map, a, s) : launch_shrink<__half>(splits, x, a_map, a, s);
 }
 
@@ -384,6 +386,13 @@ cudaError_t launch_lora_pairs(const LoraPairsArgs& a, cudaStream_t s) {
   if (a.pairs <= 0) return cudaSuccess;
   auto* kernel = a.bf16 ? &lora_pairs_kernel<__nv_bfloat16> : &lora_pairs_kernel<__half>;
   return launch_pdl(kernel, dim3(a.pairs), dim3(256), 0, s, nullptr, 0, a);
+}
+
+int lora_splits(int rows, int num_sms) {
+  const int halves = (rows + kLoraItemRows - 1) / kLoraItemRows;
+  int splits = 1;
+  while (splits < 8 && 2 * splits * halves <= num_sms) splits *= 2;
+  return splits;
 }
 
 LoraItems lora_items(const LoraLayout& L, int num_sms) {
@@ -403,10 +412,11 @@ LoraItems lora_items(const LoraLayout& L, int num_sms) {
     }
   }
   // the smallest group whose items still run at once
+  const size_t most = num_sms / lora_splits(L.rows, num_sms);
   for (it.group = 1;; it.group *= 2) {
     size_t items = 0;
     for (const auto& v : need) items += (v.size() + it.group - 1) / it.group;
-    if (items <= static_cast<size_t>(num_sms) || it.group == kLoraMaxGroup) break;
+    if (items <= most || it.group == kLoraMaxGroup) break;
   }
   for (int h = 0; h < halves; ++h)
     for (size_t i = 0; i < need[h].size(); i += it.group) {
@@ -415,6 +425,76 @@ LoraItems lora_items(const LoraLayout& L, int num_sms) {
       it.entry.insert(it.entry.end(), need[h].begin() + i, need[h].begin() + i + n);
     }
   return it;
+}
+
+namespace {
+
+float bits_f32(uint32_t u) {
+  float f;
+  memcpy(&f, &u, 4);
+  return f;
+}
+uint32_t f32_bits(float f) {
+  uint32_t u;
+  memcpy(&u, &f, 4);
+  return u;
+}
+
+float host_f32(const void* p, int type, size_t i) {
+  if (type == LAYA_F32) return static_cast<const float*>(p)[i];
+  const uint16_t v = static_cast<const uint16_t*>(p)[i];
+  if (type == LAYA_BF16) return bits_f32(static_cast<uint32_t>(v) << 16);
+  __half_raw r;
+  r.x = v;
+  return __half2float(__half(r));
+}
+
+// Nearest value of the 16-bit type, ties to even; false if it is not finite.
+bool host_bf16(float f, uint16_t* out) {
+  const uint32_t u = f32_bits(f);
+  const uint32_t r = u + 0x7fffu + ((u >> 16) & 1u);
+  *out = static_cast<uint16_t>(r >> 16);
+  return (u & 0x7f800000u) != 0x7f800000u && (r & 0x7f800000u) != 0x7f800000u;
+}
+bool host_f16(float f, uint16_t* out) {
+  const uint32_t u = f32_bits(f), sign = (u >> 16) & 0x8000u, mag = u & 0x7fffffffu;
+  if (mag >= 0x477ff000u) return false;  // rounds to 65536 or more, or is not finite
+  uint32_t h;
+  if (mag < 0x38800000u)  // below 2^-14: the sum with 1/2 rounds at 2^-24, f16's last place there
+    h = f32_bits(bits_f32(mag) + 0.5f) - 0x3f000000u;
+  else
+    h = (mag - 0x38000000u + 0x0fffu + ((mag >> 13) & 1u)) >> 13;
+  *out = static_cast<uint16_t>(sign | h);
+  return true;
+}
+uint16_t host_round(const void* p, int type, size_t i, bool bf16) {
+  // the type's own values pass through when they are finite
+  uint16_t h;
+  const float f = host_f32(p, type, i);
+  op_require(bf16 ? host_bf16(f, &h) : host_f16(f, &h), "adapter: a value is not finite in the projection's type");
+  return h;
+}
+
+}  // namespace
+
+std::vector<uint16_t> lora_pack_a(const void* a, int type, int rank, int in, int in_pad, bool bf16) {
+  std::vector<uint16_t> v(static_cast<size_t>(lora_chunks(rank)) * kLoraChunk * in_pad);
+  for (int r = 0; r < rank; ++r)
+    for (int c = 0; c < in; ++c)
+      v[static_cast<size_t>(r) * in_pad + c] = host_round(a, type, static_cast<size_t>(r) * in + c, bf16);
+  return v;
+}
+
+std::vector<uint16_t> lora_pack_b(const void* b, int type, int rank, int out, int out_pad, bool bf16,
+                                  const std::vector<int>& row_of) {
+  std::vector<uint16_t> v(static_cast<size_t>(lora_chunks(rank)) * out_pad * kLoraChunk);
+  for (int n = 0; n < out; ++n) {
+    const int row = row_of.empty() ? n : row_of[n];
+    for (int r = 0; r < rank; ++r)
+      v[(static_cast<size_t>(r / kLoraChunk) * out_pad + row) * kLoraChunk + r % kLoraChunk] =
+          host_round(b, type, static_cast<size_t>(n) * rank + r, bf16);
+  }
+  return v;
 }
 
 LoraLayout lora_layout(const int32_t* rows, const int32_t* slot, int n, const std::vector<int>& chunks_of) {
@@ -536,34 +616,6 @@ struct Plan {
   }
 };
 
-float load_host(const void* p, int type, size_t i) {
-  if (type == LAYA_F32) return static_cast<const float*>(p)[i];
-  const uint16_t v = static_cast<const uint16_t*>(p)[i];
-  if (type == LAYA_BF16) {
-    const uint32_t u = static_cast<uint32_t>(v) << 16;
-    float f;
-    memcpy(&f, &u, 4);
-    return f;
-  }
-  __half_raw r;
-  r.x = v;
-  return __half2float(__half(r));
-}
-
-uint16_t store_host(float v, bool bf16) {
-  uint16_t b;
-  if (bf16) {
-    const __nv_bfloat16 h = __float2bfloat16_rn(v);
-    op_require(std::isfinite(__bfloat162float(h)), "lora_set: a value is not finite in the projection's type");
-    memcpy(&b, &h, 2);
-  } else {
-    const __half h = __float2half_rn(v);
-    op_require(std::isfinite(__half2float(h)), "lora_set: a value is not finite in the projection's type");
-    memcpy(&b, &h, 2);
-  }
-  return b;
-}
-
 // Few (row, chunk) pairs take a block each, reading 16 rows of A from L2.
 constexpr size_t kLoraMaxPairs = 512;
 
@@ -648,20 +700,19 @@ int laya_lora_set(laya_lora* lora, int slot, int rank, const void* a, const void
     op_require(rank >= 1 && rank <= k.max_rank, "lora_set: rank must be 1..max_rank");
     op_require(host_type == LAYA_F16 || host_type == LAYA_BF16 || host_type == LAYA_F32, "lora_set: unknown type");
     op_require(std::isfinite(scale), "lora_set: scale is not finite");
-    // the slot's chunks, zero past the rank
-    std::vector<uint16_t> ha(static_cast<size_t>(k.cps) * kLoraChunk * k.in_pad), hb(static_cast<size_t>(k.cps) * kLoraChunk * k.out_pad);
-    for (int r = 0; r < rank; ++r)
-      for (int c = 0; c < k.in; ++c)
-        ha[static_cast<size_t>(r) * k.in_pad + c] = store_host(load_host(a, host_type, static_cast<size_t>(r) * k.in + c), k.bf16);
-    for (int n = 0; n < k.out; ++n)
-      for (int r = 0; r < rank; ++r)
-        hb[(static_cast<size_t>(r / kLoraChunk) * k.out_pad + n) * kLoraChunk + r % kLoraChunk] =
-            store_host(load_host(b, host_type, static_cast<size_t>(n) * rank + r), k.bf16);
+    const std::vector<uint16_t> ha = lora_pack_a(a, host_type, rank, k.in, k.in_pad, k.bf16);
+    const std::vector<uint16_t> hb = lora_pack_b(b, host_type, rank, k.out, k.out_pad, k.bf16, {});
     DeviceScope scope(k.device);
     // runs already queued on the caller's streams may still read the slot
     op_check(cudaDeviceSynchronize(), "lora_set");
-    op_check(cudaMemcpyAsync(k.a.as<uint16_t>() + ha.size() * slot, ha.data(), ha.size() * 2, cudaMemcpyHostToDevice, k.stream), "lora upload");
-    op_check(cudaMemcpyAsync(k.b.as<uint16_t>() + hb.size() * slot, hb.data(), hb.size() * 2, cudaMemcpyHostToDevice, k.stream), "lora upload");
+    const size_t na = static_cast<size_t>(k.cps) * kLoraChunk * k.in_pad, nb = static_cast<size_t>(k.cps) * kLoraChunk * k.out_pad;
+    uint16_t* da = k.a.as<uint16_t>() + na * slot;
+    uint16_t* db = k.b.as<uint16_t>() + nb * slot;
+    op_check(cudaMemcpyAsync(da, ha.data(), ha.size() * 2, cudaMemcpyHostToDevice, k.stream), "lora upload");
+    op_check(cudaMemcpyAsync(db, hb.data(), hb.size() * 2, cudaMemcpyHostToDevice, k.stream), "lora upload");
+    // chunks an earlier, larger rank used
+    op_check(cudaMemsetAsync(da + ha.size(), 0, (na - ha.size()) * 2, k.stream), "lora upload");
+    op_check(cudaMemsetAsync(db + hb.size(), 0, (nb - hb.size()) * 2, k.stream), "lora upload");
     op_check(cudaMemcpyAsync(k.scale.as<float>() + slot, &scale, 4, cudaMemcpyHostToDevice, k.stream), "lora upload");
     op_check(cudaStreamSynchronize(k.stream), "lora upload");
     k.slot[slot].rank = rank;

@@ -42,6 +42,15 @@ struct LoraLayout {
 // Throws OpError; chunks_of(slot) is the slot's chunk count, 0 if it is empty.
 LoraLayout lora_layout(const int32_t* rows, const int32_t* slot, int n, const std::vector<int>& chunks_of);
 
+// An adapter's host matrices (a [rank, in], b [out, rank], `type` LAYA_F16,
+// LAYA_BF16 or LAYA_F32) as the bank's chunks in the 16-bit type: [chunk][16][in_pad]
+// and [chunk][out_pad][16], zeros past rank, in and out.  Output row n of b goes
+// to row row_of[n] (empty: n).  Throws OpError on a value that is not finite in
+// the 16-bit type.
+std::vector<uint16_t> lora_pack_a(const void* a, int type, int rank, int in, int in_pad, bool bf16);
+std::vector<uint16_t> lora_pack_b(const void* b, int type, int rank, int out, int out_pad, bool bf16,
+                                  const std::vector<int>& row_of);
+
 // Values a row of an entry.
 constexpr int lora_u_width(bool bf16) { return bf16 ? 2 * kLoraChunk : kLoraChunk; }
 constexpr size_t lora_entry_elems(bool bf16) { return static_cast<size_t>(kLoraBlock) * lora_u_width(bf16); }
@@ -57,6 +66,9 @@ struct LoraItems {
   std::vector<int> entry;
 };
 LoraItems lora_items(const LoraLayout& L, int num_sms);
+// K parts of the rank-space product of `rows` rows: 1, 2, 4 or 8, as many as
+// one 128-row item a block leaves SMs for.
+int lora_splits(int rows, int num_sms);
 
 struct LoraShrinkArgs {
   const int4* item;

@@ -87,8 +87,23 @@ def lib():
         _i32p = ctypes.POINTER(ctypes.c_int32)
         L.laya_plan_layout.argtypes = [ctypes.POINTER(_CReq), _i64p, _i64p, _i32p, ctypes.c_int64, _i64p, _i32p,
                                        ctypes.c_int64]
+        vp_f32 = [vp, ctypes.POINTER(_CReq), _i32p, _f32p, _f32p]
+        L.laya_adapters_create.argtypes = [vp, ctypes.c_int, ctypes.c_int]
+        L.laya_adapter_create.argtypes = [vp, ctypes.c_int, ctypes.c_int, ctypes.c_float]
+        L.laya_adapter_upload.argtypes = [vp, ctypes.c_int, ctypes.c_char_p, vp, vp, ctypes.c_int]
+        L.laya_adapter_drop.argtypes = [vp, ctypes.c_int]
+        L.laya_forward_adapted.argtypes = vp_f32
+        L.laya_plan_create_adapted.argtypes = [vp, ctypes.POINTER(_CReq), _i32p, ctypes.POINTER(vp)]
         _lib = L
     return _lib
+
+
+def _adapter_array(req: "Req", adapters) -> np.ndarray:
+    """One int32 slot per sequence (-1: none)."""
+    a = np.ascontiguousarray(adapters, dtype=np.int32).ravel()
+    if a.size != req.n:
+        raise ValueError(f"{a.size} adapters for {req.n} sequences")
+    return a
 
 
 def _check(rc: int) -> None:
@@ -143,11 +158,16 @@ class EngineInfo:
 class Plan:
     """A request uploaded once to device memory (device-resident runs)."""
 
-    def __init__(self, engine: "Engine", req: Req):
+    def __init__(self, engine: "Engine", req: Req, adapters=None):
         self._e = engine
         self.req = req
         h = ctypes.c_void_p()
-        _check(lib().laya_plan_create(engine._h, ctypes.byref(req._c()), ctypes.byref(h)))
+        if adapters is None:
+            _check(lib().laya_plan_create(engine._h, ctypes.byref(req._c()), ctypes.byref(h)))
+        else:
+            a = _adapter_array(req, adapters)
+            _check(lib().laya_plan_create_adapted(engine._h, ctypes.byref(req._c()),
+                                                  a.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), ctypes.byref(h)))
         self._h = h
 
     def run(self) -> None:
@@ -216,6 +236,7 @@ class Engine:
             _check(lib().laya_open(device, os.fsencode(gguf_path), ctypes.byref(h)))
         self._h = h
         self.device = device
+        self._adapter_rank: dict[int, int] = {}  # slots created here
 
     def upload_f16(self, name: str, data: np.ndarray) -> None:
         a = np.ascontiguousarray(data, dtype=np.float16)
@@ -245,11 +266,19 @@ class Engine:
         d = json.loads(buf.value.decode())
         return EngineInfo(d["id"], d["device"], d["dtype"], d["layers"], d["calibration"])
 
-    def forward(self, req: Req, taps: dict | None = None) -> Out:
+    def forward(self, req: Req, taps: dict | None = None, adapters=None) -> Out:
+        """Engine::forward; `adapters`: the adapter slot of each sequence, -1
+        for none (laya_forward_adapted; not with taps)."""
         logits = np.empty(req.n * req.k, np.float32)
         act = np.empty(req.n * 2, np.float32)
         c = req._c()
-        if taps is None:
+        if adapters is not None:
+            if taps is not None:
+                raise ValueError("taps are not available with adapters")
+            a = _adapter_array(req, adapters)
+            _check(lib().laya_forward_adapted(self._h, ctypes.byref(c), a.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)),
+                                              logits.ctypes.data_as(_f32p), act.ctypes.data_as(_f32p)))
+        elif taps is None:
             _check(lib().laya_forward(self._h, ctypes.byref(c), logits.ctypes.data_as(_f32p),
                                       act.ctypes.data_as(_f32p)))
         else:
@@ -260,8 +289,32 @@ class Engine:
                                              act.ctypes.data_as(_f32p), fn, None))
         return Out(req.n, req.k, logits, act)
 
-    def plan(self, req: Req) -> Plan:
-        return Plan(self, req)
+    def plan(self, req: Req, adapters=None) -> Plan:
+        return Plan(self, req, adapters)
+
+    def adapters_create(self, slots: int, max_rank: int) -> None:
+        """Room for `slots` low-rank adapters of rank <= max_rank on every
+        encoder projection (replaces the slots there were)."""
+        _check(lib().laya_adapters_create(self._h, slots, max_rank))
+
+    def adapter_create(self, slot: int, rank: int, scale: float) -> None:
+        """Empties a slot and gives it its rank and scale, without matrices."""
+        _check(lib().laya_adapter_create(self._h, slot, rank, scale))
+        self._adapter_rank[slot] = rank
+
+    def adapter_upload(self, slot: int, name: str, a: np.ndarray, b: np.ndarray) -> None:
+        """The adapter's matrices on one projection, named like its weight:
+        a [rank, in], b [out, rank] (f16 or converted to f32)."""
+        half = np.asarray(a).dtype == np.float16 and np.asarray(b).dtype == np.float16
+        a, b = (np.ascontiguousarray(v, dtype=np.float16 if half else np.float32) for v in (a, b))
+        shape, rank = arch.stored_shapes().get(name), self._adapter_rank.get(slot)
+        if shape and rank and (a.shape != (rank, shape[1]) or b.shape != (shape[0], rank)):
+            raise ValueError(f"adapter shapes {a.shape}, {b.shape} do not fit rank {rank} of {name} {shape}")
+        _check(lib().laya_adapter_upload(self._h, slot, name.encode(), a.ctypes.data, b.ctypes.data, 0 if half else 2))
+
+    def adapter_drop(self, slot: int) -> None:
+        _check(lib().laya_adapter_drop(self._h, slot))
+        self._adapter_rank.pop(slot, None)
 
     def decision_tail_static(self, x: int, n: int, k: int, cls_row: int, mk_row: int, mmask: int,
                              logits: int, act: int, stream: int = 0) -> None:

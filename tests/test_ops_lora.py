@@ -76,3 +76,9 @@ def test_null_handles():
     assert L.laya_lora_status(None) == E.LAYA_E_INVALID
     L.laya_lora_destroy(None)
     L.laya_lora_plan_destroy(None)
+    assert L.laya_adapters_create(None, 1, 16) == E.LAYA_E_INVALID
+    assert L.laya_adapter_create(None, 0, 16, 1.0) == E.LAYA_E_INVALID
+    assert L.laya_adapter_upload(None, 0, b"x", None, None, 0) == E.LAYA_E_INVALID
+    assert L.laya_adapter_drop(None, 0) == E.LAYA_E_INVALID
+    assert L.laya_forward_adapted(None, None, None, None, None) == E.LAYA_E_INVALID
+    assert L.laya_plan_create_adapted(None, None, None, None) == E.LAYA_E_INVALID
