@@ -872,7 +872,10 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     // x W^T and u B^T in one accumulator
     const bool early = !fused && (q.pairs > 0 || q.items > 0);
     if (q.small) {
-      if (make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, 128))
+      const int width = lora_small_width(fused ? entries : 0, q.lay.rows);
+      CUtensorMap mb;
+      if (make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, width) ||
+          make_tmap_lora(&mb, k.b.p, k.bf16, static_cast<uint64_t>(k.slots) * k.cps * k.out_pad, kLoraChunk, width))
         throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
       LoraSmallArgs g{};
       g.entry_chunk = q.d_entry_chunk;
@@ -891,7 +894,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       g.bf16 = k.bf16;
       g.early = early;
       g.err = q.d_err;
-      op_check(launch_lora_small(mx, mw, q.u_map, k.b_map[0], k.a_map, g, fused, k.num_sms, st), "lora launch");
+      op_check(launch_lora_small(mx, mw, q.u_map, mb, k.a_map, g, fused, k.num_sms, st), "lora launch");
       return;
     }
     // 256 x 128 tiles where 256 x 256 ones would fill at most half the

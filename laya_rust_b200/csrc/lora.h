@@ -109,8 +109,9 @@ cudaError_t launch_lora_pairs(const LoraPairsArgs& a, cudaStream_t s);
 // The projection of at most kLoraBlock rows (one block, so entries
 // 0 .. entries - 1): lora_small.cu.  `fused` (1 to kLoraMaxGroup entries): it
 // computes u too, otherwise u is there, or comes from the launch before it
-// (early).  Maps: x [rows, in] box 64 x lora_small_tile(rows), W box 64 x 128, u
-// box 16 x lora_small_tile(rows), B box 16 x 128, A box 64 x 16.
+// (early).  Maps: x [rows, in] box 64 x lora_small_tile(rows), W box 64 x
+// lora_small_width, u box 16 x lora_small_tile(rows), B box 16 x
+// lora_small_width, A box 64 x 16.
 struct LoraSmallArgs {
   const int* entry_chunk;
   const int* row_entry;
@@ -129,6 +130,8 @@ struct LoraSmallArgs {
 };
 // Rows a tile of the small projection: a multiple of 16, at most 64.
 int lora_small_tile(int rows);
+// Output columns a tile, with this many entries fused in (0: not fused).
+int lora_small_width(int fused_entries, int rows);
 cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const CUtensorMap& b,
                               const CUtensorMap& a_map, const LoraSmallArgs& a, bool fused, int num_sms, cudaStream_t s);
 

@@ -51,6 +51,7 @@ struct SmallShape {
   int xrows;   // rows a tile (N of the MMA): 16..64
   int stages;
   int own;     // FUSED: most entries a CTA owns
+  int width;   // output columns a tile
   int ring_bytes;
 };
 
@@ -130,17 +131,19 @@ __global__ void __launch_bounds__(kThreads)
   uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = SPLITS > 1 ? static_cast<int>(cluster_rank()) : 0;
-  const int n0 = static_cast<int>(blockIdx.x) / SPLITS * kCols;
+  const int width = sh.width;                 // output columns of a tile
+  const bool joint = FUSED && width < kCols;  // A rows beside W's
+  const int n0 = static_cast<int>(blockIdx.x) / SPLITS * width;
   const int xrows = sh.xrows, m0 = static_cast<int>(blockIdx.y) * xrows;
   const int rows = min(xrows, a.rows - m0);
   constexpr int kParts = std::is_same<T, __nv_bfloat16>::value ? 2 : 1;  // operands of u an entry has
   constexpr int kPerStage = 4 / kParts;                                    // entries a stage
   const int x_bytes = xrows * 128, u_bytes = xrows * 32;
-  const int a_bytes = FUSED ? a.entries * kABytes : 0;
-  const int stage_bytes = kWBytes + x_bytes + a_bytes;
+  // a stage: [W | A, joint] [x] [A, apart]
+  const int stage_bytes = kWBytes + x_bytes + (FUSED && !joint ? a.entries * kABytes : 0);
   const int kb0 = rank * a.num_kb / SPLITS, kb1 = (rank + 1) * a.num_kb / SPLITS;
   const int e0 = rank * a.entries / SPLITS, e1 = (rank + 1) * a.entries / SPLITS;
-  const int need_cols = FUSED ? 2 * xrows : xrows;
+  const int need_cols = FUSED && !joint ? 2 * xrows : xrows;
   const uint32_t tmem_cols = need_cols <= 32 ? 32 : need_cols <= 64 ? 64 : 128;
   // [FUSED: owned B operands | owned u operands] [ring] [part] [parts sent here]
   // [FUSED: rank-space part] [parts sent here]; apart from the ring, which this
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(kThreads)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_holder, tmem_u = tmem + xrows;
+  const uint32_t tmem = tmem_holder, tmem_u = joint ? tmem : tmem + xrows;
   if (!a.early) grid_dep_wait();
   grid_dep_trigger();
 
@@ -207,13 +210,14 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
           for (int i = 0; i < kLoraMaxGroup; ++i)
             if (i < a.entries)
-              tma_load_2d(sw + kWBytes + x_bytes + i * kABytes, &maps.a, kb * 64, a.chunk[i] * kLoraChunk, &full[stage]);
+              tma_load_2d((joint ? sw + width * 128 : sw + kWBytes + x_bytes) + i * kABytes, &maps.a, kb * 64,
+                          a.chunk[i] * kLoraChunk, &full[stage]);
         }
         next();
       }
       if constexpr (FUSED) {
         if (e0 < e1 && ok) {
-          mbar_arrive_expect_tx(&b_full, (e1 - e0) * kBBytes);
+          mbar_arrive_expect_tx(&b_full, (e1 - e0) * width * 32);
 #pragma unroll
           for (int i = 0; i < kLoraMaxGroup; ++i)
             if (i >= e0 && i < e1) tma_load_2d(own_b + (i - e0) * kBBytes, &maps.b, 0, a.chunk[i] * a.b_rows + n0, &b_full);
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kThreads)
         for (int k = 0; k < 4; ++k)
           umma_f16(tmem, umma_desc_sw128(w_addr + k * 32), umma_desc_sw128(x_addr + k * 32), idesc,
                    (kb != kb0 || k != 0) ? 1u : 0u);
-        if constexpr (FUSED) {
+        if (FUSED && !joint) {
           // 128 rows from the A operand on: past the entries' they are whatever
           // follows in shared memory, and their sums are never read
 #pragma unroll
@@ -309,14 +313,15 @@ __global__ void __launch_bounds__(kThreads)
   tc_fence_after();
   if (SPLITS > 1) cluster_wait();  // every CTA of the cluster has started
   if constexpr (FUSED) {
-    // thread = row of A
-    if (warp * 32 < a.entries * kLoraChunk) {
-      float* dst = part_u + (static_cast<int>(threadIdx.x) / kLoraChunk) * u_entry + threadIdx.x % kLoraChunk;
+    // lane = row of A, from the first rank-space lane on
+    const int lane0 = joint ? width : 0, ar = static_cast<int>(threadIdx.x) - lane0;
+    if (warp * 32 + 31 >= lane0 && warp * 32 < lane0 + a.entries * kLoraChunk) {
+      float* dst = part_u + (ar / kLoraChunk) * u_entry + ar % kLoraChunk;
       for (int m = 0; m < rows; m += 16) {
         uint32_t v[16];
         tmem_ld_32x32b_x16(tmem_u + lane_base + m, v);
         tmem_ld_wait();
-        if (static_cast<int>(threadIdx.x) < a.entries * kLoraChunk) {
+        if (ar >= 0 && ar < a.entries * kLoraChunk) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) dst[(m + j) * kPartULd] = __uint_as_float(v[j]);
         }
@@ -399,7 +404,8 @@ __global__ void __launch_bounds__(kThreads)
   }
   // the owned rows: 16 threads a row, 8 columns each
   const int col = n0 + static_cast<int>(threadIdx.x & 15) * 8;
-  const int left = a.out - col;  // columns of this thread that exist
+  // columns of this thread that exist (the tile's, then the output's)
+  const int left = static_cast<int>(threadIdx.x & 15) * 8 < width ? a.out - col : 0;
   for (int i = static_cast<int>(threadIdx.x >> 4); i < own_rows && left > 0 && ok; i += 8) {
     const int m = rank * own_rows + i;
     if (m >= rows) break;
@@ -451,7 +457,7 @@ cudaError_t launch(const SmallMaps& maps, const LoraSmallArgs& a, const SmallSha
   attr[0].val.clusterDim.x = SPLITS;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  const dim3 grid((a.out + kCols - 1) / kCols * SPLITS, (a.rows + sh.xrows - 1) / sh.xrows);
+  const dim3 grid((a.out + sh.width - 1) / sh.width * SPLITS, (a.rows + sh.xrows - 1) / sh.xrows);
   return launch_pdl(lora_small_kernel<T, SPLITS, FUSED>, grid, dim3(kThreads), smem, s, attr, 1, maps, a, sh);
 }
 
@@ -474,6 +480,13 @@ int lora_small_tile(int rows) {
   return ((rows + tiles - 1) / tiles + 15) / 16 * 16;
 }
 
+int lora_small_width(int fused_entries, int rows) {
+  // joint pays where the K loop carries many rows (256 rows, 1024 -> 3072, one
+  // entry: 9.9 us, apart 12.0 us); with few, more tiles cost more than a second
+  // operand (1 row: joint 5.7 us, apart 5.4 us)
+  return fused_entries >= 1 && fused_entries <= 4 && rows > 32 ? kCols - fused_entries * kLoraChunk : kCols;
+}
+
 cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const CUtensorMap& b,
                               const CUtensorMap& a_map, const LoraSmallArgs& a, bool fused, int num_sms, cudaStream_t s) {
   if (a.rows <= 0) return cudaSuccess;
@@ -481,7 +494,9 @@ cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const 
     return cudaErrorInvalidValue;
   SmallShape sh{};
   sh.xrows = lora_small_tile(a.rows);
-  const int tiles = (a.out + kCols - 1) / kCols * ((a.rows + sh.xrows - 1) / sh.xrows);
+  sh.width = lora_small_width(fused ? a.entries : 0, a.rows);
+  const bool apart = fused && sh.width == kCols;
+  const int tiles = (a.out + sh.width - 1) / sh.width * ((a.rows + sh.xrows - 1) / sh.xrows);
   // K parts: as many as still run at once, one CTA an SM (measured at 64 rows,
   // 1024 -> 3072: 4 parts, 96 CTAs, 5.7 us; 8 parts, in two rounds, 10.3 us), two
   // for tiles of 16 rows, whose CTAs are small (1 row: 4 parts 4.2 us, 8 parts
@@ -490,14 +505,14 @@ cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const 
   int splits = 1;
   while (splits < 8 && 2 * splits <= a.num_kb && 2 * splits * tiles <= room_ctas) splits *= 2;
   sh.own = fused ? (a.entries + splits - 1) / splits : 0;
-  const int stage_bytes = kWBytes + sh.xrows * 128 + (fused ? a.entries * kABytes : 0);
+  const int stage_bytes = kWBytes + sh.xrows * 128 + (apart ? a.entries * kABytes : 0);
   const int per_stage = a.bf16 ? 2 : 4;
   const int steps = (a.num_kb + splits - 1) / splits + (fused ? 0 : ((a.entries + splits - 1) / splits + per_stage - 1) / per_stage);
   const size_t parts =
       sizeof(float) * sh.xrows * (2 * kPartLd + (fused ? (a.entries + (splits - 1) * sh.own) * kPartULd : 0));
-  // fused: the last stage's A operand is read as 128 rows; what follows is the
+  // apart: the last stage's A operand is read as 128 rows; what follows is the
   // parts, long enough with the padding here
-  const size_t fixed = 1024 + static_cast<size_t>(sh.own) * (kBBytes + sh.xrows * 64) + std::max<size_t>(parts, fused ? 128 * 128 : 0);
+  const size_t fixed = 1024 + static_cast<size_t>(sh.own) * (kBBytes + sh.xrows * 64) + std::max<size_t>(parts, apart ? 128 * 128 : 0);
   const int room = static_cast<int>((kSmemLimit - fixed) / stage_bytes);
   sh.stages = std::max(1, std::min(std::min(kMaxStages, steps), room));
   sh.ring_bytes = sh.stages * stage_bytes;
@@ -505,7 +520,7 @@ cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const 
   // waiting one holds: shared memory in proportion to the TMEM columns (456 of
   // an SM's 233472 bytes a column, of its 512) keeps the columns of the CTAs
   // on an SM, of this kernel and the other clustered ones, within 512.
-  const int need = fused ? 2 * sh.xrows : sh.xrows;
+  const int need = apart ? 2 * sh.xrows : sh.xrows;
   const int cols = need <= 32 ? 32 : need <= 64 ? 64 : 128;
   const size_t smem = std::max(fixed + static_cast<size_t>(sh.ring_bytes), static_cast<size_t>(cols) * 456 - 1024);
   const SmallMaps maps{x, w, u, b, a_map};
