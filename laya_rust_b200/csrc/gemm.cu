@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   grid_dep_trigger();
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (leader && lane == 0) {
+    if (leader && elect_one()) {
       const uint32_t idesc = EPI == kEpiPlainBf16 ? umma_idesc_bf16(BM, BN) : umma_idesc_f16(BM, BN);
       int stage = 0;
       uint32_t phase = 0;

@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(128, 1)
     int a_rows[kLoraMaxGroup];
 #pragma unroll
     for (int i = 0; i < kLoraMaxGroup; ++i) a_rows[i] = __shfl_sync(0xffffffffu, a_row, i);
-    if (lane == 0) {
+    if (elect_one()) {
       bool ok = true;
       int stage = 0;
       uint32_t phase = 0;
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(128, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc = std::is_same<T, __nv_bfloat16>::value ? umma_idesc_bf16(kLoraItemRows, 16 * n)
                                                                     : umma_idesc_f16(kLoraItemRows, 16 * n);
       int stage = 0;

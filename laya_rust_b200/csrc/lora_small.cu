@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   const int rank = SPLITS > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int width = sh.width;                 // output columns of a tile
   const bool joint = FUSED && width < kCols;  // A rows beside W's
@@ -167,6 +167,11 @@ __global__ void __launch_bounds__(kThreads)
     mbar_init(&done2, 1);
     mbar_init(&in_full, 1);
     mbar_init(&in_u_full, 1);
+    tma_prefetch_desc(&maps.w);
+    tma_prefetch_desc(&maps.x);
+    if (FUSED) tma_prefetch_desc(&maps.a);
+    tma_prefetch_desc(&maps.b);
+    if (!FUSED) tma_prefetch_desc(&maps.u);
     abort_word = 0;
     fence_mbar_init();
     if (SPLITS > 1) {
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(kThreads)
 
   const uint32_t idesc = std::is_same<T, __nv_bfloat16>::value ? umma_idesc_bf16(kCols, xrows) : umma_idesc_f16(kCols, xrows);
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       bool ok = true;
       int stage = 0;
       uint32_t phase = 0;
@@ -249,7 +254,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       bool ok = true;
       int stage = 0;
       uint32_t phase = 0;
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(kThreads)
     fence_proxy_async_smem();
     __syncthreads();
     if (e0 < e1 && ok) {
-      if (threadIdx.x == 32) {
+      if (warp == 1 && elect_one()) {
         if (mbar_wait_bounded(&b_full, 0, a.err, kErrLoraWait, abort_flag)) {
           tc_fence_after();
           for (int i = 0; i < e1 - e0; ++i) {
