@@ -228,21 +228,40 @@ __global__ void __launch_bounds__(kThreads)
             if (i >= e0 && i < e1) tma_load_2d(own_b + (i - e0) * kBBytes, &maps.b, 0, a.chunk[i] * a.b_rows + n0, &b_full);
         }
       } else if (e0 < e1 && ok) {
-        int chunk = __ldg(a.entry_chunk + e0);
+        // B operands do not wait for u: those of the stages that are free now go
+        // ahead of it
+        auto load_b = [&](int st, int e, int n) {
+          uint8_t* sb = ring + st * stage_bytes;
+          mbar_arrive_expect_tx(&full[st], n * (kBBytes + kParts * u_bytes));
+          for (int i = 0; i < n; ++i)
+            tma_load_2d(sb + i * kBBytes, &maps.b, 0, __ldg(a.entry_chunk + e + i) * a.b_rows + n0, &full[st]);
+        };
+        auto load_u = [&](int st, int e, int n) {
+          for (int i = 0; i < n; ++i) {
+            uint8_t* su = ring + st * stage_bytes + kWBytes + i * kParts * u_bytes;
+            tma_load_2d(su, &maps.u, 0, (e + i) * kLoraBlock + m0, &full[st]);
+            if (kParts == 2) tma_load_2d(su + u_bytes, &maps.u, 16, (e + i) * kLoraBlock + m0, &full[st]);
+          }
+        };
+        int ahead = e0, st = stage;
+        uint32_t ph = phase;
+        for (int i = 0; i < sh.stages && ahead < e1 && mbar_try_wait(&empty[st], ph ^ 1u); ++i) {
+          load_b(st, ahead, min(kPerStage, e1 - ahead));
+          ahead += kPerStage;
+          if (++st == sh.stages) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
         grid_dep_wait();  // u is complete
         for (int e = e0; e < e1; e += kPerStage) {
           const int n = min(kPerStage, e1 - e);
-          ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag);
-          if (!ok) break;
-          uint8_t* sb = ring + stage * stage_bytes;
-          mbar_arrive_expect_tx(&full[stage], n * (kBBytes + kParts * u_bytes));
-          for (int i = 0; i < n; ++i) {
-            uint8_t* su = sb + kWBytes + i * kParts * u_bytes;
-            tma_load_2d(sb + i * kBBytes, &maps.b, 0, chunk * a.b_rows + n0, &full[stage]);
-            tma_load_2d(su, &maps.u, 0, (e + i) * kLoraBlock + m0, &full[stage]);
-            if (kParts == 2) tma_load_2d(su + u_bytes, &maps.u, 16, (e + i) * kLoraBlock + m0, &full[stage]);
-            if (e + i + 1 < e1) chunk = __ldg(a.entry_chunk + e + i + 1);
+          if (e >= ahead) {
+            ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag);
+            if (!ok) break;
+            load_b(stage, e, n);
           }
+          load_u(stage, e, n);
           next();
         }
       }
