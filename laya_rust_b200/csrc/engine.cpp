@@ -662,8 +662,8 @@ struct Engine {
         ck(cudaMemsetAsync(v[i].a.p, 0, an, stream), "adapters clear");
         ck(cudaMemsetAsync(v[i].b.p, 0, bn, stream), "adapters clear");
         if (make_tmap_pitched(&v[i].a_map, v[i].a.p, false, chunks * kLoraChunk, proj_in(p), proj_in(p), kLoraChunk) ||
-            make_tmap_lora(&v[i].b_map, v[i].b.p, false, chunks * proj_rows(p), kLoraChunk, kGemmBBoxRows) ||
-            make_tmap_lora(&v[i].b_narrow, v[i].b.p, false, chunks * proj_rows(p), kLoraChunk, kGemmBBoxRowsNarrow))
+            make_tmap_lora(&v[i].b_map, v[i].b.p, false, chunks * proj_rows(p), kGemmBBoxRows) ||
+            make_tmap_lora(&v[i].b_narrow, v[i].b.p, false, chunks * proj_rows(p), kGemmBBoxRowsNarrow))
           throw Error(LAYA_E_CUDA, "tensor map encode failed for the adapters");
         v[i].has.assign(n, 0);
       }
@@ -1132,7 +1132,7 @@ struct Engine {
             make_tmap_2d(&q.o_hmlp, hmlp.as<__half>() + r0 * HEAD_INTER, false, rows, HEAD_INTER, 64, ob);
     }
     if (!bad && p.adapted)
-      bad = make_tmap_lora(&m.u, u.p, false, p.lora.chunk.size() * kLoraBlock, kLoraChunk, kGemmABoxRows) != 0;
+      bad = make_tmap_lora(&m.u, u.p, false, p.lora.chunk.size() * kLoraBlock, kGemmABoxRows) != 0;
     if (bad) throw Error(LAYA_E_CUDA, "tensor map encode failed for the arena");
     m.gen = arena_gen;
   }

@@ -32,7 +32,7 @@
 // With EXT (rows that have low-rank adapters), a tile's K loop goes on over the
 // adapters its row block needs: entry e multiplies 16 columns of rank-space
 // vectors u (zero in rows of other adapters) with 16 columns of that adapter's
-// B (operands of 32 bytes a row, 32-byte swizzle).  A stage holds four entries,
+// B (operands of 32 bytes a row, laid out in memory as the MMA reads them).  A stage holds four entries,
 // or two of bf16, whose u is a value and a remainder: four K = 16 MMAs, as many
 // as a stage of the K loop.  So adapters cost a tile entries / 4 (bf16: / 2) more
 // k-blocks and no pass of their own over the output.
@@ -628,10 +628,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int i = 0; i < kPerStage; ++i) {
               if (i >= n) break;
               uint8_t* sa = sA + stage * C::A_BYTES + i * kParts * EXT_A_BYTES;
-              const int y = (e + i) * BM + static_cast<int>(rank) * CTA_ROWS;
-              tma_load_2d_pair(sa, &ext.u, 0, y, fb);
-              if (kParts == 2) tma_load_2d_pair(sa + EXT_A_BYTES, &ext.u, 16, y, fb);
-              tma_load_2d_pair(sB + stage * C::B_BYTES + i * (BN / 2 * 32), &ext.b, 0, chunk[i] * ext.b_rows + n0, fb);
+              const int y = (e + i) * kParts * BM + static_cast<int>(rank) * CTA_ROWS;
+              tma_load_2d_pair(sa, &ext.u, 0, y / 4, fb);
+              if (kParts == 2) tma_load_2d_pair(sa + EXT_A_BYTES, &ext.u, 0, (y + BM) / 4, fb);
+              tma_load_2d_pair(sB + stage * C::B_BYTES + i * (BN / 2 * 32), &ext.b, 0,
+                               (chunk[i] * ext.b_rows + n0) / 4, fb);
             }
 #pragma unroll
             for (int i = 0; i < kPerStage; ++i)
@@ -938,9 +939,9 @@ int make_tmap_pitched(CUtensorMap* map, const void* base, bool bf16, uint64_t ro
   return encode_16bit(map, base, bf16, rows, cols, pitch, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-int make_tmap_lora(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols, uint32_t box_rows) {
-  if (cols != 16 && cols != 32) return -2;
-  return encode_16bit(map, base, bf16, rows, cols, cols, 16, box_rows, CU_TENSOR_MAP_SWIZZLE_32B);
+int make_tmap_lora(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint32_t box_rows) {
+  if (rows % 4 || box_rows % 4) return -2;
+  return encode_16bit(map, base, bf16, rows / 4, 64, 64, 64, box_rows / 4, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 int make_tmap_f16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t k, uint32_t box_rows) {

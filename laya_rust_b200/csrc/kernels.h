@@ -88,9 +88,11 @@ int make_tmap_2d(CUtensorMap* map, const void* base, bool f32, uint64_t rows, ui
 // as zero and are not stored.
 int make_tmap_pitched(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols, uint64_t pitch,
                       uint32_t box_rows);
-// 16-bit map of rows of `cols` (16 or 32) elements, box 16 columns (32 bytes,
-// 32-byte swizzle) x box_rows: the adapter operands of GemmExt.
-int make_tmap_lora(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols, uint32_t box_rows);
+// The adapter operands of GemmExt, `rows` rows (a multiple of 16) of 16
+// elements laid out as the MMA reads them from shared memory (lora_at in
+// lora.h): box_rows of them are one contiguous piece, copied as rows of 128
+// bytes, so coordinates count four rows.
+int make_tmap_lora(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint32_t box_rows);
 
 // Tensor maps of one GEMM: A operand (box 64 x kGemmABoxRows), weights
 // (box 64 x kGemmBBoxRows) and the output (box 128 B x kGemmOutBoxRows; any
@@ -104,8 +106,8 @@ struct GemmMaps {
 
 // Low-rank adapters of the rows (see lora.h): after its K loop, row block m of
 // every tile adds, for each entry e in [off[m], off[m + 1]), the product of
-// u's entry e (256 rows of 16 values, bf16: and 16 remainders) with the 16
-// columns of B's chunk chunk[e] (b_rows rows, ordered like the weight's).
+// u's entry e (256 rows of 16 values, bf16: and 256 rows of 16 remainders) with
+// the 16 columns of B's chunk chunk[e] (b_rows rows, ordered like the weight's).
 struct GemmExt {
   const CUtensorMap* u;  // make_tmap_lora, box rows kGemmABoxRows
   const CUtensorMap* b;  // make_tmap_lora, box rows bn / 2

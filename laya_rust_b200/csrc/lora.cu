@@ -40,39 +40,50 @@ struct Num<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 };
 
-// Two rank values into u: packed values, and for bf16 the packed remainders
-// (0 where a value is not finite: inf - inf would be NaN) 16 elements further.
+// bf16: elements from a value in u to its remainder.
+constexpr int kRemainder = kLoraBlock * kLoraChunk;
+
+// Two rank values as a packed pair, and in bf16 their packed remainders (0
+// where a value is not finite: inf - inf would be NaN).
 template <class T>
-__device__ __forceinline__ void store_u2(T* dst, float a, float b) {
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const __nv_bfloat162 hi = __floats2bfloat162_rn(a, b);
-    const float2 h = __bfloat1622float2(hi);
-    *reinterpret_cast<__nv_bfloat162*>(dst) = hi;
-    *reinterpret_cast<__nv_bfloat162*>(dst + kLoraChunk) =
-        __floats2bfloat162_rn(isfinite(h.x) ? a - h.x : 0.0f, isfinite(h.y) ? b - h.y : 0.0f);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(isfinite(f.x) ? a - f.x : 0.0f, isfinite(f.y) ? b - f.y : 0.0f);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
   } else {
-    *reinterpret_cast<__half2*>(dst) = __floats2half2_rn(a, b);
+    const __half2 h = __floats2half2_rn(a, b);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = 0;
   }
 }
 template <class T>
-__device__ __forceinline__ T* u_row(void* u, int entry, int row) {
-  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  return static_cast<T*>(u) + static_cast<size_t>(entry) * lora_entry_elems(bf16) +
-         static_cast<size_t>(row % kLoraBlock) * lora_u_width(bf16);
+__device__ __forceinline__ T* u_entry(void* u, int entry) {
+  return static_cast<T*>(u) + static_cast<size_t>(entry) * lora_entry_elems(std::is_same<T, __nv_bfloat16>::value);
 }
-// 16 rank values, as 16-byte stores.
+// Rank values j, j + 1 (j even) of a row of the batch into an entry.
 template <class T>
-__device__ __forceinline__ void store_u16(T* dst, const float (&v)[16]) {
-  __align__(16) T t[2 * kLoraChunk];
+__device__ __forceinline__ void store_u2(T* entry, int row, int j, float a, float b) {
+  uint32_t hi, lo;
+  split_pair<T>(a, b, hi, lo);
+  T* d = entry + lora_at(row % kLoraBlock, j);
+  *reinterpret_cast<uint32_t*>(d) = hi;
+  if (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<uint32_t*>(d + kRemainder) = lo;
+}
+// All 16, as 16-byte stores.
+template <class T>
+__device__ __forceinline__ void store_u16(T* entry, int row, const float (&v)[16]) {
 #pragma unroll
-  for (int j = 0; j < 16; j += 2) store_u2<T>(t + j, v[j], v[j + 1]);
-  const uint4* src = reinterpret_cast<const uint4*>(t);
-  uint4* d = reinterpret_cast<uint4*>(dst);
-  d[0] = src[0];
-  d[1] = src[1];
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    d[2] = src[2];
-    d[3] = src[3];
+  for (int h = 0; h < 2; ++h) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split_pair<T>(v[8 * h + 2 * j], v[8 * h + 2 * j + 1], hi[j], lo[j]);
+    T* d = entry + lora_at(row % kLoraBlock, 8 * h);
+    *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (std::is_same<T, __nv_bfloat16>::value)
+      *reinterpret_cast<uint4*>(d + kRemainder) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
 }
 
@@ -245,7 +256,7 @@ __global__ void __launch_bounds__(128, 1)
       float f[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[j]) * scale;
-      store_u16<T>(u_row<T>(a.u, item_entry[i], item.x * kLoraItemRows + r), f);
+      store_u16<T>(u_entry<T>(a.u, item_entry[i]), item.x * kLoraItemRows + r, f);
     }
     tc_fence_before();
     __syncthreads();
@@ -283,7 +294,7 @@ __global__ void __launch_bounds__(128, 1)
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) f[j] *= row_scale[r];
-      store_u16<T>(u_row<T>(a.u, item_entry[i], item.x * kLoraItemRows + r), f);
+      store_u16<T>(u_entry<T>(a.u, item_entry[i]), item.x * kLoraItemRows + r, f);
     }
   }
   if (warp == 1) {
@@ -333,7 +344,7 @@ __global__ void __launch_bounds__(256) lora_pairs_kernel(const LoraPairsArgs a) 
     s1 += __shfl_xor_sync(0xffffffffu, s1, o);
   }
   if (lane == 0) {
-    store_u2<T>(u_row<T>(a.u, p.y, p.x) + 2 * warp, s0 * scale, s1 * scale);
+    store_u2<T>(u_entry<T>(a.u, p.y), p.x, 2 * warp, s0 * scale, s1 * scale);
   }
 }
 
@@ -491,7 +502,7 @@ std::vector<uint16_t> lora_pack_b(const void* b, int type, int rank, int out, in
   for (int n = 0; n < out; ++n) {
     const int row = row_of.empty() ? n : row_of[n];
     for (int r = 0; r < rank; ++r)
-      v[(static_cast<size_t>(r / kLoraChunk) * out_pad + row) * kLoraChunk + r % kLoraChunk] =
+      v[static_cast<size_t>(r / kLoraChunk) * out_pad * kLoraChunk + lora_at(row, r % kLoraChunk)] =
           host_round(b, type, static_cast<size_t>(n) * rank + r, bf16);
   }
   return v;
@@ -525,7 +536,7 @@ LoraLayout lora_layout(const int32_t* rows, const int32_t* slot, int n, const st
         first[s] = static_cast<int>(L.chunk.size());
         used.push_back(s);
         for (int c = 0; c < chunks_of[s]; ++c) L.chunk.push_back(make_int2(s, c));
-        op_require(L.chunk.size() < (size_t{1} << 22), "lora plan: too many adapters in one batch");
+        op_require(L.chunk.size() < (size_t{1} << 21), "lora plan: too many adapters in one batch");
       }
       L.row_entry[m] = first[s];
     }
@@ -685,8 +696,8 @@ int laya_lora_create(int device, int type, int64_t in, int64_t out, const void* 
     op_check(cudaMemsetAsync(k->scale.p, 0, sizeof(float) * slots, k->stream), "lora clear");
     op_check(cudaStreamSynchronize(k->stream), "lora clear");
     if (make_tmap_pitched(&k->a_map, k->a.p, k->bf16, chunks * kLoraChunk, in_pad, in_pad, kLoraChunk) ||
-        make_tmap_lora(&k->b_map[0], k->b.p, k->bf16, chunks * out_pad, kLoraChunk, kGemmBBoxRows) ||
-        make_tmap_lora(&k->b_map[1], k->b.p, k->bf16, chunks * out_pad, kLoraChunk, kGemmBBoxRowsNarrow))
+        make_tmap_lora(&k->b_map[0], k->b.p, k->bf16, chunks * out_pad, kGemmBBoxRows) ||
+        make_tmap_lora(&k->b_map[1], k->b.p, k->bf16, chunks * out_pad, kGemmBBoxRowsNarrow))
       throw OpError(LAYA_E_CUDA, "lora_create: tensor map encode failed");
     *lora = new laya_lora{k};
   });
@@ -785,7 +796,7 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     const size_t entries = std::max<size_t>(1, L.chunk.size());
     q.u.alloc(entries * lora_entry_elems(k.bf16) * 2, "lora workspace");
     q.small = lora_use_small(L.rows);
-    if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock, lora_u_width(k.bf16),
+    if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock * (k.bf16 ? 2 : 1),
                        q.small ? lora_small_tile(L.rows) : kGemmABoxRows))
       throw OpError(LAYA_E_CUDA, "lora_plan_create: tensor map encode failed");
     op_check(cudaMemcpyAsync(q.dev.p, h.data(), h.size() * 4, cudaMemcpyHostToDevice, k.stream), "lora plan upload");
@@ -875,7 +886,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       const int width = lora_small_width(fused ? entries : 0, q.lay.rows);
       CUtensorMap mb;
       if (make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, width) ||
-          make_tmap_lora(&mb, k.b.p, k.bf16, static_cast<uint64_t>(k.slots) * k.cps * k.out_pad, kLoraChunk, width))
+          make_tmap_lora(&mb, k.b.p, k.bf16, static_cast<uint64_t>(k.slots) * k.cps * k.out_pad, width))
         throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
       LoraSmallArgs g{};
       g.entry_chunk = q.d_entry_chunk;

@@ -14,10 +14,22 @@ namespace laya {
 // MMA, 32 bytes a row), the last one filled up with zeros.  In a bank, chunk c
 // of slot s is chunk s * chunks_per_slot + c of
 //   A [chunk][16][in_pad]   (in_pad: in rounded up to 64)
-//   B [chunk][out_pad][16]  (out_pad: out rounded up to 256)
+//   B [chunk][out_pad][16]  (out_pad: out rounded up to 256; a row's two 8-element
+//                            halves placed by lora_at)
 constexpr int kLoraChunk = 16;
 // Rows of a block: the GEMM's row tile.
 constexpr int kLoraBlock = 256;
+
+// Where element j of row r of an MMA operand of 16 columns lies: the 32-byte
+// swizzle of a K-major operand, which swaps a row's halves in every second
+// group of four rows.  Kept in memory, so that a tile is one contiguous copy:
+// the copy unit works by rows, and rows of 128 bytes are a fourth as many as rows
+// of 32 through a swizzling tensor map (16384 rows, 1024 -> 5248, ranks to 128:
+// 165.5 us, this way 161.7).
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+constexpr int lora_at(int r, int j) { return r * kLoraChunk + ((((j >> 3) ^ (r >> 2)) & 1) << 3) + (j & 7); }
 
 inline int lora_chunks(int rank) { return (rank + kLoraChunk - 1) / kLoraChunk; }
 
@@ -25,8 +37,9 @@ inline int lora_chunks(int rank) { return (rank + kLoraChunk - 1) / kLoraChunk; 
 // is one chunk of one adapter that some row of block b has; a slot's chunks
 // are consecutive entries, slots in order of first use.  row_entry[m]: the
 // first entry of row m's adapter, or -1.  u, the rank-space vectors scale *
-// (x A^T), is [entries][256 rows][16 values], in bf16 [16 values | 16
-// remainders], zero for rows of other adapters.
+// (x A^T), is [entries][256 rows][16 values], in bf16 [entries][values,
+// remainders][256 rows][16], halves placed by lora_at, zero for rows of other
+// adapters.
 //
 // u passes between the two products in the 16-bit type.  In f16 one value: half a
 // step is 2^-11 of it, so what it adds to y's error is at most 2^-11 of the
@@ -44,16 +57,15 @@ LoraLayout lora_layout(const int32_t* rows, const int32_t* slot, int n, const st
 
 // An adapter's host matrices (a [rank, in], b [out, rank], `type` LAYA_F16,
 // LAYA_BF16 or LAYA_F32) as the bank's chunks in the 16-bit type: [chunk][16][in_pad]
-// and [chunk][out_pad][16], zeros past rank, in and out.  Output row n of b goes
+// and [chunk][out_pad][16] (lora_at), zeros past rank, in and out.  Output row n of b goes
 // to row row_of[n] (empty: n).  Throws OpError on a value that is not finite in
 // the 16-bit type.
 std::vector<uint16_t> lora_pack_a(const void* a, int type, int rank, int in, int in_pad, bool bf16);
 std::vector<uint16_t> lora_pack_b(const void* b, int type, int rank, int out, int out_pad, bool bf16,
                                   const std::vector<int>& row_of);
 
-// Values a row of an entry.
-constexpr int lora_u_width(bool bf16) { return bf16 ? 2 * kLoraChunk : kLoraChunk; }
-constexpr size_t lora_entry_elems(bool bf16) { return static_cast<size_t>(kLoraBlock) * lora_u_width(bf16); }
+// Elements of an entry of u.
+constexpr size_t lora_entry_elems(bool bf16) { return static_cast<size_t>(kLoraBlock) * kLoraChunk * (bf16 ? 2 : 1); }
 
 // The work of the rank-space product: item i computes entries
 // entry[item.y .. item.y + item.z) for rows [128 item.x, 128 item.x + 128).

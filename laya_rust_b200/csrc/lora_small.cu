@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads)
           mbar_arrive_expect_tx(&b_full, (e1 - e0) * width * 32);
 #pragma unroll
           for (int i = 0; i < kLoraMaxGroup; ++i)
-            if (i >= e0 && i < e1) tma_load_2d(own_b + (i - e0) * kBBytes, &maps.b, 0, a.chunk[i] * a.b_rows + n0, &b_full);
+            if (i >= e0 && i < e1) tma_load_2d(own_b + (i - e0) * kBBytes, &maps.b, 0, (a.chunk[i] * a.b_rows + n0) / 4, &b_full);
         }
       } else if (e0 < e1 && ok) {
         // B operands do not wait for u: those of the stages that are free now go
@@ -234,13 +234,14 @@ __global__ void __launch_bounds__(kThreads)
           uint8_t* sb = ring + st * stage_bytes;
           mbar_arrive_expect_tx(&full[st], n * (kBBytes + kParts * u_bytes));
           for (int i = 0; i < n; ++i)
-            tma_load_2d(sb + i * kBBytes, &maps.b, 0, __ldg(a.entry_chunk + e + i) * a.b_rows + n0, &full[st]);
+            tma_load_2d(sb + i * kBBytes, &maps.b, 0, (__ldg(a.entry_chunk + e + i) * a.b_rows + n0) / 4, &full[st]);
         };
         auto load_u = [&](int st, int e, int n) {
           for (int i = 0; i < n; ++i) {
             uint8_t* su = ring + st * stage_bytes + kWBytes + i * kParts * u_bytes;
-            tma_load_2d(su, &maps.u, 0, (e + i) * kLoraBlock + m0, &full[st]);
-            if (kParts == 2) tma_load_2d(su + u_bytes, &maps.u, 16, (e + i) * kLoraBlock + m0, &full[st]);
+            const int y = (e + i) * kParts * kLoraBlock + m0;
+            tma_load_2d(su, &maps.u, 0, y / 4, &full[st]);
+            if (kParts == 2) tma_load_2d(su + u_bytes, &maps.u, 0, (y + kLoraBlock) / 4, &full[st]);
           }
         };
         int ahead = e0, st = stage;
@@ -379,8 +380,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int j = 0; j < 4; ++j) split2<T>(v[2 * j] * scale, v[2 * j + 1] * scale, hi[j], lo[j]);
       }
-      // 32-byte swizzle: 16-byte piece h of row m at piece h ^ (m / 4 % 2)
-      const int at = m * 32 + ((h ^ ((m >> 2) & 1)) << 4);
+      const int at = 2 * lora_at(m, 8 * h);
       *reinterpret_cast<uint4*>(hi_op + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       if (kParts == 2) *reinterpret_cast<uint4*>(hi_op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
