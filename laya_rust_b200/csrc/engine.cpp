@@ -1191,8 +1191,8 @@ struct Engine {
                         (epi == kEpiQkvRope || epi == kEpiQkvBias || epi == kEpiGeglu || epi == kEpiBiasRelu);
     GemmExt ext{};
     if (ad.bank)
-      ext = GemmExt{&ad.dp->maps.u, narrow ? &ad.bank->b_narrow : &ad.bank->b_map, ad.dp->at<int>(ad.dp->lay.lora_off),
-                    ad.dp->at<int>(ad.dp->lay.entry_chunk), ad.rows, true};
+      ext = GemmExt{&ad.dp->maps.u, narrow ? &ad.bank->b_narrow : &ad.bank->b_map, &Wt.tmap_narrow, &ad.bank->b_narrow,
+                    ad.dp->at<int>(ad.dp->lay.lora_off), ad.dp->at<int>(ad.dp->lay.entry_chunk), ad.rows, true};
     ck(launch_gemm(epi, GemmMaps{&A, narrow ? &Wt.tmap_narrow : &Wt.tmap, &Out, out2}, a, num_sms, s,
                    narrow ? kGemmBNNarrow : kGemmBN, ad.bank ? &ext : nullptr),
        "gemm launch");

@@ -244,14 +244,31 @@ struct Stager {
 // A persistent work unit: an output tile and the K range [kb0, kb1) of it
 // this unit accumulates; `part` is the K part (kEpiPartial, and the split
 // tail tiles of kEpiResidTail) and `tail` marks those tail units.
+// `half`: -1, or which 128-column half of the tile the unit is (EXT kernels,
+// see half_tiles).
 struct Unit {
   int tile, part, kb0, kb1;
   bool tail;
+  int half;
 };
+
+// Epilogues whose EXT kernels run the tiles of a partial last round as two
+// 256 x 128 halves each (K loop of a half: 0.19 us a k-block against 0.38), so
+// that the round takes half as long.
+template <int EPI, int BN, bool EXT>
+constexpr bool kHalves = EXT && BN == kGemmBN &&
+                         (EPI == kEpiQkvRope || EPI == kEpiGeglu || EPI == kEpiPlainF16 || EPI == kEpiPlainBf16);
+
+// First tile that runs as halves (num_tiles: none): those left over after whole
+// rounds of `clusters` tiles, if their halves fit one round.
+__host__ __device__ inline int half_tiles(int num_tiles, int clusters) {
+  const int rest = num_tiles % clusters;
+  return num_tiles > clusters && 2 * rest <= clusters ? num_tiles - rest : num_tiles;
+}
 
 template <int EPI>
 __device__ __forceinline__ Unit unit_of(int u, const GemmArgs& a, int num_kb) {
-  Unit w{u, 0, 0, num_kb, false};
+  Unit w{u, 0, 0, num_kb, false, -1};
   if constexpr (EPI == kEpiPartial) {
     const int S = a.splits;
     w.tile = u / S;
@@ -484,6 +501,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmArgs& a, const CUtensorM
 // The EXT kernels' further parameters (nothing for the others).
 struct ExtParams {
   CUtensorMap u, b;
+  CUtensorMap w_half, b_half;  // kHalves: the weight's and b's maps with 64-row boxes
   const int* off;
   const int* chunk;
   int b_rows;
@@ -527,9 +545,15 @@ __global__ void __launch_bounds__(THREADS, 1)
   // work units (unit_of): one per tile, or per (tile, K part) for
   // kEpiPartial and for the tail tiles of kEpiResidTail; part p of S covers
   // k-blocks [p * num_kb / S, (p + 1) * num_kb / S)
+  constexpr bool HALVES = kHalves<EPI, BN, EXT>;
+  const int half0 = HALVES ? half_tiles(num_tiles, num_clusters) : num_tiles;
   const int num_units = EPI == kEpiPartial    ? num_tiles * args.splits
                         : EPI == kEpiResidTail ? args.main_tiles + (num_tiles - args.main_tiles) * args.splits
-                                               : num_tiles;
+                                               : num_tiles + (num_tiles - half0);
+  auto unit = [&](int u) {
+    if (HALVES && u >= half0) return Unit{half0 + (u - half0) / 2, 0, 0, num_kb, false, (u - half0) & 1};
+    return unit_of<EPI>(u, args, num_kb);
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -576,7 +600,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // at about the same time, and not after: evict-first
       const uint64_t pol_a = l2_evict_first();
       for (int u = cluster_id; u < num_units && ok; u += num_clusters) {
-        const Unit w = unit_of<EPI>(u, args, num_kb);
+        const Unit w = unit(u);
         const int m0 = (w.tile / num_n) * BM + static_cast<int>(rank) * CTA_ROWS;
         int n0 = (w.tile % num_n) * BN + static_cast<int>(rank) * (BN / 2);
         if constexpr (EPI == kEpiGeglu && BN == kGemmBNNarrow) {
@@ -586,6 +610,15 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int t = w.tile % num_n;
           n0 = 256 * (t >> 1) + 128 * static_cast<int>(rank) + 64 * (t & 1);
         }
+        const bool half = HALVES && w.half >= 0;
+        // bytes of a k-block's, and rows of an entry's, B operand per CTA
+        const uint32_t b_bytes = half ? C::B_BYTES / 2 : C::B_BYTES;
+        if (half) {
+          // columns 128 half.. of the tile (GeGLU: 64 gate rows and their 64 up
+          // rows, as a narrow tile)
+          n0 = (w.tile % num_n) * BN +
+               (EPI == kEpiGeglu ? 128 * static_cast<int>(rank) + 64 * w.half : 128 * w.half + 64 * static_cast<int>(rank));
+        }
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, args.err, kErrGemmProducerWait, abort_flag,
                                  args.wait_limit_ns)) {
@@ -593,9 +626,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             break;
           }
           const uint32_t fb = map_to_rank(smem_u32(&full[stage]), 0);
-          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * (C::A_BYTES + b_bytes));
           tma_load_2d_pair_hint(sA + stage * C::A_BYTES, &tmA, kb * BK, m0, fb, pol_a);
-          tma_load_2d_pair(sB + stage * C::B_BYTES, &tmB, kb * BK, n0, fb);
+          const CUtensorMap* tw = &tmB;
+          if constexpr (HALVES) tw = half ? &ext.w_half : &tmB;
+          tma_load_2d_pair(sB + stage * C::B_BYTES, tw, kb * BK, n0, fb);
           if (++stage == C::STAGES) {
             stage = 0;
             phase ^= 1u;
@@ -623,7 +658,10 @@ __global__ void __launch_bounds__(THREADS, 1)
               break;
             }
             const uint32_t fb = map_to_rank(smem_u32(&full[stage]), 0);
-            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * n * (kParts * EXT_A_BYTES + BN / 2 * 32));
+            const uint32_t eb_bytes = half ? BN / 4 * 32 : BN / 2 * 32;
+            const CUtensorMap* tb = &ext.b;
+            if constexpr (HALVES) tb = half ? &ext.b_half : &ext.b;
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * n * (kParts * EXT_A_BYTES + eb_bytes));
 #pragma unroll
             for (int i = 0; i < kPerStage; ++i) {
               if (i >= n) break;
@@ -631,8 +669,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               const int y = (e + i) * kParts * BM + static_cast<int>(rank) * CTA_ROWS;
               tma_load_2d_pair(sa, &ext.u, 0, y / 4, fb);
               if (kParts == 2) tma_load_2d_pair(sa + EXT_A_BYTES, &ext.u, 0, (y + BM) / 4, fb);
-              tma_load_2d_pair(sB + stage * C::B_BYTES + i * (BN / 2 * 32), &ext.b, 0,
-                               (chunk[i] * ext.b_rows + n0) / 4, fb);
+              tma_load_2d_pair(sB + stage * C::B_BYTES + i * (BN / 2 * 32), tb, 0, (chunk[i] * ext.b_rows + n0) / 4, fb);
             }
 #pragma unroll
             for (int i = 0; i < kPerStage; ++i)
@@ -653,15 +690,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp == 1) {
     if (leader && elect_one()) {
-      const uint32_t idesc = EPI == kEpiPlainBf16 ? umma_idesc_bf16(BM, BN) : umma_idesc_f16(BM, BN);
+      const uint32_t idesc_tile = EPI == kEpiPlainBf16 ? umma_idesc_bf16(BM, BN) : umma_idesc_f16(BM, BN);
+      const uint32_t idesc_half = EPI == kEpiPlainBf16 ? umma_idesc_bf16(BM, BN / 2) : umma_idesc_f16(BM, BN / 2);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
       uint32_t aphase = 0;
       bool ok = true;
       for (int u = cluster_id; u < num_units && ok; u += num_clusters) {
-        const Unit w = unit_of<EPI>(u, args, num_kb);
+        const Unit w = unit(u);
         const int kb0 = w.kb0, kb1 = w.kb1;
+        const uint32_t idesc = HALVES && w.half >= 0 ? idesc_half : idesc_tile;
         if (!mbar_wait_bounded(&tempty[acc], aphase ^ 1u, args.err, kErrGemmMmaWait, abort_flag, args.wait_limit_ns)) {
           ok = false;
           break;
@@ -732,7 +771,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     int acc = 0;
     uint32_t aphase = 0;
     for (int u = cluster_id; u < num_units; u += num_clusters) {
-      const Unit w = unit_of<EPI>(u, args, num_kb);
+      const Unit w = unit(u);
       const int tile = w.tile;
       int ok = 1;
       if (lane == 0)
@@ -753,6 +792,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                                  w.part * args.split_rows - args.tail_row0, false, w.part == 0);
         else
           epilogue_tile<EPI, BN>(args, &tmOut, st, t_row, row0, row0 + lane, n0, hc, 0, true, true);
+      } else if (HALVES && w.half >= 0) {
+        epilogue_tile<EPI, BN / 2>(args, &tmOut, st, t_row, row0, row0 + lane, n0 + w.half * (BN / 2), hc, 0, false, false);
       } else {
         epilogue_tile<EPI, BN>(args, &tmOut, st, t_row, row0, row0 + lane, n0, hc,
                                EPI == kEpiPartial ? w.part * args.split_rows : 0, EPI == kEpiResid,
@@ -798,6 +839,7 @@ cudaError_t launch_one(const GemmMaps& m, const GemmArgs& args, int num_sms, cud
   const int num_units = EPI == kEpiPartial    ? num_tiles * args.splits
                         : EPI == kEpiResidTail ? args.main_tiles + (num_tiles - args.main_tiles) * args.splits
                                                : num_tiles;
+  // (halves only split tiles of a round that the whole grid is there for)
   const int max_clusters = num_sms / 2;
   const int clusters = num_units < max_clusters ? num_units : max_clusters;
   cudaLaunchAttribute attr[1];
@@ -836,7 +878,8 @@ cudaError_t launch_gemm(int epilogue, const GemmMaps& m, const GemmArgs& args, i
   }
   if (ext) {
     if (!ext->u || !ext->b || !ext->off || !ext->chunk || ext->b_rows < args.N) return cudaErrorInvalidValue;
-    const ExtParams x{*ext->u, *ext->b, ext->off, ext->chunk, ext->b_rows, ext->early ? 1 : 0};
+    if (bn == kGemmBN && (!ext->w_half || !ext->b_half)) return cudaErrorInvalidValue;
+    const ExtParams x{*ext->u, *ext->b, ext->w_half ? *ext->w_half : *m.b, ext->b_half ? *ext->b_half : *ext->b, ext->off, ext->chunk, ext->b_rows, ext->early ? 1 : 0};
     if (bn == kGemmBNNarrow) {
       switch (epilogue) {
         case kEpiQkvRope: return launch_one<kEpiQkvRope, kGemmBNNarrow, true>(m, args, num_sms, stream, x);

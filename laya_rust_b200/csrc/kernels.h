@@ -111,6 +111,8 @@ struct GemmMaps {
 struct GemmExt {
   const CUtensorMap* u;  // make_tmap_lora, box rows kGemmABoxRows
   const CUtensorMap* b;  // make_tmap_lora, box rows bn / 2
+  const CUtensorMap* w_half;  // bn == kGemmBN: the weight's map and b's with the
+  const CUtensorMap* b_half;  // boxes of kGemmBNNarrow
   const int* off;
   const int* chunk;
   int b_rows;

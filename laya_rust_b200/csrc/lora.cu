@@ -913,7 +913,9 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     const int tiles = (q.lay.rows + kGemmBM - 1) / kGemmBM * (k.out_pad / kGemmBN);
     const bool narrow = tiles * 2 <= k.num_sms / 2;
     const int bn = narrow ? kGemmBNNarrow : kGemmBN;
+    CUtensorMap mw_half;
     if (make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, bn / 2) ||
+        make_tmap_pitched(&mw_half, k.w, k.bf16, k.out, k.in, k.ldw, kGemmBBoxRowsNarrow) ||
         make_tmap_pitched(&my, y, k.bf16, q.lay.rows, std::max(k.out & ~7, 8), ldy, kGemmOutBoxRows))
       throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
     GemmArgs g{};
@@ -925,7 +927,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     g.ldo = static_cast<int>(ldy);
     g.bias = k.bias;
     g.n_valid = k.out;
-    const GemmExt ext{&q.u_map, &k.b_map[narrow], q.d_off, q.d_entry_chunk, k.out_pad, early};
+    const GemmExt ext{&q.u_map, &k.b_map[narrow], &mw_half, &k.b_map[1], q.d_off, q.d_entry_chunk, k.out_pad, early};
     op_check(launch_gemm(k.bf16 ? kEpiPlainBf16 : kEpiPlainF16, GemmMaps{&mx, &mw, &my}, g, k.num_sms, st, bn, &ext),
              "lora launch");
   });

@@ -86,12 +86,14 @@ def on(req):
     return req.mmask.reshape(req.n, req.k) != 0
 
 
-# a single request (split K), one row block, several, and sequences of the flash kernel
+# a single request (split K), one row block, several, sequences of the flash
+# kernel, and 900 rows, whose Wi leaves a partial round of tiles (run as halves)
 LENS = [[90, 89], [31, 77, 128, 64, 90, 12, 1 + 4], [300, 40, 400, 128, 129, 77, 256, 200, 30, 390, 64, 100],
-        [60 + (7 * i) % 69 for i in range(128)]]
+        [60 + (7 * i) % 69 for i in range(128)], [100] * 9]
+IDS = ["request", "one-block", "long", "batch", "halves"]
 
 
-@pytest.mark.parametrize("lens", LENS, ids=["request", "one-block", "long", "batch"])
+@pytest.mark.parametrize("lens", LENS, ids=IDS)
 def test_against_merged_weights(engine, merged, lens):
     """Every sequence under one adapter equals the engine whose weights hold
     it, within the parity bar the engine has against the reference's f32
@@ -109,7 +111,7 @@ def test_against_merged_weights(engine, merged, lens):
         assert moved > 4 * np.abs(got.logits - want.logits)[m].max(), moved   # the adapter is what the answers follow
 
 
-@pytest.mark.parametrize("lens", LENS, ids=["request", "one-block", "long", "batch"])
+@pytest.mark.parametrize("lens", LENS, ids=IDS)
 def test_sequences_keep_to_their_own_adapter(engine, lens):
     """A mixed batch: each sequence bit for bit as in a batch where all have
     its adapter (adapters of other rows add exact zeros), and those without one
@@ -273,8 +275,8 @@ def torch_layer(header, layer, x, lens, who, freqs, m):
     return torch.cat(out)
 
 
-@pytest.mark.parametrize("lens", [[90, 89], [300, 40, 200, 128, 129, 77], [60 + (7 * i) % 69 for i in range(64)]],
-                         ids=["request", "long", "batch"])
+@pytest.mark.parametrize("lens", [[90, 89], [300, 40, 200, 128, 129, 77], [60 + (7 * i) % 69 for i in range(64)], [100] * 9],
+                         ids=["request", "long", "batch", "halves"])
 @pytest.mark.parametrize("layer", [1, 3])
 def test_a_layer_with_mixed_adapters_and_stretched_rotation(engine, header, lens, layer):
     """Relative error under 1e-2 per row, the bar of the plain layer's test."""
