@@ -402,7 +402,7 @@ cudaError_t launch_lora_pairs(const LoraPairsArgs& a, cudaStream_t s) {
 int lora_splits(int rows, int num_sms) {
   const int halves = (rows + kLoraItemRows - 1) / kLoraItemRows;
   int splits = 1;
-  while (splits < 8 && 2 * splits * halves <= num_sms) splits *= 2;
+  while (splits < 8 && 2 * splits * halves <= lora_cluster_room(2 * splits, num_sms)) splits *= 2;
   return splits;
 }
 
@@ -603,7 +603,7 @@ struct Plan {
   LoraLayout lay;
   std::vector<std::pair<int, int>> used;  // (slot, chunks)
   Buf dev, u;
-  bool small = false;  // lora_small.cu, not the GEMM
+  LoraSmallPlan small;  // use: lora_small.cu, not the GEMM
   int items = 0, group = 0;
   const int4* d_item = nullptr;
   const int* d_item_entry = nullptr;
@@ -629,9 +629,6 @@ struct Plan {
 
 // Few (row, chunk) pairs take a block each, reading 16 rows of A from L2.
 constexpr size_t kLoraMaxPairs = 512;
-
-// The rows lora_small.cu takes.
-bool lora_use_small(int rows) { return rows >= 1 && rows <= kLoraBlock; }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -759,16 +756,20 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     std::sort(q.used.begin(), q.used.end());
     q.used.erase(std::unique(q.used.begin(), q.used.end()), q.used.end());
     DeviceScope scope(k.device);
-    // few (row, chunk) pairs: one block each; else items of 128 rows
+    q.small = lora_small_plan(L, k.out, k.cps, k.num_sms);
+    // u apart from the projection: few (row, chunk) pairs one block each, else
+    // items of 128 rows
+    const bool u_apart = !q.small.fused;
     std::vector<int4> pair;
-    for (int m = 0; m < L.rows && pair.size() <= kLoraMaxPairs; ++m) {
+    for (int m = 0; u_apart && m < L.rows && pair.size() <= kLoraMaxPairs; ++m) {
       const int e0 = L.row_entry[m];
       if (e0 < 0) continue;
       for (int e = e0; e < static_cast<int>(L.chunk.size()) && (e == e0 || L.chunk[e].y > 0); ++e)
         pair.push_back(make_int4(m, e, entry_chunk[e], L.chunk[e].x));
     }
     LoraItems it;
-    if (pair.size() <= kLoraMaxPairs) {
+    if (!u_apart) {
+    } else if (pair.size() <= kLoraMaxPairs) {
       q.pairs = static_cast<int>(pair.size());
     } else {
       pair.clear();
@@ -795,9 +796,8 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     q.dev.alloc(h.size() * 4, "lora plan");
     const size_t entries = std::max<size_t>(1, L.chunk.size());
     q.u.alloc(entries * lora_entry_elems(k.bf16) * 2, "lora workspace");
-    q.small = lora_use_small(L.rows);
     if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock * (k.bf16 ? 2 : 1),
-                       q.small ? lora_small_tile(L.rows) : kGemmABoxRows))
+                       q.small.use ? q.small.xrows : kGemmABoxRows))
       throw OpError(LAYA_E_CUDA, "lora_plan_create: tensor map encode failed");
     op_check(cudaMemcpyAsync(q.dev.p, h.data(), h.size() * 4, cudaMemcpyHostToDevice, k.stream), "lora plan upload");
     // rows of other adapters are zero in an entry, and stay zero: every run
@@ -838,15 +838,11 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     require_device_ptr(x, k.device, "lora_run: x");
     require_device_ptr(y, k.device, "lora_run: y");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const uint32_t xbox = q.small ? lora_small_tile(q.lay.rows) : kGemmABoxRows;
-    const int entries = static_cast<int>(q.lay.chunk.size());
-    const bool fused = q.small && entries >= 1 && entries <= kLoraMaxGroup;
+    const uint32_t xbox = q.small.use ? q.small.xrows : kGemmABoxRows;
     CUtensorMap mx, mw, my;
     if (make_tmap_pitched(&mx, x, k.bf16, q.lay.rows, k.in, ldx, xbox))
       throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
-    if (fused) {
-      // u comes with the projection
-    } else if (q.pairs > 0) {
+    if (q.pairs > 0) {
       LoraPairsArgs s{};
       s.pair = q.d_pair;
       s.pairs = q.pairs;
@@ -881,9 +877,9 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       op_check(launch_lora_shrink(mxi, k.a_map, s, k.num_sms, st), "lora launch");
     }
     // x W^T and u B^T in one accumulator
-    const bool early = !fused && (q.pairs > 0 || q.items > 0);
-    if (q.small) {
-      const int width = lora_small_width(fused ? entries : 0, q.lay.rows);
+    const bool early = q.pairs > 0 || q.items > 0;
+    if (q.small.use) {
+      const int width = q.small.width;
       CUtensorMap mb;
       if (make_tmap_pitched(&mw, k.w, k.bf16, k.out, k.in, k.ldw, width) ||
           make_tmap_lora(&mb, k.b.p, k.bf16, static_cast<uint64_t>(k.slots) * k.cps * k.out_pad, width))
@@ -892,8 +888,11 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       g.entry_chunk = q.d_entry_chunk;
       g.row_entry = q.d_row_entry;
       g.scale = k.scale.as<float>();
-      g.entries = entries;
-      for (int i = 0; fused && i < entries; ++i) g.chunk[i] = q.lay.chunk[i].x * k.cps + q.lay.chunk[i].y;
+      g.entries = q.small.entries;
+      g.xrows = q.small.xrows;
+      g.width = width;
+      memcpy(g.tile_entries, q.small.tile_entries, sizeof g.tile_entries);
+      memcpy(g.chunk, q.small.chunk, sizeof g.chunk);
       g.chunks_per_slot = k.cps;
       g.b_rows = k.out_pad;
       g.bias = k.bias;
@@ -905,7 +904,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       g.bf16 = k.bf16;
       g.early = early;
       g.err = q.d_err;
-      op_check(launch_lora_small(mx, mw, q.u_map, mb, k.a_map, g, fused, k.num_sms, st), "lora launch");
+      op_check(launch_lora_small(mx, mw, q.u_map, mb, k.a_map, g, q.small.fused, k.num_sms, st), "lora launch");
       return;
     }
     // 256 x 128 tiles where 256 x 256 ones would fill at most half the

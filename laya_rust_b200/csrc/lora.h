@@ -78,6 +78,12 @@ struct LoraItems {
   std::vector<int> entry;
 };
 LoraItems lora_items(const LoraLayout& L, int num_sms);
+// CTAs, one an SM, that are taken to run at once in clusters of this size: a
+// cluster lies within a group of SMs that its size need not divide (33 clusters of
+// 4 do; 16 of 8 were no faster than 16 of 4).
+inline int lora_cluster_room(int cluster, int num_sms) {
+  return cluster <= 2 ? num_sms : cluster <= 4 ? num_sms * 9 / 10 : num_sms * 2 / 3;
+}
 // K parts of the rank-space product of `rows` rows: 1, 2, 4 or 8, as many as
 // one 128-row item a block leaves SMs for.
 int lora_splits(int rows, int num_sms);
@@ -118,18 +124,32 @@ struct LoraPairsArgs {
 };
 cudaError_t launch_lora_pairs(const LoraPairsArgs& a, cudaStream_t s);
 
-// The projection of at most kLoraBlock rows (one block, so entries
-// 0 .. entries - 1): lora_small.cu.  `fused` (1 to kLoraMaxGroup entries): it
-// computes u too, otherwise u is there, or comes from the launch before it
-// (early).  Maps: x [rows, in] box 64 x lora_small_tile(rows), W box 64 x
-// lora_small_width, u box 16 x lora_small_tile(rows), B box 16 x
-// lora_small_width, A box 64 x 16.
+// The projection of few rows: lora_small.cu.  Row tiles of xrows (a multiple
+// of 16), tiles of `width` output columns.  `fused`: it computes u too, for at
+// most kLoraMaxGroup entries a row tile; otherwise u is there, or comes from the
+// launch before it (early), for one block of rows (entries 0 .. entries - 1).
+// Maps: x [rows, in] box 64 x xrows, W box 64 x width, u box xrows, B box
+// width, A box 64 x 16.
+constexpr int kLoraSmallTile = 128;   // most rows a tile
+constexpr int kLoraSmallTiles = 40;   // most row tiles with entries
+struct LoraSmallPlan {
+  bool use = false, fused = false;
+  int xrows = 0, width = 0;
+  int entries = 0;                                     // fused: of the fullest tile
+  int tile_entries[kLoraSmallTiles] = {};              // fused: of each row tile,
+  int chunk[kLoraSmallTiles][kLoraMaxGroup] = {};      // and their chunks in the bank
+};
+// Whether and how the rows of L go through lora_small.cu.
+LoraSmallPlan lora_small_plan(const LoraLayout& L, int out, int chunks_per_slot, int num_sms);
+
 struct LoraSmallArgs {
   const int* entry_chunk;
   const int* row_entry;
   const float* scale;
-  int entries;
-  int chunk[kLoraMaxGroup];  // fused: the entries' chunks in the bank
+  int entries;                                    // as in LoraSmallPlan
+  int xrows, width;
+  int tile_entries[kLoraSmallTiles];
+  int chunk[kLoraSmallTiles][kLoraMaxGroup];
   int chunks_per_slot;
   int b_rows;
   const float* bias;
@@ -140,10 +160,6 @@ struct LoraSmallArgs {
   int early;              // see GemmExt; not with fused
   int* err;
 };
-// Rows a tile of the small projection: a multiple of 16, at most 64.
-int lora_small_tile(int rows);
-// Output columns a tile, with this many entries fused in (0: not fused).
-int lora_small_width(int fused_entries, int rows);
 cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const CUtensorMap& b,
                               const CUtensorMap& a_map, const LoraSmallArgs& a, bool fused, int num_sms, cudaStream_t s);
 

@@ -1,8 +1,8 @@
-// The adapter projection for few rows (at most 256): y = x W^T + bias + u B^T.
+// The adapter projection for few rows: y = x W^T + bias + u B^T.
 //
 // With few rows the product is a stream of W: what counts is how many SMs read
 // it at once and how short the chain behind the loads is.  So W takes the M
-// side of the MMA (128 output columns a tile) and a tile of 16..64 rows of x
+// side of the MMA (128 output columns a tile) and a tile of 16..128 rows of x
 // the N side (no padding beyond 16), and K is cut over a cluster of up to 8
 // CTAs, each with a few k-blocks that are all in flight together: 3072 outputs
 // are 24 tiles x 8 parts.  The adapter entries are dealt out over the cluster
@@ -13,11 +13,14 @@
 // through the cluster measured 4 us for 16 KB), and it adds them in rank order
 // and stores 16 bytes a thread.
 //
-// With at most 8 entries (FUSED) the same launch computes u as well: the A rows
-// of the entries ride along the K loop as a second M = 128 operand against the
-// same x, the cluster adds those sums first, and each CTA turns the entries it
-// owns into 16-bit operands of the adapter step in its own shared memory.  Every cluster repeats u for its rows (16 rows of A per entry from
-// L2), which costs less than a launch of its own.
+// With at most 8 entries a row tile (FUSED) the same launch computes u as well:
+// the A rows of the entries ride along the K loop against the same x.  Joint, they
+// share the M side with W: a tile is then 128 - 16 entries output columns, and D's
+// last lanes are rank space.  Apart, they are a second M = 128 operand with an
+// accumulator of its own.  The cluster adds the rank-space sums first, and each
+// CTA turns the entries it owns into 16-bit operands of the adapter step in its
+// own shared memory.  Every cluster repeats u for its rows (16 rows of A per entry
+// from L2), which costs less than a launch of its own.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -37,10 +40,10 @@ constexpr int kBBytes = kCols * 32;           // one entry's B operand
 constexpr int kABytes = kLoraChunk * 64 * 2;  // one entry's A operand of a k-block
 constexpr int kMaxStages = 8;
 constexpr int kThreads = 128;
-constexpr int kMaxRows = 64;                  // rows a tile
+constexpr int kMaxRows = kLoraSmallTile;      // rows a tile
 constexpr int kPartLd = kCols + 4;            // floats a row of the f32 parts
 constexpr int kPartULd = kLoraChunk + 4;      // and of the rank-space parts
-constexpr size_t kSmemLimit = 232448 - 1024;  // dynamic, beside the static barriers
+constexpr size_t kSmemLimit = 232448 - 2048;  // dynamic, beside the static barriers and tables
 
 struct SmallMaps {
   CUtensorMap x, w, u, b, a;
@@ -48,10 +51,8 @@ struct SmallMaps {
 
 // What the launch decides.
 struct SmallShape {
-  int xrows;   // rows a tile (N of the MMA): 16..64
   int stages;
   int own;     // FUSED: most entries a CTA owns
-  int width;   // output columns a tile
   int ring_bytes;
 };
 
@@ -131,31 +132,38 @@ __global__ void __launch_bounds__(kThreads)
   uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5;
   const int rank = SPLITS > 1 ? static_cast<int>(cluster_rank()) : 0;
-  const int width = sh.width;                 // output columns of a tile
+  const int width = a.width;                  // output columns of a tile
   const bool joint = FUSED && width < kCols;  // A rows beside W's
   const int n0 = static_cast<int>(blockIdx.x) / SPLITS * width;
-  const int xrows = sh.xrows, m0 = static_cast<int>(blockIdx.y) * xrows;
+  const int xrows = a.xrows, m0 = static_cast<int>(blockIdx.y) * xrows;
+  // FUSED: this row tile's entries
+  const int* const chunk = a.chunk[FUSED ? blockIdx.y : 0];
+  const int entries = FUSED ? a.tile_entries[blockIdx.y] : a.entries;
   const int rows = min(xrows, a.rows - m0);
   constexpr int kParts = std::is_same<T, __nv_bfloat16>::value ? 2 : 1;  // operands of u an entry has
   constexpr int kPerStage = 4 / kParts;                                    // entries a stage
   const int x_bytes = xrows * 128, u_bytes = xrows * 32;
-  // a stage: [W | A, joint] [x] [A, apart]
+  // a stage: [W | A, joint] [x] [A, apart], room for the fullest tile's entries
   const int stage_bytes = kWBytes + x_bytes + (FUSED && !joint ? a.entries * kABytes : 0);
+  const int load_bytes = width * 128 + x_bytes + (FUSED ? entries * kABytes : 0);
   const int kb0 = rank * a.num_kb / SPLITS, kb1 = (rank + 1) * a.num_kb / SPLITS;
-  const int e0 = rank * a.entries / SPLITS, e1 = (rank + 1) * a.entries / SPLITS;
+  const int e0 = rank * entries / SPLITS, e1 = (rank + 1) * entries / SPLITS;
   const int need_cols = FUSED && !joint ? 2 * xrows : xrows;
-  const uint32_t tmem_cols = need_cols <= 32 ? 32 : need_cols <= 64 ? 64 : 128;
-  // [FUSED: owned B operands | owned u operands] [ring] [part] [parts sent here]
-  // [FUSED: rank-space part] [parts sent here]; apart from the ring, which this
-  // CTA may still be using when another one's sums arrive
+  const uint32_t tmem_cols = need_cols <= 32 ? 32 : need_cols <= 64 ? 64 : need_cols <= 128 ? 128 : 256;
+  // A cluster: [owned B operands | owned u operands] [ring] [part] [parts sent
+  // here] [rank-space part] [parts sent here], the parts apart from the ring,
+  // which this CTA may still be using when another one's sums arrive.  One CTA
+  // alone: [owned B operands] [ring], and over the idle ring first [rank-space
+  // part] [u operands], then [part].
+  const int u_entry = xrows * kPartULd;
+  const int own_rows = xrows / SPLITS;                            // rows rank * own_rows ..
   uint8_t* own_b = smem;
   uint8_t* own_u = own_b + sh.own * kBBytes;
-  uint8_t* ring = own_u + sh.own * kParts * u_bytes;
-  const int own_rows = xrows / SPLITS;                            // rows rank * own_rows ..
-  float* part = reinterpret_cast<float*>(ring + sh.ring_bytes);   // [xrows][kPartLd]
-  float* part_in = part + xrows * kPartLd;                        // [SPLITS - 1][own_rows][kPartLd]
-  float* part_u = part_in + (SPLITS - 1) * own_rows * kPartLd;    // [entries][xrows][kPartULd]
-  const int u_entry = xrows * kPartULd;
+  uint8_t* ring = SPLITS > 1 ? own_u + sh.own * kParts * u_bytes : own_u;
+  if (SPLITS == 1) own_u = ring + a.entries * u_entry * 4;
+  float* part = reinterpret_cast<float*>(SPLITS > 1 ? ring + sh.ring_bytes : ring);   // [xrows][kPartLd]
+  float* part_in = part + xrows * kPartLd;                                            // [SPLITS - 1][own_rows][kPartLd]
+  float* part_u = SPLITS > 1 ? part_in + (SPLITS - 1) * own_rows * kPartLd : part;    // [entries][xrows][kPartULd]
   float* part_u_in = part_u + a.entries * u_entry;                // [SPLITS - 1][e1 - e0][xrows][kPartULd]
   if (threadIdx.x == 0) {
     for (int s = 0; s < sh.stages; ++s) {
@@ -208,15 +216,15 @@ __global__ void __launch_bounds__(kThreads)
         ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag);
         if (!ok) break;
         uint8_t* sw = ring + stage * stage_bytes;
-        mbar_arrive_expect_tx(&full[stage], stage_bytes);
+        mbar_arrive_expect_tx(&full[stage], load_bytes);
         tma_load_2d(sw, &maps.w, kb * 64, n0, &full[stage]);
         tma_load_2d(sw + kWBytes, &maps.x, kb * 64, m0, &full[stage]);
         if constexpr (FUSED) {
 #pragma unroll
           for (int i = 0; i < kLoraMaxGroup; ++i)
-            if (i < a.entries)
+            if (i < entries)
               tma_load_2d((joint ? sw + width * 128 : sw + kWBytes + x_bytes) + i * kABytes, &maps.a, kb * 64,
-                          a.chunk[i] * kLoraChunk, &full[stage]);
+                          chunk[i] * kLoraChunk, &full[stage]);
         }
         next();
       }
@@ -225,7 +233,7 @@ __global__ void __launch_bounds__(kThreads)
           mbar_arrive_expect_tx(&b_full, (e1 - e0) * width * 32);
 #pragma unroll
           for (int i = 0; i < kLoraMaxGroup; ++i)
-            if (i >= e0 && i < e1) tma_load_2d(own_b + (i - e0) * kBBytes, &maps.b, 0, (a.chunk[i] * a.b_rows + n0) / 4, &b_full);
+            if (i >= e0 && i < e1) tma_load_2d(own_b + (i - e0) * kBBytes, &maps.b, 0, (chunk[i] * a.b_rows + n0) / 4, &b_full);
         }
       } else if (e0 < e1 && ok) {
         // B operands do not wait for u: those of the stages that are free now go
@@ -294,7 +302,7 @@ __global__ void __launch_bounds__(kThreads)
         for (int k = 0; k < 4; ++k)
           umma_f16(tmem, umma_desc_sw128(w_addr + k * 32), umma_desc_sw128(x_addr + k * 32), idesc,
                    (kb != kb0 || k != 0) ? 1u : 0u);
-        if (FUSED && !joint) {
+        if (FUSED && !joint && entries > 0) {
           // 128 rows from the A operand on: past the entries' they are whatever
           // follows in shared memory, and their sums are never read
 #pragma unroll
@@ -324,8 +332,7 @@ __global__ void __launch_bounds__(kThreads)
     __syncwarp();
   } else if (FUSED) {
     // whose adapter each row has, while the other warps load and multiply
-    const int m = static_cast<int>(threadIdx.x) - 64;
-    if (m < xrows) {
+    for (int m = static_cast<int>(threadIdx.x) - 64; m < xrows; m += 64) {
       const int re = m < rows ? __ldg(a.row_entry + m0 + m) : -1;
       const int slot = re >= 0 ? __ldg(a.entry_chunk + re) / a.chunks_per_slot : -1;
       row_slot[m] = slot;
@@ -340,13 +347,13 @@ __global__ void __launch_bounds__(kThreads)
   if constexpr (FUSED) {
     // lane = row of A, from the first rank-space lane on
     const int lane0 = joint ? width : 0, ar = static_cast<int>(threadIdx.x) - lane0;
-    if (warp * 32 + 31 >= lane0 && warp * 32 < lane0 + a.entries * kLoraChunk) {
+    if (warp * 32 + 31 >= lane0 && warp * 32 < lane0 + entries * kLoraChunk) {
       float* dst = part_u + (ar / kLoraChunk) * u_entry + ar % kLoraChunk;
       for (int m = 0; m < rows; m += 16) {
         uint32_t v[16];
         tmem_ld_32x32b_x16(tmem_u + lane_base + m, v);
         tmem_ld_wait();
-        if (ar >= 0 && ar < a.entries * kLoraChunk) {
+        if (ar >= 0 && ar < entries * kLoraChunk) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) dst[(m + j) * kPartULd] = __uint_as_float(v[j]);
         }
@@ -358,7 +365,7 @@ __global__ void __launch_bounds__(kThreads)
       // each owner's entries, to the owner
       const int to = static_cast<int>(threadIdx.x);
       if (to < SPLITS && to != rank) {
-        const int f0 = to * a.entries / SPLITS, f1 = (to + 1) * a.entries / SPLITS;
+        const int f0 = to * entries / SPLITS, f1 = (to + 1) * entries / SPLITS;
         if (f0 < f1)
           bulk_to_rank(part_u_in + (rank < to ? rank : rank - 1) * (f1 - f0) * u_entry, &in_u_full, part_u + f0 * u_entry,
                        (f1 - f0) * u_entry * 4, to);
@@ -366,23 +373,24 @@ __global__ void __launch_bounds__(kThreads)
       if (e0 < e1 && !mbar_wait_bounded(&in_u_full, 0, a.err, kErrLoraWait, nullptr)) ok = false;
     }
     for (int e = e0; e < e1; ++e) {
-      // thread: half (8 of 16 rank values) of row threadIdx.x / 2
-      const int slot = a.chunk[e] / a.chunks_per_slot;
+      const int slot = chunk[e] / a.chunks_per_slot;
       uint8_t* hi_op = own_u + (e - e0) * kParts * u_bytes;
-      const int m = static_cast<int>(threadIdx.x >> 1), h = threadIdx.x & 1;
-      if (m >= xrows) continue;
-      uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-      if (row_slot[m] == slot) {
-        float v[8];
-        sum_parts<SPLITS>(part_u + e * u_entry + m * kPartULd + 8 * h,
-                          part_u_in + (e - e0) * u_entry + m * kPartULd + 8 * h, (e1 - e0) * u_entry, rank, v);
-        const float scale = row_scale[m];
+      // thread: half (8 of 16 rank values) of a row
+      for (int i = threadIdx.x; i < 2 * xrows; i += kThreads) {
+        const int m = i >> 1, h = i & 1;
+        uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+        if (row_slot[m] == slot) {
+          float v[8];
+          sum_parts<SPLITS>(part_u + e * u_entry + m * kPartULd + 8 * h,
+                            part_u_in + (e - e0) * u_entry + m * kPartULd + 8 * h, (e1 - e0) * u_entry, rank, v);
+          const float scale = row_scale[m];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split2<T>(v[2 * j] * scale, v[2 * j + 1] * scale, hi[j], lo[j]);
+          for (int j = 0; j < 4; ++j) split2<T>(v[2 * j] * scale, v[2 * j + 1] * scale, hi[j], lo[j]);
+        }
+        const int at = 2 * lora_at(m, 8 * h);
+        *reinterpret_cast<uint4*>(hi_op + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (kParts == 2) *reinterpret_cast<uint4*>(hi_op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
-      const int at = 2 * lora_at(m, 8 * h);
-      *reinterpret_cast<uint4*>(hi_op + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if (kParts == 2) *reinterpret_cast<uint4*>(hi_op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     tc_fence_before();
     fence_proxy_async_smem();
@@ -481,7 +489,7 @@ cudaError_t launch(const SmallMaps& maps, const LoraSmallArgs& a, const SmallSha
   attr[0].val.clusterDim.x = SPLITS;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  const dim3 grid((a.out + sh.width - 1) / sh.width * SPLITS, (a.rows + sh.xrows - 1) / sh.xrows);
+  const dim3 grid((a.out + a.width - 1) / a.width * SPLITS, (a.rows + a.xrows - 1) / a.xrows);
   return launch_pdl(lora_small_kernel<T, SPLITS, FUSED>, grid, dim3(kThreads), smem, s, attr, 1, maps, a, sh);
 }
 
@@ -498,55 +506,108 @@ cudaError_t launch_splits(int splits, const SmallMaps& maps, const LoraSmallArgs
 
 }  // namespace
 
-int lora_small_tile(int rows) {
-  // row tiles of at most 64, of equal size
-  const int tiles = (rows + kMaxRows - 1) / kMaxRows;
-  return ((rows + tiles - 1) / tiles + 15) / 16 * 16;
-}
-
-int lora_small_width(int fused_entries, int rows) {
-  // joint pays where the K loop carries many rows (256 rows, 1024 -> 3072, one
-  // entry: 9.9 us, apart 12.0 us); with few, more tiles cost more than a second
-  // operand (1 row: joint 5.7 us, apart 5.4 us)
-  return fused_entries >= 1 && fused_entries <= 4 && rows > 32 ? kCols - fused_entries * kLoraChunk : kCols;
+LoraSmallPlan lora_small_plan(const LoraLayout& L, int out, int chunks_per_slot, int num_sms) {
+  const int rows = L.rows;
+  LoraSmallPlan best;
+  if (rows < 1) return best;
+  const bool one_block = rows <= kLoraBlock, any = !L.chunk.empty();
+  // row tiles of at most 64, of equal size within one block, or of 128
+  const int tiles64 = (rows + 63) / 64;
+  const int even = one_block ? ((rows + tiles64 - 1) / tiles64 + 15) / 16 * 16 : 64;
+  for (int xrows : {even, kLoraSmallTile}) {
+    const int tiles = (rows + xrows - 1) / xrows;
+    if (tiles > kLoraSmallTiles || (xrows > even && rows <= even)) continue;
+    // without adapters the GEMM has no launch before it, and beats tiles of 128
+    // (1357 rows, 1000 -> 1536: 9.3 and 10.3 us; with one adapter 14.2 and 12.6)
+    if (!any && !one_block && xrows > even) continue;
+    LoraSmallPlan p;
+    p.use = true;
+    p.xrows = xrows;
+    // the chunks some row of each tile has
+    bool fits = true;
+    for (int m = 0; m < rows && fits; ++m) {
+      const int e0 = L.row_entry[m];
+      if (e0 < 0) continue;
+      int* const chunk = p.chunk[m / xrows];
+      int& n = p.tile_entries[m / xrows];
+      for (int e = e0; e < static_cast<int>(L.chunk.size()) && (e == e0 || L.chunk[e].y > 0); ++e) {
+        const int c = L.chunk[e].x * chunks_per_slot + L.chunk[e].y;
+        if (std::find(chunk, chunk + n, c) != chunk + n) continue;
+        if (n == kLoraMaxGroup) {
+          fits = false;
+          break;
+        }
+        chunk[n++] = c;
+      }
+    }
+    if (any && !fits && !one_block) continue;  // u by its own launch: one block of rows only
+    p.fused = any && fits;
+    const int most = *std::max_element(p.tile_entries, p.tile_entries + tiles);
+    p.entries = p.fused ? most : static_cast<int>(L.chunk.size());
+    // joint pays where the K loop carries many rows (256 rows, 1024 -> 3072, one
+    // entry: 9.9 us, apart 12.0 us); with few, more tiles cost more than a second
+    // operand (1 row: joint 5.7 us, apart 5.4 us)
+    for (int width : {kCols - most * kLoraChunk, kCols}) {
+      if (width < kCols && !(p.fused && most <= 4 && rows > 32)) continue;
+      p.width = width;
+      // every CTA on an SM of its own; failing that, within one block of rows,
+      // the smaller tiles in rounds (beyond it the GEMM is faster)
+      if ((out + width - 1) / width * tiles <= num_sms) return p;
+      if (one_block && !best.use) best = p;
+    }
+  }
+  return best;
 }
 
 cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const CUtensorMap& b,
                               const CUtensorMap& a_map, const LoraSmallArgs& a, bool fused, int num_sms, cudaStream_t s) {
   if (a.rows <= 0) return cudaSuccess;
-  if (a.rows > kLoraBlock || a.num_kb < 1 || (fused && (a.entries < 1 || a.entries > kLoraMaxGroup)))
+  const int row_tiles = a.xrows > 0 ? (a.rows + a.xrows - 1) / a.xrows : 0;
+  if (a.num_kb < 1 || a.xrows < 16 || a.xrows > kLoraSmallTile || a.xrows % 16 || a.width < 16 || a.width > kCols ||
+      (fused && (a.entries < 1 || a.entries > kLoraMaxGroup || row_tiles > kLoraSmallTiles)) ||
+      (!fused && a.entries > 0 && a.rows > kLoraBlock))
     return cudaErrorInvalidValue;
   SmallShape sh{};
-  sh.xrows = lora_small_tile(a.rows);
-  sh.width = lora_small_width(fused ? a.entries : 0, a.rows);
-  const bool apart = fused && sh.width == kCols;
-  const int tiles = (a.out + sh.width - 1) / sh.width * ((a.rows + sh.xrows - 1) / sh.xrows);
-  // K parts: as many as still run at once, one CTA an SM (measured at 64 rows,
-  // 1024 -> 3072: 4 parts, 96 CTAs, 5.7 us; 8 parts, in two rounds, 10.3 us), two
-  // for tiles of 16 rows, whose CTAs are small (1 row: 4 parts 4.2 us, 8 parts
-  // 3.7 us)
-  const int room_ctas = sh.xrows <= 16 ? 2 * num_sms : num_sms;
+  const bool apart = fused && a.width == kCols;
+  const int tiles = (a.out + a.width - 1) / a.width * row_tiles;
+  // K parts: as many as still run at once (measured at 64 rows, 1024 -> 3072: 4
+  // parts, 96 CTAs, 5.7 us; 8 parts, in two rounds, 10.3 us); tiles of 16 rows
+  // leave room for two CTAs an SM (1 row: 4 parts 4.2 us, 8 parts 3.7 us)
   int splits = 1;
-  while (splits < 8 && 2 * splits <= a.num_kb && 2 * splits * tiles <= room_ctas) splits *= 2;
-  sh.own = fused ? (a.entries + splits - 1) / splits : 0;
-  const int stage_bytes = kWBytes + sh.xrows * 128 + (apart ? a.entries * kABytes : 0);
-  const int per_stage = a.bf16 ? 2 : 4;
-  const int steps = (a.num_kb + splits - 1) / splits + (fused ? 0 : ((a.entries + splits - 1) / splits + per_stage - 1) / per_stage);
-  const size_t parts =
-      sizeof(float) * sh.xrows * (2 * kPartLd + (fused ? (a.entries + (splits - 1) * sh.own) * kPartULd : 0));
-  // apart: the last stage's A operand is read as 128 rows; what follows is the
-  // parts, long enough with the padding here
-  const size_t fixed = 1024 + static_cast<size_t>(sh.own) * (kBBytes + sh.xrows * 64) + std::max<size_t>(parts, apart ? 128 * 128 : 0);
-  const int room = static_cast<int>((kSmemLimit - fixed) / stage_bytes);
-  sh.stages = std::max(1, std::min(std::min(kMaxStages, steps), room));
-  sh.ring_bytes = sh.stages * stage_bytes;
+  while (splits < 8 && 2 * splits <= a.num_kb &&
+         2 * splits * tiles <= (a.xrows <= 16 ? 2 : 1) * lora_cluster_room(2 * splits, num_sms))
+    splits *= 2;
+  const int parts_of_u = a.bf16 ? 2 : 1, per_stage = 4 / parts_of_u;
+  const int stage_bytes = kWBytes + a.xrows * 128 + (apart ? a.entries * kABytes : 0);
+  const size_t rank_part = fused ? sizeof(float) * a.xrows * kPartULd : 0;   // of one entry
+  const size_t u_ops = static_cast<size_t>(parts_of_u) * a.xrows * 32;       // of one entry
   // A CTA waits for its cluster, so no CTA may be left waiting for TMEM that a
   // waiting one holds: shared memory in proportion to the TMEM columns (456 of
   // an SM's 233472 bytes a column, of its 512) keeps the columns of the CTAs
   // on an SM, of this kernel and the other clustered ones, within 512.
-  const int need = apart ? 2 * sh.xrows : sh.xrows;
-  const int cols = need <= 32 ? 32 : need <= 64 ? 64 : 128;
-  const size_t smem = std::max(fixed + static_cast<size_t>(sh.ring_bytes), static_cast<size_t>(cols) * 456 - 1024);
+  const int need = apart ? 2 * a.xrows : a.xrows;
+  const int cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : 256;
+  size_t smem = 0;
+  for (;; splits /= 2) {
+    sh.own = fused ? (a.entries + splits - 1) / splits : 0;
+    const int steps = (a.num_kb + splits - 1) / splits +
+                      (fused ? 0 : ((a.entries + splits - 1) / splits + per_stage - 1) / per_stage);
+    // what lies behind the ring (a cluster), or over it (one CTA)
+    const size_t parts = splits > 1 ? sizeof(float) * kPartLd * (a.xrows + (splits - 1) * (a.xrows / splits)) +
+                                          rank_part * (a.entries + (splits - 1) * sh.own)
+                                    : 0;
+    const size_t over =
+        splits > 1 ? 0 : std::max(sizeof(float) * kPartLd * a.xrows, (rank_part + (fused ? u_ops : 0)) * a.entries);
+    // apart: the last stage's A operand is read as 128 rows, so 16 KB must follow
+    const size_t fixed = 1024 + static_cast<size_t>(sh.own) * (kBBytes + (splits > 1 ? u_ops : 0)) +
+                         std::max<size_t>(parts, apart ? 128 * 128 : 0);
+    const int room = fixed < kSmemLimit ? static_cast<int>((kSmemLimit - fixed) / stage_bytes) : 0;
+    sh.stages = std::min(std::min(kMaxStages, steps), room);
+    sh.ring_bytes = sh.stages * stage_bytes;
+    smem = std::max(fixed + std::max(static_cast<size_t>(sh.ring_bytes), over), static_cast<size_t>(cols) * 456 - 1024);
+    if (sh.stages >= std::min(2, steps) && smem <= kSmemLimit) break;
+    if (splits == 1) return cudaErrorInvalidValue;
+  }
   const SmallMaps maps{x, w, u, b, a_map};
   if (a.bf16)
     return fused ? launch_splits<__nv_bfloat16, true>(splits, maps, a, sh, smem, s)

@@ -113,10 +113,26 @@ def test_few_rows(type, inn, out, rows):
 
 @BOTH
 @pytest.mark.parametrize("inn,out", [(1024, 3072), (1000, 1531), (2624, 1024), (72, 264)])
-@pytest.mark.parametrize("m", [40, 64, 65, 127, 128, 129, 179, 256, 257, 600, 1357])
+@pytest.mark.parametrize("m", [40, 64, 65, 127, 128, 129, 179, 256, 257, 385, 600, 1357, 2300])
 def test_more_rows(type, inn, out, m):
     cut = m // 3
     c = Case(type, [cut, 0, 1, m - cut - 1], [1, 0, -1, 0], [16, 11], inn, out, bias=True, seed=m)
+    c.run()
+    c.check()
+
+
+@BOTH
+@pytest.mark.parametrize("inn,out", [(1024, 1024), (1000, 1531), (200, 136)])
+@pytest.mark.parametrize("lens,slots,ranks", [
+    # row tiles with 0, 1, 4, 5, 8 and 9 adapter chunks, adapters that start in the middle of a tile
+    ([64] * 10, [-1, 0, -1, 1, 1, -1, 0, -1, -1, 1], [16, 9]),
+    ([100, 30, 30, 30, 30, 100, 300], [0, 1, 2, 3, -1, 0, 2], [16, 16, 32, 7]),
+    ([130, 130, 130], [0, 1, 2], [128, 112, 5]),
+    ([500, 14, 14, 14], [0, 1, 2, 3], [64, 33, 16, 1]),
+    ([8] * 70, [i % 9 for i in range(70)], [16] * 9),
+    ([700, 3, 600], [-1, 0, -1], [100])])
+def test_tiles_with_few_and_many_adapters(type, inn, out, lens, slots, ranks):
+    c = Case(type, lens, slots, ranks, inn, out, bias=True, seed=len(lens))
     c.run()
     c.check()
 
