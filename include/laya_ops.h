@@ -17,7 +17,8 @@
  * Every call runs on the device it names (or its handle was made on) and
  * restores the caller's current device.  `stream` is a cudaStream_t of that
  * device (NULL: the default stream); calls enqueue work and return without
- * waiting for it, and may be captured into a graph.
+ * waiting for it, and may be captured into a graph (make the first call of a kind
+ * on a device before any capture: it loads and configures the kernels).
  */
 #ifndef LAYA_OPS_H
 #define LAYA_OPS_H
@@ -72,7 +73,7 @@ typedef struct {
   int32_t inverse;
   int32_t dim, rot;    /* head size (<= LAYA_ROPE_MAX_DIM) and its rotated part (even, 2..dim) */
   float mscale;
-  const double *freqs; /* host, [rot / 2], radians per position; read during the call */
+  const double *freqs; /* host, [rot / 2], radians per position, at most 2^20; read during the call */
 } laya_rope_spec;
 
 /* A [tokens, heads, dim] view and where its rotation goes; strides in elements,
@@ -87,8 +88,8 @@ typedef struct {
 } laya_rope_tensor;
 
 /* Rotates `count` (1..4) tensors over the same tokens, e.g. q and k, in one
- * launch.  pos: device int32 [tokens], any values, or NULL for pos0, pos0 + 1,
- * ...  (pos0 + tokens - 1 < 2^31).  tokens == 0 does nothing. */
+ * launch, 65535 heads in all.  pos: device int32 [tokens], any values, or NULL for
+ * pos0, pos0 + 1, ...  (pos0 + tokens - 1 < 2^31).  tokens == 0 does nothing. */
 int laya_rope(int device, const laya_rope_spec *spec, const laya_rope_tensor *tensors, int count, int64_t tokens,
               const int32_t *pos, int64_t pos0, void *stream);
 
@@ -139,7 +140,9 @@ int laya_lora_plan_create(laya_lora *lora, const int32_t *rows, const int32_t *s
  * multiples of 16 bytes, x and y apart.  Only elements of y's rows and
  * columns are written.  A plan's runs share its workspace: give them one
  * stream, or order them (a graph's replays count).  LAYA_E_STATE: an adapter
- * of the plan was cleared, or changed its up16(rank). */
+ * of the plan was cleared, or changed its up16(rank).  A graph captured from a
+ * run cannot be told: it goes on with what the slots' memory holds, so capture
+ * again where a new run would ask for a new plan. */
 int laya_lora_run(laya_lora *lora, laya_lora_plan *plan, const void *x, int64_t ldx, void *y, int64_t ldy,
                   void *stream);
 /* Waits for the device and reports a bounded wait that expired in a run of

@@ -34,6 +34,7 @@ namespace {
 
 constexpr int kMaxPairs = LAYA_ROPE_MAX_DIM / 2;
 constexpr int kMaxTensors = 4;
+constexpr double kMaxFreq = 1048576.0;  // radians per position; keeps rope_turns' remainder in 64 bits
 
 struct RopeTensorArg {
   const void* x;
@@ -221,6 +222,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __gr
   // the first of the angles it computes
   const int my_at = static_cast<int>(threadIdx.x) / half, my_j = static_cast<int>(threadIdx.x) - my_at * half;
 
+  grid_dep_wait();  // positions and inputs may come from the launch before
+  grid_dep_trigger();
+
   auto compute_angles = [&](long long tile, float* buf) {
     int at = my_at, j = my_j;
     for (int i = threadIdx.x; i < n_angles; i += kThreads) {
@@ -291,6 +295,8 @@ struct TableArgs {
 };
 
 __global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__ TableArgs a) {
+  grid_dep_wait();
+  grid_dep_trigger();
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= a.positions * a.n) return;
   float c, s;
@@ -302,11 +308,8 @@ __global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__
 template <class T, int VEC>
 cudaError_t launch_vec(const RopeArgs& a, bool half, dim3 grid, cudaStream_t st) {
   const size_t smem = 4 * sizeof(float) * a.block_tokens * (a.rot / 2);
-  if (half)
-    rope_kernel<T, VEC, true><<<grid, kThreads, smem, st>>>(a);
-  else
-    rope_kernel<T, VEC, false><<<grid, kThreads, smem, st>>>(a);
-  return cudaGetLastError();
+  return half ? launch_pdl(rope_kernel<T, VEC, true>, grid, dim3(kThreads), smem, st, nullptr, 0, a)
+              : launch_pdl(rope_kernel<T, VEC, false>, grid, dim3(kThreads), smem, st, nullptr, 0, a);
 }
 
 // Whether pieces of `v` elements of `es` bytes fit the head, every stride and
@@ -342,7 +345,6 @@ cudaError_t launch_rope(RopeArgs& a, bool half, int num_sms, cudaStream_t st) {
   a.block_tokens = std::max(1, kThreads / (a.block_groups * units));
   const unsigned gz = (units + kThreads - 1) / kThreads;
   const unsigned gy = (a.groups + a.block_groups - 1) / a.block_groups;
-  if (gy > 65535) return cudaErrorInvalidValue;
   // the resident blocks, each walking over its share of the tiles
   const long long tiles = (a.tokens + a.block_tokens - 1) / a.block_tokens;
   const long long want = std::max<long long>(1, static_cast<long long>(kBlocksPerSm) * num_sms / (gy * gz));
@@ -406,8 +408,7 @@ cudaError_t launch_rope_table(const double* freqs, int n, float mscale, int posi
   a.mscale = mscale;
   a.cosb = cosb;
   a.sinb = sinb;
-  rope_table_kernel<<<(positions * n + 255) / 256, 256, 0, s>>>(a);
-  return cudaGetLastError();
+  return launch_pdl(rope_table_kernel, dim3((positions * n + 255) / 256), dim3(256), 0, s, nullptr, 0, a);
 }
 
 }  // namespace laya
@@ -440,11 +441,15 @@ extern "C" int laya_rope(int device, const laya_rope_spec* spec, const laya_rope
     op_require(tokens >= 0 && tokens <= kMaxPos, "rope: tokens out of range");
     op_require(pos || (pos0 >= -kMaxPos && pos0 + tokens <= kMaxPos + 1 && pos0 <= kMaxPos),
                "rope: positions must fit 32 bits");
+    op_require(reinterpret_cast<uintptr_t>(pos) % 4 == 0, "rope: pos is not aligned");
     RopeArgs a{};
+    int64_t heads = 0;
     const size_t es = spec->type == LAYA_F32 ? 4 : 2;
     for (int i = 0; i < count; ++i) {
       const laya_rope_tensor& t = tensors[i];
       op_require(t.heads >= 0 && t.heads <= 65535, "rope: heads must be 0..65535");
+      heads += t.heads;
+      op_require(heads <= 65535, "rope: more than 65535 heads in all");
       if (t.heads == 0 || tokens == 0) continue;
       op_require(t.x && t.out, "rope: null tensor");
       op_require(reinterpret_cast<uintptr_t>(t.x) % es == 0 && reinterpret_cast<uintptr_t>(t.out) % es == 0,
@@ -474,7 +479,7 @@ extern "C" int laya_rope(int device, const laya_rope_spec* spec, const laya_rope
       r.heads = static_cast<int>(t.heads);
     }
     for (int j = 0; j < spec->rot / 2; ++j) {
-      op_require(std::isfinite(spec->freqs[j]), "rope: a frequency is not finite");
+      op_require(std::fabs(spec->freqs[j]) <= kMaxFreq, "rope: a frequency is not finite, or above 2^20");
       a.turns[j] = rope_turns(spec->freqs[j]);
     }
     if (a.count == 0) return;

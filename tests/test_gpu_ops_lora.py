@@ -138,6 +138,15 @@ def test_tiles_with_few_and_many_adapters(type, inn, out, lens, slots, ranks):
 
 
 @BOTH
+@pytest.mark.parametrize("out", [5, 263, 8])
+def test_many_rows_and_few_columns(type, out):
+    """More rows than the few-row kernel takes, outputs narrower than a tile."""
+    c = Case(type, [3000, 1, 3200], [0, -1, 1], [16, 5], 72, out, bias=True)
+    c.run()
+    c.check()
+
+
+@BOTH
 def test_a_large_packed_batch(type):
     rng = np.random.default_rng(1)
     rows = rng.integers(24, 129, 64).tolist()

@@ -87,6 +87,9 @@ def spec(type=ops.F16, dim=64, rot=64, layout=ops.ROPE_HALF, mscale=1.0, freqs=N
     ("rot", lambda: ops.rope(spec(rot=33), [tensor()], 4)),
     ("mscale", lambda: ops.rope(spec(mscale=float("inf")), [tensor()], 4)),
     ("frequency", lambda: ops.rope(spec(freqs=np.full(32, np.nan)), [tensor()], 4)),
+    ("frequency", lambda: ops.rope(spec(freqs=np.full(32, 2.0e6)), [tensor()], 4)),
+    ("pos", lambda: ops.rope(spec(), [tensor()], 4, pos=FAKE + 2)),
+    ("65535", lambda: ops.rope(spec(), [tensor(heads=40000, out_head=64, out_token=40000 * 64)] * 2, 4)),
     ("1 to 4", lambda: ops.rope(spec(), [], 4)),
     ("1 to 4", lambda: ops.rope(spec(), [tensor()] * 5, 4)),
     ("tokens", lambda: ops.rope(spec(), [tensor()], -1)),
