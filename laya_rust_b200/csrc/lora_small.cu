@@ -134,6 +134,10 @@ __global__ void __launch_bounds__(kThreads)
   const int rank = SPLITS > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int width = a.width;                  // output columns of a tile
   const bool joint = FUSED && width < kCols;  // A rows beside W's
+  // apart, a whole tile of 128 rows in one CTA: x takes the M side against the
+  // entries' A rows (N = 16 entries), so only their rows are read, and a thread
+  // finds its row's rank values in its own TMEM lane
+  const bool by_row = SPLITS == 1 && FUSED && !joint && a.xrows == kCols;
   const int n0 = static_cast<int>(blockIdx.x) / SPLITS * width;
   const int xrows = a.xrows, m0 = static_cast<int>(blockIdx.y) * xrows;
   // FUSED: this row tile's entries
@@ -201,6 +205,8 @@ __global__ void __launch_bounds__(kThreads)
   grid_dep_trigger();
 
   const uint32_t idesc = std::is_same<T, __nv_bfloat16>::value ? umma_idesc_bf16(kCols, xrows) : umma_idesc_f16(kCols, xrows);
+  const uint32_t idesc_u = std::is_same<T, __nv_bfloat16>::value ? umma_idesc_bf16(kCols, kLoraChunk * entries)
+                                                                  : umma_idesc_f16(kCols, kLoraChunk * entries);
   if (warp == 0) {
     if (elect_one()) {
       bool ok = true;
@@ -302,7 +308,12 @@ __global__ void __launch_bounds__(kThreads)
         for (int k = 0; k < 4; ++k)
           umma_f16(tmem, umma_desc_sw128(w_addr + k * 32), umma_desc_sw128(x_addr + k * 32), idesc,
                    (kb != kb0 || k != 0) ? 1u : 0u);
-        if (FUSED && !joint && entries > 0) {
+        if (by_row && entries > 0) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tmem_u, umma_desc_sw128(x_addr + k * 32), umma_desc_sw128(x_addr + x_bytes + k * 32), idesc_u,
+                     (kb != kb0 || k != 0) ? 1u : 0u);
+        } else if (FUSED && !joint && entries > 0) {
           // 128 rows from the A operand on: past the entries' they are whatever
           // follows in shared memory, and their sums are never read
 #pragma unroll
@@ -345,9 +356,32 @@ __global__ void __launch_bounds__(kThreads)
   tc_fence_after();
   if (SPLITS > 1) cluster_wait();  // every CTA of the cluster has started
   if constexpr (FUSED) {
+    if (by_row) {
+      const int m = threadIdx.x, slot_of_row = row_slot[m];
+      const float scale = row_scale[m];
+      for (int e = 0; e < entries; ++e) {
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(tmem_u + lane_base + e * kLoraChunk, v);
+        tmem_ld_wait();
+        const bool mine = slot_of_row == chunk[e] / a.chunks_per_slot;
+        uint8_t* op = own_u + e * kParts * u_bytes;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+          if (mine) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              split2<T>(__uint_as_float(v[8 * h + 2 * j]) * scale, __uint_as_float(v[8 * h + 2 * j + 1]) * scale, hi[j], lo[j]);
+          }
+          const int at = 2 * lora_at(m, 8 * h);
+          *reinterpret_cast<uint4*>(op + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if (kParts == 2) *reinterpret_cast<uint4*>(op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+    }
     // lane = row of A, from the first rank-space lane on
     const int lane0 = joint ? width : 0, ar = static_cast<int>(threadIdx.x) - lane0;
-    if (warp * 32 + 31 >= lane0 && warp * 32 < lane0 + entries * kLoraChunk) {
+    if (!by_row && warp * 32 + 31 >= lane0 && warp * 32 < lane0 + entries * kLoraChunk) {
       float* dst = part_u + (ar / kLoraChunk) * u_entry + ar % kLoraChunk;
       for (int m = 0; m < rows; m += 16) {
         uint32_t v[16];
@@ -372,7 +406,7 @@ __global__ void __launch_bounds__(kThreads)
       }
       if (e0 < e1 && !mbar_wait_bounded(&in_u_full, 0, a.err, kErrLoraWait, nullptr)) ok = false;
     }
-    for (int e = e0; e < e1; ++e) {
+    for (int e = e0; e < e1 && !by_row; ++e) {
       const int slot = chunk[e] / a.chunks_per_slot;
       uint8_t* hi_op = own_u + (e - e0) * kParts * u_bytes;
       // thread: half (8 of 16 rank values) of a row
