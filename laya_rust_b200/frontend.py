@@ -218,15 +218,20 @@ class Requests:
 
 
 def run_requests(engine, tok: Tokenizer, requests: list, max_tokens: int = 16384, across_requests: bool = False,
-                 threads: int = 0, calibration: dict | None = None) -> list:
+                 threads: int = 0, calibration: dict | None = None, adapters: list | None = None) -> list:
     """Requests in, responses out: plan (threads), pack, one laya_forward per
     forward, score, respond -- run_all (main.rs:520-557) for each request.
-    Requests that fail to plan come back as {"error": message}."""
+    Requests that fail to plan come back as {"error": message}.
+    adapters: the engine's adapter slot of each request, -1 for none
+    (laya_forward_adapted); requests with different adapters share forwards."""
+    if adapters is not None and len(adapters) != len(requests):
+        raise ValueError(f"{len(adapters)} adapters for {len(requests)} requests")
     rq = Requests(tok, requests, threads)
     if calibration:
         rq.set_calibration(calibration.get("temperature", (1.0, 1.0, 1.0)), calibration.get("by_options"))
     for f in range(rq.pack(max_tokens, across_requests)):
-        out = engine.forward(rq.batch(f))
+        who = None if adapters is None else [adapters[rq.question_shape(q)[0]] for q in rq.forward_questions(f)]
+        out = engine.forward(rq.batch(f), adapters=who) if who is not None else engine.forward(rq.batch(f))
         rq.score(f, out.logits, out.act)
     res = []
     for i in range(rq.n_requests):

@@ -224,6 +224,33 @@ def test_uploads_reach_the_next_call_and_drops_are_refused():
         eng.close()
 
 
+def test_requests_of_several_tenants_share_forwards(engine, merged):
+    """Request JSON to response JSON, each request under its own adapter, packed
+    together: the answers of the engine whose weights hold that adapter, within
+    the front end's bar (2e-2 on probabilities)."""
+    from laya_rust_b200 import frontend as FE, tokgen, workloads
+    words = workloads.vocab_words(tokgen.tokenizer_json(0))
+    reqs = [workloads.single_request_json(words, i) for i in range(5)]
+    who = [0, -1, 2, 1, 0]
+    tok = FE.Tokenizer(gguf_path=modelgen.cached_model(seed=0))
+    got = FE.run_requests(engine, tok, reqs, across_requests=True, adapters=who)
+    base = FE.run_requests(engine, tok, reqs, across_requests=True)
+    moved = 0.0
+    for i, slot in enumerate(who):
+        want = FE.run_requests(engine if slot < 0 else merged(slot), tok, [reqs[i]])[0]
+        assert set(got[i]["answers"]) == set(want["answers"])
+        for qid, w in want["answers"].items():
+            g, b = got[i]["answers"][qid], base[i]["answers"][qid]
+            for k, p in w.get("probabilities", {}).items():
+                assert abs(g["probabilities"][k] - p) <= 2e-2
+                moved = max(moved, abs(b["probabilities"][k] - p))
+            assert abs(g["rl_agent"]["act_probability"] - w["rl_agent"]["act_probability"]) <= 2e-2
+    assert moved > 1e-3
+    with pytest.raises(ValueError):
+        FE.run_requests(engine, tok, reqs, adapters=[0])
+    tok.close()
+
+
 def test_an_engine_without_weights_refuses():
     eng = E.Engine(None, device=0)
     try:
