@@ -302,8 +302,9 @@ def torch_layer(header, layer, x, lens, who, freqs, m):
     return torch.cat(out)
 
 
-@pytest.mark.parametrize("lens", [[90, 89], [300, 40, 200, 128, 129, 77], [60 + (7 * i) % 69 for i in range(64)], [100] * 9],
-                         ids=["request", "long", "batch", "halves"])
+@pytest.mark.parametrize("lens", [[90, 89], [300, 40, 200, 128, 129, 77], [60 + (7 * i) % 69 for i in range(64)], [100] * 9,
+                                  [1500, 40, 700]],
+                         ids=["request", "long", "batch", "halves", "beyond-512"])
 @pytest.mark.parametrize("layer", [1, 3])
 def test_a_layer_with_mixed_adapters_and_stretched_rotation(engine, header, lens, layer):
     """Relative error under 1e-2 per row, the bar of the plain layer's test."""

@@ -262,6 +262,12 @@ def test_another_stream_and_a_replayed_graph(m):
     g.replay()
     torch.cuda.synchronize()
     c.check()
+    # an adapter changed in place reaches the replays
+    c.a[0], c.b[0] = c.a[0] * -2, torch.randn_like(c.b[0].float()).to(torch.bfloat16) * 0.1
+    c.put(0)
+    g.replay()
+    torch.cuda.synchronize()
+    c.check()
 
 
 @pytest.mark.parametrize("m", [3, 200])
