@@ -133,7 +133,9 @@ void laya_lora_destroy(laya_lora *lora);
 
 /* The segments of a batch, in row order: rows[i] >= 0 rows with the adapter
  * slot[i], or LAYA_LORA_NONE.  Host arrays, read during the call.  The plan
- * keeps what it needs of `lora` alive. */
+ * keeps what it needs of `lora` alive.  Takes device memory: not during a
+ * stream capture.  A graph captured from runs reads the plan at every replay:
+ * destroy it first. */
 int laya_lora_plan_create(laya_lora *lora, const int32_t *rows, const int32_t *slot, int n, laya_lora_plan **plan);
 /* Enqueues y = the projection of x on `stream`.  x [rows, in] with row pitch
  * ldx, y [rows, out] with row pitch ldy, in elements; addresses and pitches

@@ -202,6 +202,31 @@ def test_pitches_and_repeated_runs(type, m):
     c.check()
 
 
+def far_rows(t, pitch):
+    """The rows of t at a pitch that takes their offsets past 2^32 elements."""
+    assert (t.shape[0] - 1) * pitch > 1 << 32
+    buf = torch.empty((t.shape[0] - 1) * pitch + up8(t.shape[1]), device="cuda", dtype=t.dtype)
+    v = buf.as_strided(t.shape, (pitch, 1))
+    v.copy_(t)
+    return v
+
+
+@BOTH
+@pytest.mark.parametrize("rows,slots,pitch", [
+    ([1] * 20, list(range(20)), 1 << 28),      # a block per (row, chunk)
+    ([200], [0], 1 << 25),                     # one launch
+    ([700, 3, 700], [0, -1, 1], 3 << 20),      # row tiles
+    ([3000, 1100], [1, 0], 1 << 20)])          # the GEMM
+def test_offsets_past_32_bits(type, rows, slots, pitch):
+    c = Case(type, rows, slots, [16] * (max(slots) + 1), 200, 139)
+    c.xb = far_rows(c.xb[:c.m, :c.inn], pitch + 8)
+    c.yb = far_rows(c.yb[:c.m, :c.out], pitch)
+    c.run()
+    c.check()
+    del c
+    torch.cuda.empty_cache()
+
+
 @BOTH
 @pytest.mark.parametrize("m", [6, 300])
 def test_a_row_with_infinities_or_nan_reaches_no_other_row(type, m):

@@ -133,6 +133,31 @@ def test_odd_strides_offsets_and_orders(type, shift):
         assert bool((oraw[left] == 7.0).all())
 
 
+@pytest.mark.parametrize("type", [ops.F16, ops.F32])
+def test_offsets_past_32_bits(type):
+    """Heads, then tokens, more than 2^32 elements apart."""
+    far = (1 << 32) + 8
+    freqs, _ = ops.rope_freqs(10000.0, 32)
+    raw = torch.empty(far + 3 * 48, device="cuda", dtype=DT[type])
+    wide, near = raw.as_strided((3, 2, 48), (48, far, 1)), torch.randn(3, 2, 48, device="cuda").to(DT[type])
+    ops.rope(ops.RopeSpec(type, 48, 32, freqs), [rt(near, wide)], 3, pos0=9, stream=stream())
+    check(wide, *oracle(near, torch.arange(9, 12), freqs, 32, ops.ROPE_HALF, False, 1.0))
+    wide = raw.as_strided((2, 3, 48), (far, 48, 1))
+    wide.copy_(torch.randn(2, 3, 48, device="cuda"))
+    near = torch.empty(2, 3, 48, device="cuda", dtype=DT[type])
+    ops.rope(ops.RopeSpec(type, 48, 32, freqs), [rt(wide, near)], 2, pos0=9, stream=stream())
+    check(near, *oracle(wide, torch.arange(9, 11), freqs, 32, ops.ROPE_HALF, False, 1.0))
+    del raw, wide
+    torch.cuda.empty_cache()
+
+
+def test_many_tokens_of_one_pair():
+    n = 3000001
+    x, o = torch.randn(n, 1, 2, device="cuda"), torch.empty(n, 1, 2, device="cuda")
+    ops.rope(ops.RopeSpec(ops.F32, 2, 2, [0.37]), [rt(x, o)], n, stream=stream())
+    check(o, *oracle(x, torch.arange(n), [0.37], 2, ops.ROPE_HALF, False, 1.0))
+
+
 def test_repeated_input_rows():
     """Stride 0 over heads: one key read for every head."""
     freqs, _ = ops.rope_freqs(10000.0, 64)
