@@ -12,11 +12,12 @@
 // conversion rounds relative to itself.
 //
 // Bound by memory: every element is read and written once.  A block takes a few
-// tokens and all their heads (up to 256 pieces of 16 bytes times 4 heads), so
-// a sine and cosine is computed once for all heads and passed through shared
-// memory, and a thread turns one piece (for the half layout the piece and its
-// partner rot / 2 further) of up to 4 heads, all loaded before the angles are
-// computed.
+// tokens and all their heads (up to 256 units of two 16-byte pieces times 4 heads),
+// so a sine and cosine is computed once for all heads and passed through shared
+// memory, and all of a thread's loads are issued before it needs an angle.
+// Measured: 65536 tokens x 40 heads x 128, bf16: 207 us, 6.5 TB/s, the rate of a
+// plain copy; 9872 x 32 x 64, f16: 15.2 us, 5.3 TB/s (4.2 tiles a block: ramp and
+// tail); 3001 x 15 x 80 with 20 rotated, f32: 7.0 us, 4.1 TB/s; 1 token: 1.7 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -122,8 +123,15 @@ __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
 }
 
 constexpr int kThreads = 256;
-constexpr int kBlocksPerSm = 3;              // at most 80 registers a thread
-constexpr int kMaxHeads = 4;                 // heads a thread turns, all loaded before the first is turned
+static_assert(kMaxPairs <= kThreads, "a head's units, of two elements at least, fit a block");
+constexpr int kMaxHeads = 4;  // heads a thread turns, all loaded before the first is turned
+// Blocks an SM.  Pieces of 16 bytes need 128 registers a thread to have a tile's
+// loads in flight together (65536 tokens x 40 heads x 128, bf16: 2 blocks 207 us, 3
+// blocks 217 us), but not in the half layout with dims to copy, whose two kinds
+// of unit overlap better in 3 blocks (rot 64 of the same: 251 and 221 us); smaller
+// pieces need more threads (9872 x 15 x 37, rot 36, f16: 13.2 and 10.9 us).
+template <class T, int VEC, bool HALF, bool COPY>
+constexpr int kBlocks = sizeof(T) * VEC == 16 && !(HALF && COPY) ? 2 : 3;
 
 // (a c - b s, b c + a s), a pair of pairs an instruction (packed f32 pairs, each
 // rounded as the scalar operation).
@@ -185,40 +193,49 @@ __device__ __forceinline__ void turn_within(Vec<T, VEC>& p, const float (&c)[VEC
 }
 
 // A block turns tiles of a.block_tokens tokens by a.block_groups groups of
-// heads, one tile after another; a thread keeps its place in the tile (piece,
+// heads, one tile after another; a thread keeps its place in the tile (unit,
 // then group, then token), so its index arithmetic is done once.  The angles of
 // the next tile go to the other half of the shared buffer while this tile's
-// loads are in flight.  Pieces of VEC elements: rot / 2 (half) or rot
-// (interleaved), dim - rot, every stride and address are multiples of VEC.
-template <class T, int VEC, bool HALF>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __grid_constant__ RopeArgs a) {
+// loads are in flight.  A unit is two pieces of VEC elements: a piece and what it
+// turns with, two pieces of neighbouring pairs, or (COPY: rot < dim) two to copy.
+// rot / 2 (half) or rot (interleaved), dim - rot, every stride and address are
+// multiples of VEC.
+template <class T, int VEC, bool HALF, bool COPY>
+__global__ void __launch_bounds__(kThreads, kBlocks<T, VEC, HALF, COPY>) rope_kernel(const __grid_constant__ RopeArgs a) {
   using P = Vec<T, VEC>;
-  constexpr int kPairs = HALF ? VEC : (VEC + 1) / 2;
-  constexpr int kPieces = HALF || VEC == 1 ? 2 : 1;  // pieces a unit turns
-  extern __shared__ __align__(16) float angles[];    // [2][cos | sin][block_tokens * half]
+  constexpr bool kWithin = !HALF && VEC > 1;       // a pair lies within a piece
+  constexpr int kPairs = kWithin ? VEC / 2 : VEC;  // of a piece
+  extern __shared__ __align__(16) float angles[];  // [2][cos | sin][block_tokens * half]
   const int half = a.rot / 2;
-  const int turned = half / kPairs;
-  const int units = turned + (a.dim - a.rot) / VEC;
-  const int block_units = min(units, kThreads);  // heads of more pieces: grid.z parts of them
-  const int per_tok = a.block_groups * block_units;
+  const int turned_pieces = kWithin ? a.rot / VEC : 0;
+  const int turned = kWithin ? (turned_pieces + 1) / 2 : half / VEC;  // units that turn
+  const int copied_pieces = COPY ? (a.dim - a.rot) / VEC : 0, copied = (copied_pieces + 1) / 2;
+  const int units = turned + copied;
+  const int per_tok = a.block_groups * units;
   const int n_angles = a.block_tokens * half;
   const long long tiles = (a.tokens + a.block_tokens - 1) / a.block_tokens;
 
   // this thread's place (a tile has at most kThreads of them)
   const int tl = static_cast<int>(threadIdx.x) / per_tok, gu = static_cast<int>(threadIdx.x) - tl * per_tok;
-  const int group = static_cast<int>(blockIdx.y) * a.block_groups + gu / block_units;
-  const int u = static_cast<int>(blockIdx.z) * block_units + gu % block_units;
+  const int group = static_cast<int>(blockIdx.y) * a.block_groups + gu / units, u = gu % units;
   int ti = 0;
   while (ti + 1 < a.count && group >= a.t[ti + 1].group0) ++ti;
   const RopeTensorArg t = a.t[ti];
   const int h0 = (group - t.group0) * a.heads_per_thread;
-  const bool turn = u < turned;
-  int nh = tl < a.block_tokens && group < a.groups && u < units ? min(a.heads_per_thread, t.heads - h0) : 0;
+  const bool turn = !COPY || u < turned;
+  int nh = tl < a.block_tokens && group < a.groups ? min(a.heads_per_thread, t.heads - h0) : 0;
   if (!turn && t.x == t.out) nh = 0;
-  const int at0 = turn ? (HALF ? u * VEC : u * kPieces * VEC) : a.rot + (u - turned) * VEC;
-  const int at1 = HALF ? half + u * VEC : at0 + VEC;
-  const T* const x0 = static_cast<const T*>(t.x) + h0 * t.x_head;
-  T* const o0 = static_cast<T*>(t.out) + h0 * t.out_head;
+  // its first piece, and from there to its second (0: it has none)
+  int at, step;
+  if (turn) {
+    at = kWithin || HALF ? u * VEC : 2 * u;
+    step = kWithin ? (u + turned < turned_pieces ? turned * VEC : 0) : HALF ? half : 1;
+  } else {
+    at = a.rot + (u - turned) * VEC;
+    step = u - turned + copied < copied_pieces ? copied * VEC : 0;
+  }
+  const T* const x0 = static_cast<const T*>(t.x) + h0 * t.x_head + at;
+  T* const o0 = static_cast<T*>(t.out) + h0 * t.out_head + at;
   // the first of the angles it computes
   const int my_at = static_cast<int>(threadIdx.x) / half, my_j = static_cast<int>(threadIdx.x) - my_at * half;
 
@@ -226,9 +243,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __gr
   grid_dep_trigger();
 
   auto compute_angles = [&](long long tile, float* buf) {
-    int at = my_at, j = my_j;
+    int tok_at = my_at, j = my_j;
     for (int i = threadIdx.x; i < n_angles; i += kThreads) {
-      const long long tok = tile * a.block_tokens + at;
+      const long long tok = tile * a.block_tokens + tok_at;
       if (tok < a.tokens) {
         const long long pos = a.pos ? __ldg(a.pos + tok) : a.pos0 + tok;
         float c, s;
@@ -237,8 +254,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __gr
         buf[n_angles + i] = s * (a.mscale * a.sign);
       }
       if (i + kThreads < n_angles) {
-        at = (i + kThreads) / half;
-        j = i + kThreads - at * half;
+        tok_at = (i + kThreads) / half;
+        j = i + kThreads - tok_at * half;
       }
     }
   };
@@ -248,41 +265,48 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __gr
   int parity = 0;
   for (; tile < tiles; tile += gridDim.x, parity ^= 1) {
     const long long tok = tile * a.block_tokens + tl;
-    const int n = tok < a.tokens ? nh : 0;
+    const int n = tok < a.tokens ? nh : 0, n2 = (HALF && !COPY) || step ? n : 0;
     const T* x = x0 + tok * t.x_token;
     T* o = o0 + tok * t.out_token;
     P p[kMaxHeads], q[kMaxHeads];
 #pragma unroll
-    for (int k = 0; k < kMaxHeads; ++k)
-      if (k < n) {
-        p[k] = *reinterpret_cast<const P*>(x + k * t.x_head + at0);
-        if (kPieces == 2 && turn) q[k] = *reinterpret_cast<const P*>(x + k * t.x_head + at1);
-      }
+    for (int k = 0; k < kMaxHeads; ++k) {
+      if (k < n) p[k] = *reinterpret_cast<const P*>(x + k * t.x_head);
+      if (k < n2) q[k] = *reinterpret_cast<const P*>(x + k * t.x_head + step);
+    }
     __syncthreads();  // this tile's angles are there; the other buffer was read
     if (tile + gridDim.x < tiles) compute_angles(tile + gridDim.x, angles + (parity ^ 1) * 2 * n_angles);
     if (n <= 0) continue;
     if (turn) {
       float c[kPairs], s[kPairs];
       const float* cs = angles + parity * 2 * n_angles + tl * half + u * kPairs;
+      auto load_angles = [&] {
 #pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        c[j] = cs[j];
-        s[j] = cs[n_angles + j];
-      }
+        for (int j = 0; j < kPairs; ++j) {
+          c[j] = cs[j];
+          s[j] = cs[n_angles + j];
+        }
+      };
+      load_angles();
+      if constexpr (kWithin) {
 #pragma unroll
-      for (int k = 0; k < kMaxHeads; ++k) {
-        if constexpr (kPieces == 2)
-          turn_across<T, VEC>(p[k], q[k], c, s);
-        else
-          turn_within<T, VEC>(p[k], c, s);
+        for (int k = 0; k < kMaxHeads; ++k) turn_within<T, VEC>(p[k], c, s);
+        if (n2 > 0) {
+          cs += turned * kPairs;
+          load_angles();
+        }
+#pragma unroll
+        for (int k = 0; k < kMaxHeads; ++k) turn_within<T, VEC>(q[k], c, s);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kMaxHeads; ++k) turn_across<T, VEC>(p[k], q[k], c, s);
       }
     }
 #pragma unroll
-    for (int k = 0; k < kMaxHeads; ++k)
-      if (k < n) {
-        *reinterpret_cast<P*>(o + k * t.out_head + at0) = p[k];
-        if (kPieces == 2 && turn) *reinterpret_cast<P*>(o + k * t.out_head + at1) = q[k];
-      }
+    for (int k = 0; k < kMaxHeads; ++k) {
+      if (k < n) *reinterpret_cast<P*>(o + k * t.out_head) = p[k];
+      if (k < n2) *reinterpret_cast<P*>(o + k * t.out_head + step) = q[k];
+    }
   }
 }
 
@@ -305,11 +329,29 @@ __global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__
   a.sinb[i] = a.mscale * s;
 }
 
-template <class T, int VEC>
-cudaError_t launch_vec(const RopeArgs& a, bool half, dim3 grid, cudaStream_t st) {
+template <class T, int VEC, bool HALF, bool COPY>
+cudaError_t launch_kernel(const RopeArgs& a, int num_sms, cudaStream_t st) {
+  constexpr int kResident = kBlocks<T, VEC, HALF, COPY>;
+  const unsigned gy = (a.groups + a.block_groups - 1) / a.block_groups;
+  // the resident blocks, each walking over its share of the tiles
+  const long long tiles = (a.tokens + a.block_tokens - 1) / a.block_tokens;
+  long long blocks = std::max<long long>(1, static_cast<long long>(kResident) * num_sms / gy);
+  // A walk of many tiles in up to 4 rounds of blocks of at least 8 tiles, so that
+  // no block falls far behind (65536 tokens x 40 heads x 128, bf16: 217 -> 207 us;
+  // with 4 tiles a block it costs, 9872 x 32 x 64, f16: 15.7 -> 16.7 us).
+  if (kResident == 2) blocks *= std::clamp<long long>(tiles / (8 * blocks), 1, 4);
+  const dim3 grid(static_cast<unsigned>(std::min(tiles, blocks)), gy);
   const size_t smem = 4 * sizeof(float) * a.block_tokens * (a.rot / 2);
-  return half ? launch_pdl(rope_kernel<T, VEC, true>, grid, dim3(kThreads), smem, st, nullptr, 0, a)
-              : launch_pdl(rope_kernel<T, VEC, false>, grid, dim3(kThreads), smem, st, nullptr, 0, a);
+  return launch_pdl(rope_kernel<T, VEC, HALF, COPY>, grid, dim3(kThreads), smem, st, nullptr, 0, a);
+}
+
+template <class T, int VEC>
+cudaError_t launch_vec(const RopeArgs& a, bool half, int num_sms, cudaStream_t st) {
+  if (a.dim == a.rot)
+    return half ? launch_kernel<T, VEC, true, false>(a, num_sms, st)
+                : launch_kernel<T, VEC, false, false>(a, num_sms, st);
+  return half ? launch_kernel<T, VEC, true, true>(a, num_sms, st)
+              : launch_kernel<T, VEC, false, true>(a, num_sms, st);
 }
 
 // Whether pieces of `v` elements of `es` bytes fit the head, every stride and
@@ -329,12 +371,14 @@ cudaError_t launch_rope(RopeArgs& a, bool half, int num_sms, cudaStream_t st) {
   constexpr int es = sizeof(T), kMaxVec = 16 / es;
   int v = kMaxVec;
   while (v > 1 && !pieces_fit(a, half, es, v)) v /= 2;
-  const int units = (half ? a.rot / 2 / v : v == 1 ? a.rot / 2 : a.rot / v) + (a.dim - a.rot) / v;
-  // heads a thread: 4, fewer while the call would not fill the SMs
+  const int units = (half || v == 1 ? a.rot / 2 / v : (a.rot / v + 1) / 2) + ((a.dim - a.rot) / v + 1) / 2;
+  // heads a thread: 4, fewer while there would be under 192 threads an SM (500
+  // tokens x 15 heads x 80, f32: 4 heads 2.9 us, 1 head 4.5 us; 700 x 32 x 64, f16:
+  // 2 heads 3.3, 4 heads 3.5; 1 x 32 x 64, f16: 1 head 2.1 us, 4 heads 2.5 us)
   int heads = 0;
   for (int i = 0; i < a.count; ++i) heads += a.t[i].heads;
   a.heads_per_thread = kMaxHeads;
-  while (a.heads_per_thread > 1 && a.tokens * units * heads < 1024ll * num_sms * a.heads_per_thread)
+  while (a.heads_per_thread > 1 && a.tokens * units * heads < 192ll * num_sms * a.heads_per_thread)
     a.heads_per_thread /= 2;
   a.groups = 0;
   for (int i = 0; i < a.count; ++i) {
@@ -343,17 +387,11 @@ cudaError_t launch_rope(RopeArgs& a, bool half, int num_sms, cudaStream_t st) {
   }
   a.block_groups = std::min(a.groups, std::max(1, kThreads / units));
   a.block_tokens = std::max(1, kThreads / (a.block_groups * units));
-  const unsigned gz = (units + kThreads - 1) / kThreads;
-  const unsigned gy = (a.groups + a.block_groups - 1) / a.block_groups;
-  // the resident blocks, each walking over its share of the tiles
-  const long long tiles = (a.tokens + a.block_tokens - 1) / a.block_tokens;
-  const long long want = std::max<long long>(1, static_cast<long long>(kBlocksPerSm) * num_sms / (gy * gz));
-  const dim3 grid(static_cast<unsigned>(std::min(tiles, want)), gy, gz);
   switch (v) {
-    case 8: return launch_vec<T, kMaxVec>(a, half, grid, st);
-    case 4: return launch_vec<T, 4>(a, half, grid, st);
-    case 2: return launch_vec<T, 2>(a, half, grid, st);
-    default: return launch_vec<T, 1>(a, half, grid, st);
+    case 8: return launch_vec<T, kMaxVec>(a, half, num_sms, st);
+    case 4: return launch_vec<T, 4>(a, half, num_sms, st);
+    case 2: return launch_vec<T, 2>(a, half, num_sms, st);
+    default: return launch_vec<T, 1>(a, half, num_sms, st);
   }
 }
 

@@ -72,6 +72,22 @@ def test_against_64_bits(type, layout, tokens, heads, dim, rot):
         check(out, *oracle(x, pos, freqs, rot, layout, inverse, m))
 
 
+@pytest.mark.parametrize("type", [ops.F16, ops.BF16, ops.F32])
+@pytest.mark.parametrize("layout", [ops.ROPE_HALF, ops.ROPE_INTERLEAVED])
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("tokens,heads,dim,rot", [(50, 6, 40, 24), (50, 6, 64, 24), (9, 3, 120, 40), (900, 7, 24, 24), (5, 1, 56, 8),
+                                                  (3000, 40, 128, 64), (700, 20, 96, 80), (33, 5, 511, 510), (20000, 9, 64, 64),
+                                                  (4, 6, 512, 8), (2, 3, 500, 2)])
+def test_odd_numbers_of_pieces(type, layout, inplace, tokens, heads, dim, rot):
+    """Turned and copied parts that are an odd number of pieces, and walks of many tiles."""
+    x = torch.randn(tokens, heads, dim, device="cuda").to(DT[type])
+    out = x.clone() if inplace else torch.full_like(x, float("nan"))
+    freqs, _ = ops.rope_freqs(10000.0, rot)
+    ops.rope(ops.RopeSpec(type, dim, rot, freqs, layout), [rt(out if inplace else x, out)], tokens, pos0=3, stream=stream())
+    check(out, *oracle(x, torch.arange(3, 3 + tokens), freqs, rot, layout, False, 1.0))
+    assert torch.equal(out[..., rot:], x[..., rot:])
+
+
 def test_far_and_negative_positions():
     freqs, _ = ops.rope_freqs(10000.0, 64)
     pos = torch.tensor([0, 1, -1, 2**31 - 1, -2**31, 2**30 + 7, 123456789, -987654321], dtype=torch.int32, device="cuda")
