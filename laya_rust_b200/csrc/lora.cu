@@ -118,6 +118,8 @@ __device__ __forceinline__ void bulk_to_rank(const void* dst, uint64_t* bar, con
 // the rows' adapters.  Then a thread has its row's sums in TMEM: alone it stores
 // them; in a cluster each CTA owns a share of the rows, the others send it
 // their sums with one bulk copy each, and it adds them in rank order.
+// Bound by the latency of its chain (loads, MMA, exchange): about 5 us for 9872
+// rows, 1024 inputs, 16 adapters of rank 16, where x alone is 3 us of HBM.
 template <class T, int SPLITS>
 __global__ void __launch_bounds__(128, 1)
     lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
@@ -306,7 +308,9 @@ __global__ void __launch_bounds__(128, 1)
 }
 
 // u = scale (x A^T) for one (row, chunk) pair a block: a warp takes two of the
-// chunk's 16 rows of A over all of K, so no sum leaves its warp.
+// chunk's 16 rows of A over all of K, so no sum leaves its warp.  A is read once
+// a pair, 32 bytes an input and pair from HBM or L2 (48 rows with an adapter each,
+// 1024 inputs, with the projection behind it: 10.5 us, by items 14).
 template <class T>
 __global__ void __launch_bounds__(256) lora_pairs_kernel(const LoraPairsArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -399,6 +403,8 @@ cudaError_t launch_lora_pairs(const LoraPairsArgs& a, cudaStream_t s) {
   return launch_pdl(kernel, dim3(a.pairs), dim3(256), 0, s, nullptr, 0, a);
 }
 
+// As many parts as keep every item on an SM (3034 rows, 1024 -> 3072, 16 adapters:
+// 4 parts 24 us, 8 parts 34; 9872 rows: 1 part 59 us, 2 parts 71).
 int lora_splits(int rows, int num_sms) {
   const int halves = (rows + kLoraItemRows - 1) / kLoraItemRows;
   int splits = 1;
@@ -422,7 +428,9 @@ LoraItems lora_items(const LoraLayout& L, int num_sms) {
       for (int e = e0; e < static_cast<int>(L.chunk.size()) && (e == e0 || L.chunk[e].y > 0); ++e) v.push_back(e);
     }
   }
-  // the smallest group whose items still run at once
+  // the smallest group whose items still run at once (9872 rows of 16 adapters,
+  // 1024 -> 3072, in all: groups of 1 entry 63 us, of 2 as chosen here 59; 3034
+  // rows: 1 or 2 28 us, 4 as chosen 24, 8 27)
   const size_t most = num_sms / lora_splits(L.rows, num_sms);
   for (it.group = 1;; it.group *= 2) {
     size_t items = 0;
@@ -609,6 +617,8 @@ struct Plan {
   const int* d_item_entry = nullptr;
   const int* d_item_chunk = nullptr;
   const int4* d_pair = nullptr;
+  const int* d_soff = nullptr;
+  const int2* d_list = nullptr;
   int pairs = 0;  // > 0: the rank-space product goes by pairs, not items
   const int* d_row_entry = nullptr;
   const int* d_entry_chunk = nullptr;
@@ -627,8 +637,13 @@ struct Plan {
   }
 };
 
-// Few (row, chunk) pairs take a block each, reading 16 rows of A from L2.
-constexpr size_t kLoraMaxPairs = 512;
+// The rank-space product by (row, chunk) pairs, a block each that reads 16 rows of
+// A, or by items of 128 rows?  Pairs while they are few, or few of them share
+// an adapter's chunk: 256 rows with an adapter each, 1024 -> 3072: 23 us, by items
+// 39; 2048 of them 85 and 147 us; 128 segments of 8 rows, 16 adapters, 16 and 24 us;
+// but 64 segments of 16 rows, 64 adapters of rank 64, 2624 -> 1024 (4096 pairs of 256
+// chunks): 63 and 58 us.
+bool lora_by_pairs(size_t pairs, size_t entries) { return pairs <= 1024 || pairs <= 8 * entries; }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -761,7 +776,7 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     // items of 128 rows
     const bool u_apart = !q.small.fused;
     std::vector<int4> pair;
-    for (int m = 0; u_apart && m < L.rows && pair.size() <= kLoraMaxPairs; ++m) {
+    for (int m = 0; u_apart && m < L.rows && lora_by_pairs(pair.size(), L.chunk.size()); ++m) {
       const int e0 = L.row_entry[m];
       if (e0 < 0) continue;
       for (int e = e0; e < static_cast<int>(L.chunk.size()) && (e == e0 || L.chunk[e].y > 0); ++e)
@@ -769,7 +784,7 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     }
     LoraItems it;
     if (!u_apart) {
-    } else if (pair.size() <= kLoraMaxPairs) {
+    } else if (lora_by_pairs(pair.size(), L.chunk.size())) {
       q.pairs = static_cast<int>(pair.size());
     } else {
       pair.clear();
@@ -780,12 +795,15 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     q.items = static_cast<int>(it.item.size());
     q.group = it.group;
     // [error word | off | row entries | entry chunks | items | their entries |
-    // their chunks | pairs], each 256-byte aligned
+    // their chunks | pairs | row tiles' lists], each 256-byte aligned
     auto up = [](size_t v) { return (v + 63) / 64 * 64; };
     const size_t o_off = 64, o_row = o_off + up(L.off.size()), o_ent = o_row + up(L.row_entry.size());
     const size_t o_item = o_ent + up(entry_chunk.size()), o_ie = o_item + up(4 * it.item.size());
     const size_t o_ic = o_ie + up(it.entry.size()), o_pair = o_ic + up(item_chunk.size());
-    std::vector<int> h(o_pair + up(4 * pair.size()));
+    const size_t o_soff = o_pair + up(4 * pair.size()), o_list = o_soff + up(q.small.off.size());
+    std::vector<int> h(o_list + up(2 * q.small.list.size()));
+    std::copy(q.small.off.begin(), q.small.off.end(), h.begin() + o_soff);
+    if (!q.small.list.empty()) memcpy(h.data() + o_list, q.small.list.data(), q.small.list.size() * sizeof(int2));
     if (!pair.empty()) memcpy(h.data() + o_pair, pair.data(), pair.size() * sizeof(int4));
     std::copy(item_chunk.begin(), item_chunk.end(), h.begin() + o_ic);
     if (!it.item.empty()) memcpy(h.data() + o_item, it.item.data(), it.item.size() * sizeof(int4));
@@ -812,6 +830,8 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     q.d_item_entry = q.dev.as<int>() + o_ie;
     q.d_item_chunk = q.dev.as<int>() + o_ic;
     q.d_pair = reinterpret_cast<const int4*>(q.dev.as<int>() + o_pair);
+    q.d_soff = q.dev.as<int>() + o_soff;
+    q.d_list = reinterpret_cast<const int2*>(q.dev.as<int>() + o_list);
     *plan = p.release();
   });
 }
@@ -885,6 +905,8 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
           make_tmap_lora(&mb, k.b.p, k.bf16, static_cast<uint64_t>(k.slots) * k.cps * k.out_pad, width))
         throw OpError(LAYA_E_CUDA, "lora_run: tensor map encode failed");
       LoraSmallArgs g{};
+      g.off = q.d_soff;
+      g.list = q.d_list;
       g.entry_chunk = q.d_entry_chunk;
       g.row_entry = q.d_row_entry;
       g.scale = k.scale.as<float>();
@@ -908,7 +930,8 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       return;
     }
     // 256 x 128 tiles where 256 x 256 ones would fill at most half the
-    // clusters, as in the engine
+    // clusters, as in the engine (600 rows, 1024 -> 1024, 2 adapters: 9.9 us and,
+    // wide, 12.4; 1300 rows -> 3072: 16.3 and, wide, 15.4)
     const int tiles = (q.lay.rows + kGemmBM - 1) / kGemmBM * (k.out_pad / kGemmBN);
     const bool narrow = tiles * 2 <= k.num_sms / 2;
     const int bn = narrow ? kGemmBNNarrow : kGemmBN;

@@ -126,8 +126,9 @@ cudaError_t launch_lora_pairs(const LoraPairsArgs& a, cudaStream_t s);
 
 // The projection of few rows: lora_small.cu.  Row tiles of xrows (a multiple
 // of 16), tiles of `width` output columns.  `fused`: it computes u too, for at
-// most kLoraMaxGroup entries a row tile; otherwise u is there, or comes from the
-// launch before it (early), for one block of rows (entries 0 .. entries - 1).
+// most kLoraMaxGroup entries a row tile; otherwise u comes from the launch before
+// it (early), and row tile t reads list[off[t]] .. list[off[t + 1] - 1], the
+// (entry, its chunk in the bank) some row of it has.
 // Maps: x [rows, in] box 64 x xrows, W box 64 x width, u box xrows, B box
 // width, A box 64 x 16.
 constexpr int kLoraSmallTile = 128;   // most rows a tile
@@ -135,7 +136,9 @@ constexpr int kLoraSmallTiles = 40;   // most row tiles with entries
 struct LoraSmallPlan {
   bool use = false, fused = false;
   int xrows = 0, width = 0;
-  int entries = 0;                                     // fused: of the fullest tile
+  int entries = 0;                                     // of the fullest tile
+  std::vector<int> off;                                // not fused: each tile's part
+  std::vector<int2> list;                              // of the list
   int tile_entries[kLoraSmallTiles] = {};              // fused: of each row tile,
   int chunk[kLoraSmallTiles][kLoraMaxGroup] = {};      // and their chunks in the bank
 };
@@ -143,6 +146,8 @@ struct LoraSmallPlan {
 LoraSmallPlan lora_small_plan(const LoraLayout& L, int out, int chunks_per_slot, int num_sms);
 
 struct LoraSmallArgs {
+  const int* off;
+  const int2* list;
   const int* entry_chunk;
   const int* row_entry;
   const float* scale;

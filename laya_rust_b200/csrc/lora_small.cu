@@ -21,6 +21,12 @@
 // CTA turns the entries it owns into 16-bit operands of the adapter step in its
 // own shared memory.  Every cluster repeats u for its rows (16 rows of A per entry
 // from L2), which costs less than a launch of its own.
+//
+// With more entries u comes from the launch before, and a row tile goes through
+// the list of the entries some row of it has (256 rows with an adapter each, 1024
+// -> 3072: 19.5 us; through all of the block's 256 entries 46.9, by the GEMM
+// 36.5).  Measured otherwise: one row, 1024 -> 3072, rank 16: 5.6 us; 179 rows,
+// 2624 -> 1024, rank 32: 9.3 us; 48 rows with an adapter each: 10.5 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -142,7 +148,7 @@ __global__ void __launch_bounds__(kThreads)
   const int xrows = a.xrows, m0 = static_cast<int>(blockIdx.y) * xrows;
   // FUSED: this row tile's entries
   const int* const chunk = a.chunk[FUSED ? blockIdx.y : 0];
-  const int entries = FUSED ? a.tile_entries[blockIdx.y] : a.entries;
+  const int entries = FUSED ? a.tile_entries[blockIdx.y] : 0;
   const int rows = min(xrows, a.rows - m0);
   constexpr int kParts = std::is_same<T, __nv_bfloat16>::value ? 2 : 1;  // operands of u an entry has
   constexpr int kPerStage = 4 / kParts;                                    // entries a stage
@@ -151,7 +157,15 @@ __global__ void __launch_bounds__(kThreads)
   const int stage_bytes = kWBytes + x_bytes + (FUSED && !joint ? a.entries * kABytes : 0);
   const int load_bytes = width * 128 + x_bytes + (FUSED ? entries * kABytes : 0);
   const int kb0 = rank * a.num_kb / SPLITS, kb1 = (rank + 1) * a.num_kb / SPLITS;
-  const int e0 = rank * entries / SPLITS, e1 = (rank + 1) * entries / SPLITS;
+  int e0 = rank * entries / SPLITS, e1 = (rank + 1) * entries / SPLITS;
+  // else: this CTA's part of the tile's list, read by each role once it has
+  // something else to wait for
+  auto find_entries = [&] {
+    if (FUSED || a.entries == 0) return;
+    const int first = __ldg(a.off + blockIdx.y), n = __ldg(a.off + blockIdx.y + 1) - first;
+    e0 = first + rank * n / SPLITS;
+    e1 = first + (rank + 1) * n / SPLITS;
+  };
   const int need_cols = FUSED && !joint ? 2 * xrows : xrows;
   const uint32_t tmem_cols = need_cols <= 32 ? 32 : need_cols <= 64 ? 64 : need_cols <= 128 ? 128 : 256;
   // A cluster: [owned B operands | owned u operands] [ring] [part] [parts sent
@@ -234,6 +248,7 @@ __global__ void __launch_bounds__(kThreads)
         }
         next();
       }
+      find_entries();
       if constexpr (FUSED) {
         if (e0 < e1 && ok) {
           mbar_arrive_expect_tx(&b_full, (e1 - e0) * width * 32);
@@ -247,13 +262,25 @@ __global__ void __launch_bounds__(kThreads)
         auto load_b = [&](int st, int e, int n) {
           uint8_t* sb = ring + st * stage_bytes;
           mbar_arrive_expect_tx(&full[st], n * (kBBytes + kParts * u_bytes));
-          for (int i = 0; i < n; ++i)
-            tma_load_2d(sb + i * kBBytes, &maps.b, 0, (__ldg(a.entry_chunk + e + i) * a.b_rows + n0) / 4, &full[st]);
+          int c[kPerStage];
+#pragma unroll
+          for (int i = 0; i < kPerStage; ++i) c[i] = i < n ? __ldg(&a.list[e + i].y) : 0;
+#pragma unroll
+          for (int i = 0; i < kPerStage; ++i)
+            if (i < n) tma_load_2d(sb + i * kBBytes, &maps.b, 0, (c[i] * a.b_rows + n0) / 4, &full[st]);
         };
-        auto load_u = [&](int st, int e, int n) {
-          for (int i = 0; i < n; ++i) {
+        // of the next stage
+        int ent[kPerStage];
+        auto find_u = [&](int e) {
+#pragma unroll
+          for (int i = 0; i < kPerStage; ++i) ent[i] = e + i < e1 ? __ldg(&a.list[e + i].x) : 0;
+        };
+        auto load_u = [&](int st, int n) {
+#pragma unroll
+          for (int i = 0; i < kPerStage; ++i) {
+            if (i >= n) break;
             uint8_t* su = ring + st * stage_bytes + kWBytes + i * kParts * u_bytes;
-            const int y = (e + i) * kParts * kLoraBlock + m0;
+            const int y = ent[i] * kParts * kLoraBlock + m0 % kLoraBlock;
             tma_load_2d(su, &maps.u, 0, y / 4, &full[st]);
             if (kParts == 2) tma_load_2d(su + u_bytes, &maps.u, 0, (y + kLoraBlock) / 4, &full[st]);
           }
@@ -268,6 +295,7 @@ __global__ void __launch_bounds__(kThreads)
             ph ^= 1u;
           }
         }
+        find_u(e0);
         grid_dep_wait();  // u is complete
         for (int e = e0; e < e1; e += kPerStage) {
           const int n = min(kPerStage, e1 - e);
@@ -276,7 +304,8 @@ __global__ void __launch_bounds__(kThreads)
             if (!ok) break;
             load_b(stage, e, n);
           }
-          load_u(stage, e, n);
+          load_u(stage, n);
+          find_u(e + kPerStage);
           next();
         }
       }
@@ -289,6 +318,7 @@ __global__ void __launch_bounds__(kThreads)
     __syncwarp();
   } else if (warp == 1) {
     if (elect_one()) {
+      find_entries();
       bool ok = true;
       int stage = 0;
       uint32_t phase = 0;
@@ -341,7 +371,14 @@ __global__ void __launch_bounds__(kThreads)
       umma_commit(&done);
     }
     __syncwarp();
-  } else if (FUSED) {
+  } else if (!FUSED) {
+    // the list, into this SM's L1 before warp 0 asks for it
+    find_entries();
+    for (int e = e0 + 16 * (static_cast<int>(threadIdx.x) - 64); e < e1; e += 16 * 64) {
+      int v;
+      asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(&a.list[e]));
+    }
+  } else {
     // whose adapter each row has, while the other warps load and multiply
     for (int m = static_cast<int>(threadIdx.x) - 64; m < xrows; m += 64) {
       const int re = m < rows ? __ldg(a.row_entry + m0 + m) : -1;
@@ -574,10 +611,24 @@ LoraSmallPlan lora_small_plan(const LoraLayout& L, int out, int chunks_per_slot,
         chunk[n++] = c;
       }
     }
-    if (any && !fits && !one_block) continue;  // u by its own launch: one block of rows only
     p.fused = any && fits;
     const int most = *std::max_element(p.tile_entries, p.tile_entries + tiles);
-    p.entries = p.fused ? most : static_cast<int>(L.chunk.size());
+    p.entries = most;
+    if (any && !fits) {
+      std::vector<int> seen(L.chunk.size(), -1);
+      for (int t = 0; t < tiles; ++t) {
+        p.off.push_back(static_cast<int>(p.list.size()));
+        for (int m = t * xrows; m < std::min(rows, (t + 1) * xrows); ++m) {
+          const int e0 = L.row_entry[m];
+          if (e0 < 0 || seen[e0] == t) continue;
+          seen[e0] = t;
+          for (int e = e0; e < static_cast<int>(L.chunk.size()) && (e == e0 || L.chunk[e].y > 0); ++e)
+            p.list.push_back(make_int2(e, L.chunk[e].x * chunks_per_slot + L.chunk[e].y));
+        }
+        p.entries = std::max(p.entries, static_cast<int>(p.list.size()) - p.off.back());
+      }
+      p.off.push_back(static_cast<int>(p.list.size()));
+    }
     // joint pays where the K loop carries many rows (256 rows, 1024 -> 3072, one
     // entry: 9.9 us, apart 12.0 us); with few, more tiles cost more than a second
     // operand (1 row: joint 5.7 us, apart 5.4 us)
@@ -585,7 +636,9 @@ LoraSmallPlan lora_small_plan(const LoraLayout& L, int out, int chunks_per_slot,
       if (width < kCols && !(p.fused && most <= 4 && rows > 32)) continue;
       p.width = width;
       // every CTA on an SM of its own; failing that, within one block of rows,
-      // the smaller tiles in rounds (beyond it the GEMM is faster)
+      // the smaller tiles in rounds (beyond it the GEMM is faster: 1000 rows of 100
+      // adapters, 1024 -> 3072, 27 us and, in two rounds, 51; in one round: 768 rows
+      // with an adapter each, 2624 -> 1024, 56 us by the GEMM, 34 here)
       if ((out + width - 1) / width * tiles <= num_sms) return p;
       if (one_block && !best.use) best = p;
     }
@@ -599,7 +652,7 @@ cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const 
   const int row_tiles = a.xrows > 0 ? (a.rows + a.xrows - 1) / a.xrows : 0;
   if (a.num_kb < 1 || a.xrows < 16 || a.xrows > kLoraSmallTile || a.xrows % 16 || a.width < 16 || a.width > kCols ||
       (fused && (a.entries < 1 || a.entries > kLoraMaxGroup || row_tiles > kLoraSmallTiles)) ||
-      (!fused && a.entries > 0 && a.rows > kLoraBlock))
+      (!fused && a.entries > 0 && (!a.off || !a.list)))
     return cudaErrorInvalidValue;
   SmallShape sh{};
   const bool apart = fused && a.width == kCols;

@@ -173,6 +173,23 @@ def test_single_rows_each_with_an_adapter_of_its_own(type, n, inn, out):
     c.check()
 
 
+@BOTH
+@pytest.mark.parametrize("n,rows,ads,ranks,inn,out", [
+    (130, 1, 130, [16], 1024, 300), (256, 1, 256, [1, 20], 200, 520), (384, 1, 384, [16], 264, 1024), (700, 1, 90, [33, 5], 130, 257),
+    (513, 1, 513, [16], 72, 64), (40, 25, 16, [64, 9], 264, 520), (11, 100, 10, [128, 200], 136, 640), (90, 7, 45, [17, 3], 1000, 131),
+    (1100, 2, 300, [16], 64, 128), (37, 3, 20, [40], 512, 1024)])
+def test_more_adapters_than_a_launch_takes(type, n, rows, ads, ranks, inn, out):
+    """Row tiles with lists of their own, some segments without an adapter, and the GEMM behind them."""
+    slots = [i % ads if i % 11 != 5 else -1 for i in range(n)]
+    c = Case(type, [rows] * n, slots, [ranks[i % len(ranks)] for i in range(ads)], inn, out, bias=True, seed=n)
+    c.run()
+    c.check()
+    first = c.y().clone()
+    c.run()
+    c.check()
+    assert torch.equal(c.y(), first)
+
+
 def test_no_adapter_anywhere_and_no_rows():
     c = Case(ops.F16, [70, 0, 9], [-1, -1, -1], [], 512, 256)
     c.run()
