@@ -15,9 +15,9 @@
 // tokens and all their heads (up to 256 units of two 16-byte pieces times 4 heads),
 // so a sine and cosine is computed once for all heads and passed through shared
 // memory, and all of a thread's loads are issued before it needs an angle.
-// Measured: 65536 tokens x 40 heads x 128, bf16: 207 us, 6.5 TB/s, the rate of a
-// plain copy; 9872 x 32 x 64, f16: 15.2 us, 5.3 TB/s (4.2 tiles a block: ramp and
-// tail); 3001 x 15 x 80 with 20 rotated, f32: 7.0 us, 4.1 TB/s; 1 token: 1.7 us.
+// Measured: 65536 tokens x 40 heads x 128, bf16: 206 us, 6.5 TB/s, the rate of a
+// plain copy; 9872 x 32 x 64, f16: 15.0 us, 5.4 TB/s (4.2 tiles a block: ramp and
+// tail); 3001 x 15 x 80 with 20 rotated, f32: 6.9 us, 4.2 TB/s; 1 token: 1.7 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T, VEC, HALF, COPY>) rope_ke
   constexpr bool kWithin = !HALF && VEC > 1;       // a pair lies within a piece
   constexpr int kPairs = kWithin ? VEC / 2 : VEC;  // of a piece
   extern __shared__ __align__(16) float angles[];  // [2][cos | sin][block_tokens * half]
+  __shared__ uint64_t turns[kMaxPairs];
   const int half = a.rot / 2;
   const int turned_pieces = kWithin ? a.rot / VEC : 0;
   const int turned = kWithin ? (turned_pieces + 1) / 2 : half / VEC;  // units that turn
@@ -236,9 +237,14 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T, VEC, HALF, COPY>) rope_ke
   }
   const T* const x0 = static_cast<const T*>(t.x) + h0 * t.x_head + at;
   T* const o0 = static_cast<T*>(t.out) + h0 * t.out_head + at;
-  // the first of the angles it computes
+  // the first of the angles it computes, and the way to its next
+  const int step_at = kThreads / half, step_j = kThreads - step_at * half;
   const int my_at = static_cast<int>(threadIdx.x) / half, my_j = static_cast<int>(threadIdx.x) - my_at * half;
 
+  // lanes that read different parameters take turns; here they do so once a block
+  // (65536 tokens of one head of 128, where angles are half the work: 44 -> 30 us)
+  for (int j = threadIdx.x; j < half; j += kThreads) turns[j] = a.turns[j];
+  __syncthreads();
   grid_dep_wait();  // positions and inputs may come from the launch before
   grid_dep_trigger();
 
@@ -249,13 +255,15 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T, VEC, HALF, COPY>) rope_ke
       if (tok < a.tokens) {
         const long long pos = a.pos ? __ldg(a.pos + tok) : a.pos0 + tok;
         float c, s;
-        rope_angle(a.turns[j], pos, c, s);
+        rope_angle(turns[j], pos, c, s);
         buf[i] = c * a.mscale;
         buf[n_angles + i] = s * (a.mscale * a.sign);
       }
-      if (i + kThreads < n_angles) {
-        tok_at = (i + kThreads) / half;
-        j = i + kThreads - tok_at * half;
+      tok_at += step_at;
+      j += step_j;
+      if (j >= half) {
+        j -= half;
+        ++tok_at;
       }
     }
   };
@@ -342,6 +350,21 @@ cudaError_t launch_kernel(const RopeArgs& a, int num_sms, cudaStream_t st) {
   if (kResident == 2) blocks *= std::clamp<long long>(tiles / (8 * blocks), 1, 4);
   const dim3 grid(static_cast<unsigned>(std::min(tiles, blocks)), gy);
   const size_t smem = 4 * sizeof(float) * a.block_tokens * (a.rot / 2);
+  // Shared memory for the resident blocks' largest angles, the rest of the SM's
+  // 228 KB as L1 for the loads in flight: behind a GEMM that left nearly all of
+  // it to shared memory, 9872 x 32 x 64 took 18.3 us, so 15.0, and in turn with one 3.5 us less.
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    constexpr int kBytes = kResident * (4 * static_cast<int>(sizeof(float)) * kThreads * VEC + 3072), kSm = 228 * 1024;
+    e = cudaFuncSetAttribute(rope_kernel<T, VEC, HALF, COPY>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                             (100 * kBytes + kSm - 1) / kSm);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
   return launch_pdl(rope_kernel<T, VEC, HALF, COPY>, grid, dim3(kThreads), smem, st, nullptr, 0, a);
 }
 
