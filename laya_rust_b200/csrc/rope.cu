@@ -351,8 +351,9 @@ cudaError_t launch_kernel(const RopeArgs& a, int num_sms, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(std::min(tiles, blocks)), gy);
   const size_t smem = 4 * sizeof(float) * a.block_tokens * (a.rot / 2);
   // Shared memory for the resident blocks' largest angles, the rest of the SM's
-  // 228 KB as L1 for the loads in flight: behind a GEMM that left nearly all of
-  // it to shared memory, 9872 x 32 x 64 took 18.3 us, so 15.0, and in turn with one 3.5 us less.
+  // 228 KB as L1 for the loads in flight: all of it as shared memory, 9872 x 32 x
+  // 64 takes 18.0 us, so 15.0.  Without a preference the split stays as the kernel
+  // before left it (in turn with the adapter projection: 3.5 us more).
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
