@@ -98,10 +98,11 @@ int laya_rope(int device, const laya_rope_spec *spec, const laya_rope_tensor *te
  * for row m of a segment with adapter a, without the last term for a segment
  * that has none.  W [out, in], A_a [rank_a, in], B_a [out, rank_a]; x, W, A, B
  * and y of one 16-bit type (LAYA_F16 or LAYA_BF16), bias f32.  Sums are f32.
- * The rank-space vector scale x A^T is rounded once between the two products:
- * to f16, or to a pair of bf16 (value and remainder); y is rounded once.  With
- * LAYA_F16 the magnitude of scale x A^T must stay below 65504, as every f16
- * activation must.  A row's sums never meet another row's values; equal calls
+ * The rank-space vector scale x A^T passes between the two products as a pair of
+ * the 16-bit type (value and remainder), off by 2^-22 of it in f16 and 2^-16 in
+ * bf16; y is rounded once.  With LAYA_F16 the magnitude of scale x A^T must stay
+ * below 65504, as every f16 activation must, and values of it below 2^-3 are
+ * off by up to 2^-25.  A row's sums never meet another row's values; equal calls
  * give equal bits.
  *
  * A laya_lora holds the adapters of one projection; W and bias stay the
@@ -176,7 +177,9 @@ int laya_lora_layout(const int32_t *rows, const int32_t *slot, int n, const int3
  * in and out as the weight is stored, host arrays of `host_type`, rounded to f16
  * (values must be finite in f16).  laya_adapter_drop empties the slot.  These
  * wait for the engine's queued work and retire captured graphs, as a weight
- * upload does. */
+ * upload does.  A forward's scale x A^T has the range and the rounding that
+ * LAYA_F16 gives it in a laya_lora: an adapter that takes it to 65504 or beyond
+ * makes infinities of that sequence's activations. */
 int laya_adapters_create(laya_engine *e, int slots, int max_rank);
 int laya_adapter_create(laya_engine *e, int slot, int rank, float scale);
 int laya_adapter_upload(laya_engine *e, int slot, const char *name, const void *a, const void *b, int host_type);

@@ -8,10 +8,12 @@
 // reads the error word after each forward and turns it into an error status.
 #pragma once
 #include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
 #include <utility>
 
 namespace laya {
@@ -286,6 +288,25 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n) {
 // The same with A = B = BF16.
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int m, int n) {
   return umma_idesc_f16(m, n) | (1u << 7) | (1u << 10);
+}
+
+// Two f32 values as a packed pair of the 16-bit type T, and what that rounding
+// left as another (0 where a value is not finite: inf - inf would be NaN).
+template <class T>
+__device__ __forceinline__ void lora_split(float a, float b, uint32_t& hi, uint32_t& lo) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(isfinite(f.x) ? a - f.x : 0.0f, isfinite(f.y) ? b - f.y : 0.0f);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(isfinite(f.x) ? a - f.x : 0.0f, isfinite(f.y) ? b - f.y : 0.0f);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  }
 }
 
 // 2^x by the hardware's approximate exponential (one MUFU op).

@@ -1035,10 +1035,10 @@ struct Engine {
   void ensure_arena(const HostPlan& p) {
     ensure_rope(p.l);
     ensure_parts();
-    if (p.adapted && u.bytes < p.lora.chunk.size() * lora_entry_elems(false) * 2) {
+    if (p.adapted && u.bytes < p.lora.chunk.size() * kLoraEntryElems * 2) {
       wait_idle();
       ++arena_gen;
-      u.alloc(p.lora.chunk.size() * lora_entry_elems(false) * 2 * 2, "adapter workspace");
+      u.alloc(p.lora.chunk.size() * kLoraEntryElems * 2 * 2, "adapter workspace");
     }
     const int rows = (p.R + kGemmBM - 1) / kGemmBM * kGemmBM;
     const int mk = (p.n * p.k + kGemmBM - 1) / kGemmBM * kGemmBM;
@@ -1132,7 +1132,7 @@ struct Engine {
             make_tmap_2d(&q.o_hmlp, hmlp.as<__half>() + r0 * HEAD_INTER, false, rows, HEAD_INTER, 64, ob);
     }
     if (!bad && p.adapted)
-      bad = make_tmap_lora(&m.u, u.p, false, p.lora.chunk.size() * kLoraBlock, kGemmABoxRows) != 0;
+      bad = make_tmap_lora(&m.u, u.p, false, p.lora.chunk.size() * kLoraBlock * kLoraParts, kGemmABoxRows) != 0;
     if (bad) throw Error(LAYA_E_CUDA, "tensor map encode failed for the arena");
     m.gen = arena_gen;
   }
@@ -1452,7 +1452,7 @@ struct Engine {
   // writes the same rows, so one clear per forward is enough.
   void clear_u(const HostPlan& p) {
     if (p.adapted)
-      ck(cudaMemsetAsync(u.p, 0, p.lora.chunk.size() * lora_entry_elems(false) * 2, stream), "adapter workspace clear");
+      ck(cudaMemsetAsync(u.p, 0, p.lora.chunk.size() * kLoraEntryElems * 2, stream), "adapter workspace clear");
   }
 
   // Enqueues one forward of plan `dp` (graph.rs:86-186).

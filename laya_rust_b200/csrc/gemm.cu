@@ -32,9 +32,9 @@
 // With EXT (rows that have low-rank adapters), a tile's K loop goes on over the
 // adapters its row block needs: entry e multiplies 16 columns of rank-space
 // vectors u (zero in rows of other adapters) with 16 columns of that adapter's
-// B (operands of 32 bytes a row, laid out in memory as the MMA reads them).  A stage holds four entries,
-// or two of bf16, whose u is a value and a remainder: four K = 16 MMAs, as many
-// as a stage of the K loop.  So adapters cost a tile entries / 4 (bf16: / 2) more
+// B (operands of 32 bytes a row, laid out in memory as the MMA reads them).  A
+// stage holds two entries, whose u is a value and a remainder: four K = 16 MMAs,
+// as many as a stage of the K loop.  So adapters cost a tile entries / 2 more
 // k-blocks and no pass of their own over the output.
 // No TMA load in this kernel uses multicast; every CTA loads its own operand
 // halves.  The MMA completion signal is delivered to both CTAs of the pair
@@ -48,6 +48,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "lora.h"
 
 namespace laya {
 
@@ -74,9 +75,7 @@ constexpr size_t SMEM_LIMIT = 232448;
 // fill a stage's A operand
 constexpr int EXT_A_BYTES = CTA_ROWS * 32;
 static_assert(4 * EXT_A_BYTES == CTA_ROWS * BK * 2, "four operands to a stage");
-// 16-column operands of u an entry has
-template <int EPI>
-constexpr int kExtParts = EPI == kEpiPlainBf16 ? 2 : 1;
+constexpr int kExtPerStage = 4 / kLoraParts;  // entries
 
 template <int BN>
 struct Cfg {
@@ -637,7 +636,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
         if constexpr (EXT) {
-          // the adapters of the row block, two entries a stage
+          // the adapters of the row block, kPerStage entries a stage
           if (!ok || w.kb1 != num_kb) continue;
           const int mb = w.tile / num_n;
           const int e1 = __ldg(ext.off + mb + 1);
@@ -645,7 +644,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             grid_dep_wait();  // u is complete
             early = false;
           }
-          constexpr int kParts = kExtParts<EPI>, kPerStage = 4 / kParts;
+          constexpr int kParts = kLoraParts, kPerStage = kExtPerStage;
           int e = __ldg(ext.off + mb);
           int chunk[kPerStage];
 #pragma unroll
@@ -668,7 +667,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               uint8_t* sa = sA + stage * C::A_BYTES + i * kParts * EXT_A_BYTES;
               const int y = (e + i) * kParts * BM + static_cast<int>(rank) * CTA_ROWS;
               tma_load_2d_pair(sa, &ext.u, 0, y / 4, fb);
-              if (kParts == 2) tma_load_2d_pair(sa + EXT_A_BYTES, &ext.u, 0, (y + BM) / 4, fb);
+              tma_load_2d_pair(sa + EXT_A_BYTES, &ext.u, 0, (y + BM) / 4, fb);
               tma_load_2d_pair(sB + stage * C::B_BYTES + i * (BN / 2 * 32), tb, 0, (chunk[i] * ext.b_rows + n0) / 4, fb);
             }
 #pragma unroll
@@ -730,7 +729,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (kb1 == num_kb) {
             const int mb = w.tile / num_n;
             const int e1 = __ldg(ext.off + mb + 1);
-            constexpr int kParts = kExtParts<EPI>, kPerStage = 4 / kParts;
+            constexpr int kParts = kLoraParts, kPerStage = kExtPerStage;
             for (int e = __ldg(ext.off + mb); e < e1; e += kPerStage) {
               if (!mbar_wait_bounded(&full[stage], phase, args.err, kErrGemmMmaWait, abort_flag, args.wait_limit_ns)) {
                 ok = false;
@@ -743,7 +742,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const uint64_t db = umma_desc_sw32(b_addr + i * (BN / 2 * 32));
                 const uint32_t sa = a_addr + i * kParts * EXT_A_BYTES;
                 umma2_f16(d_tmem, umma_desc_sw32(sa), db, idesc, 1u);
-                if (kParts == 2) umma2_f16(d_tmem, umma_desc_sw32(sa + EXT_A_BYTES), db, idesc, 1u);
+                umma2_f16(d_tmem, umma_desc_sw32(sa + EXT_A_BYTES), db, idesc, 1u);
               }
               umma2_commit_both(&empty[stage]);
               if (++stage == C::STAGES) {

@@ -106,7 +106,7 @@ struct GemmMaps {
 
 // Low-rank adapters of the rows (see lora.h): after its K loop, row block m of
 // every tile adds, for each entry e in [off[m], off[m + 1]), the product of
-// u's entry e (256 rows of 16 values, bf16: and 256 rows of 16 remainders) with
+// u's entry e (256 rows of 16 values and 256 rows of 16 remainders) with
 // the 16 columns of B's chunk chunk[e] (b_rows rows, ordered like the weight's).
 struct GemmExt {
   const CUtensorMap* u;  // make_tmap_lora, box rows kGemmABoxRows

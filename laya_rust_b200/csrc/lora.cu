@@ -40,37 +40,21 @@ struct Num<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 };
 
-// bf16: elements from a value in u to its remainder.
+// Elements from a value in u to its remainder.
 constexpr int kRemainder = kLoraBlock * kLoraChunk;
 
-// Two rank values as a packed pair, and in bf16 their packed remainders (0
-// where a value is not finite: inf - inf would be NaN).
-template <class T>
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    const float2 f = __bfloat1622float2(h);
-    const __nv_bfloat162 l = __floats2bfloat162_rn(isfinite(f.x) ? a - f.x : 0.0f, isfinite(f.y) ? b - f.y : 0.0f);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-  } else {
-    const __half2 h = __floats2half2_rn(a, b);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = 0;
-  }
-}
 template <class T>
 __device__ __forceinline__ T* u_entry(void* u, int entry) {
-  return static_cast<T*>(u) + static_cast<size_t>(entry) * lora_entry_elems(std::is_same<T, __nv_bfloat16>::value);
+  return static_cast<T*>(u) + static_cast<size_t>(entry) * kLoraEntryElems;
 }
 // Rank values j, j + 1 (j even) of a row of the batch into an entry.
 template <class T>
 __device__ __forceinline__ void store_u2(T* entry, int row, int j, float a, float b) {
   uint32_t hi, lo;
-  split_pair<T>(a, b, hi, lo);
+  lora_split<T>(a, b, hi, lo);
   T* d = entry + lora_at(row % kLoraBlock, j);
   *reinterpret_cast<uint32_t*>(d) = hi;
-  if (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<uint32_t*>(d + kRemainder) = lo;
+  *reinterpret_cast<uint32_t*>(d + kRemainder) = lo;
 }
 // All 16, as 16-byte stores.
 template <class T>
@@ -79,11 +63,10 @@ __device__ __forceinline__ void store_u16(T* entry, int row, const float (&v)[16
   for (int h = 0; h < 2; ++h) {
     uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) split_pair<T>(v[8 * h + 2 * j], v[8 * h + 2 * j + 1], hi[j], lo[j]);
+    for (int j = 0; j < 4; ++j) lora_split<T>(v[8 * h + 2 * j], v[8 * h + 2 * j + 1], hi[j], lo[j]);
     T* d = entry + lora_at(row % kLoraBlock, 8 * h);
     *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    if (std::is_same<T, __nv_bfloat16>::value)
-      *reinterpret_cast<uint4*>(d + kRemainder) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    *reinterpret_cast<uint4*>(d + kRemainder) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
 }
 
@@ -813,14 +796,14 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     std::copy(entry_chunk.begin(), entry_chunk.end(), h.begin() + o_ent);
     q.dev.alloc(h.size() * 4, "lora plan");
     const size_t entries = std::max<size_t>(1, L.chunk.size());
-    q.u.alloc(entries * lora_entry_elems(k.bf16) * 2, "lora workspace");
-    if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock * (k.bf16 ? 2 : 1),
+    q.u.alloc(entries * kLoraEntryElems * 2, "lora workspace");
+    if (make_tmap_lora(&q.u_map, q.u.p, k.bf16, entries * kLoraBlock * kLoraParts,
                        q.small.use ? q.small.xrows : kGemmABoxRows))
       throw OpError(LAYA_E_CUDA, "lora_plan_create: tensor map encode failed");
     op_check(cudaMemcpyAsync(q.dev.p, h.data(), h.size() * 4, cudaMemcpyHostToDevice, k.stream), "lora plan upload");
     // rows of other adapters are zero in an entry, and stay zero: every run
     // writes the same rows of each entry
-    op_check(cudaMemsetAsync(q.u.p, 0, entries * lora_entry_elems(k.bf16) * 2, k.stream), "lora workspace clear");
+    op_check(cudaMemsetAsync(q.u.p, 0, entries * kLoraEntryElems * 2, k.stream), "lora workspace clear");
     op_check(cudaStreamSynchronize(k.stream), "lora plan upload");
     q.d_err = q.dev.as<int>();
     q.d_off = q.dev.as<int>() + o_off;

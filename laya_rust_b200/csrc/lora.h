@@ -37,15 +37,15 @@ inline int lora_chunks(int rank) { return (rank + kLoraChunk - 1) / kLoraChunk; 
 // is one chunk of one adapter that some row of block b has; a slot's chunks
 // are consecutive entries, slots in order of first use.  row_entry[m]: the
 // first entry of row m's adapter, or -1.  u, the rank-space vectors scale *
-// (x A^T), is [entries][256 rows][16 values], in bf16 [entries][values,
-// remainders][256 rows][16], halves placed by lora_at, zero for rows of other
-// adapters.
+// (x A^T), is [entries][values, remainders][256 rows][16], halves placed by
+// lora_at, zero for rows of other adapters.
 //
-// u passes between the two products in the 16-bit type.  In f16 one value: half a
-// step is 2^-11 of it, so what it adds to y's error is at most 2^-11 of the
-// adapter's part of y (the errors of its rank values average out), beside the
-// 2^-11 of all of y that rounding y costs.  In bf16 half a step is 2^-8, and a
-// second bf16 with the remainder leaves 2^-16.
+// u passes between the two products as two values of the 16-bit type, a value
+// and what rounding it left: 2^-22 of u is lost in f16 and 2^-16 in bf16, far
+// inside the rounding of y.  One f16 alone would lose 2^-11 of the adapter's part
+// beside the 2^-11 of y's own rounding.  An f16 ends at 2^-24, so of values below
+// 2^-3 up to 2^-25 is lost, which f16's range costs y too; and u must stay below
+// 65504, f16's largest.
 struct LoraLayout {
   int rows = 0;
   std::vector<int> off;
@@ -64,8 +64,9 @@ std::vector<uint16_t> lora_pack_a(const void* a, int type, int rank, int in, int
 std::vector<uint16_t> lora_pack_b(const void* b, int type, int rank, int out, int out_pad, bool bf16,
                                   const std::vector<int>& row_of);
 
-// Elements of an entry of u.
-constexpr size_t lora_entry_elems(bool bf16) { return static_cast<size_t>(kLoraBlock) * kLoraChunk * (bf16 ? 2 : 1); }
+// 16-column operands of u that an entry has, and its elements.
+constexpr int kLoraParts = 2;
+constexpr size_t kLoraEntryElems = static_cast<size_t>(kLoraBlock) * kLoraChunk * kLoraParts;
 
 // The work of the rank-space product: item i computes entries
 // entry[item.y .. item.y + item.z) for rows [128 item.x, 128 item.x + 128).

@@ -114,17 +114,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// (a, b) as packed values and, for bf16, packed remainders (0 where a value is
-// not finite).
-template <class T>
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack2<T>(a, b);
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const float x = __uint_as_float(hi << 16), y = __uint_as_float(hi & 0xffff0000u);
-    lo = pack2<T>(isfinite(x) ? a - x : 0.0f, isfinite(y) ? b - y : 0.0f);
-  }
-}
-
 template <class T, int SPLITS, bool FUSED>
 __global__ void __launch_bounds__(kThreads)
     lora_small_kernel(const __grid_constant__ SmallMaps maps, const __grid_constant__ LoraSmallArgs a, const SmallShape sh) {
@@ -150,8 +139,8 @@ __global__ void __launch_bounds__(kThreads)
   const int* const chunk = a.chunk[FUSED ? blockIdx.y : 0];
   const int entries = FUSED ? a.tile_entries[blockIdx.y] : 0;
   const int rows = min(xrows, a.rows - m0);
-  constexpr int kParts = std::is_same<T, __nv_bfloat16>::value ? 2 : 1;  // operands of u an entry has
-  constexpr int kPerStage = 4 / kParts;                                    // entries a stage
+  constexpr int kParts = kLoraParts;      // operands of u an entry has
+  constexpr int kPerStage = 4 / kParts;   // entries a stage
   const int x_bytes = xrows * 128, u_bytes = xrows * 32;
   // a stage: [W | A, joint] [x] [A, apart], room for the fullest tile's entries
   const int stage_bytes = kWBytes + x_bytes + (FUSED && !joint ? a.entries * kABytes : 0);
@@ -173,6 +162,9 @@ __global__ void __launch_bounds__(kThreads)
   // which this CTA may still be using when another one's sums arrive.  One CTA
   // alone: [owned B operands] [ring], and over the idle ring first [rank-space
   // part] [u operands], then [part].
+  // Every operand of the ring starts on the 1024 bytes of its swizzle's period: an
+  // owned B operand is 4096 bytes and a pair of u's is xrows * 64, xrows and width
+  // are multiples of 16.
   const int u_entry = xrows * kPartULd;
   const int own_rows = xrows / SPLITS;                            // rows rank * own_rows ..
   uint8_t* own_b = smem;
@@ -282,7 +274,7 @@ __global__ void __launch_bounds__(kThreads)
             uint8_t* su = ring + st * stage_bytes + kWBytes + i * kParts * u_bytes;
             const int y = ent[i] * kParts * kLoraBlock + m0 % kLoraBlock;
             tma_load_2d(su, &maps.u, 0, y / 4, &full[st]);
-            if (kParts == 2) tma_load_2d(su + u_bytes, &maps.u, 0, (y + kLoraBlock) / 4, &full[st]);
+            tma_load_2d(su + u_bytes, &maps.u, 0, (y + kLoraBlock) / 4, &full[st]);
           }
         };
         int ahead = e0, st = stage;
@@ -363,7 +355,7 @@ __global__ void __launch_bounds__(kThreads)
             const uint64_t db = umma_desc_sw32(b_addr + i * kBBytes);
             const uint32_t su = b_addr + kWBytes + i * kParts * u_bytes;
             umma_f16(tmem, db, umma_desc_sw32(su), idesc, 1u);
-            if (kParts == 2) umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
+            umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
           }
           next();
         }
@@ -408,11 +400,11 @@ __global__ void __launch_bounds__(kThreads)
           if (mine) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              split2<T>(__uint_as_float(v[8 * h + 2 * j]) * scale, __uint_as_float(v[8 * h + 2 * j + 1]) * scale, hi[j], lo[j]);
+              lora_split<T>(__uint_as_float(v[8 * h + 2 * j]) * scale, __uint_as_float(v[8 * h + 2 * j + 1]) * scale, hi[j], lo[j]);
           }
           const int at = 2 * lora_at(m, 8 * h);
           *reinterpret_cast<uint4*>(op + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if (kParts == 2) *reinterpret_cast<uint4*>(op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
       }
     }
@@ -456,11 +448,11 @@ __global__ void __launch_bounds__(kThreads)
                             part_u_in + (e - e0) * u_entry + m * kPartULd + 8 * h, (e1 - e0) * u_entry, rank, v);
           const float scale = row_scale[m];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) split2<T>(v[2 * j] * scale, v[2 * j + 1] * scale, hi[j], lo[j]);
+          for (int j = 0; j < 4; ++j) lora_split<T>(v[2 * j] * scale, v[2 * j + 1] * scale, hi[j], lo[j]);
         }
         const int at = 2 * lora_at(m, 8 * h);
         *reinterpret_cast<uint4*>(hi_op + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (kParts == 2) *reinterpret_cast<uint4*>(hi_op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint4*>(hi_op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
     tc_fence_before();
@@ -474,7 +466,7 @@ __global__ void __launch_bounds__(kThreads)
             const uint64_t db = umma_desc_sw32(smem_u32(own_b + i * kBBytes));
             const uint32_t su = smem_u32(own_u + i * kParts * u_bytes);
             umma_f16(tmem, db, umma_desc_sw32(su), idesc, 1u);
-            if (kParts == 2) umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
+            umma_f16(tmem, db, umma_desc_sw32(su + u_bytes), idesc, 1u);
           }
         }
         umma_commit(&done2);
@@ -664,10 +656,10 @@ cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const 
   while (splits < 8 && 2 * splits <= a.num_kb &&
          2 * splits * tiles <= (a.xrows <= 16 ? 2 : 1) * lora_cluster_room(2 * splits, num_sms))
     splits *= 2;
-  const int parts_of_u = a.bf16 ? 2 : 1, per_stage = 4 / parts_of_u;
+  constexpr int per_stage = 4 / kLoraParts;
   const int stage_bytes = kWBytes + a.xrows * 128 + (apart ? a.entries * kABytes : 0);
   const size_t rank_part = fused ? sizeof(float) * a.xrows * kPartULd : 0;   // of one entry
-  const size_t u_ops = static_cast<size_t>(parts_of_u) * a.xrows * 32;       // of one entry
+  const size_t u_ops = static_cast<size_t>(kLoraParts) * a.xrows * 32;       // of one entry
   // A CTA waits for its cluster, so no CTA may be left waiting for TMEM that a
   // waiting one holds: shared memory in proportion to the TMEM columns (456 of
   // an SM's 233472 bytes a column, of its 512) keeps the columns of the CTAs
