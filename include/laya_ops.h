@@ -151,6 +151,14 @@ int laya_lora_run(laya_lora *lora, laya_lora_plan *plan, const void *x, int64_t 
 /* Waits for the device and reports a bounded wait that expired in a run of
  * this plan (LAYA_E_DEVICE_TIMEOUT; its y is then undefined). */
 int laya_lora_status(laya_lora_plan *plan);
+/* Test of the bounded waits, as laya_test_timeout_next: in the plan's next run the
+ * loads of the launch that computes scale x A^T (kind 0; LAYA_E_INVALID where the
+ * plan has none that loads through a barrier), those of the projection (kind
+ * 1), or the exchange between the thread blocks of a cluster (kind 2; nothing where
+ * none work together) wait for something that never comes, for limit_ns (at most 2
+ * s).  That run's y is undefined, laya_lora_status reports it, and the plan stays
+ * usable. */
+int laya_lora_test_timeout_next(laya_lora_plan *plan, int kind, uint64_t limit_ns);
 void laya_lora_plan_destroy(laya_lora_plan *plan);
 /* The host side of a plan with no device (tests and diagnostics): for each
  * block of 256 rows the adapters it needs, in order of first use.  ranks[s]: the

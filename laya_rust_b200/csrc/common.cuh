@@ -127,6 +127,13 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// After a wait that expired: time for copies in flight to land before the CTA
+// goes on to leave.
+__device__ __forceinline__ void wait_for_copies() {
+  const unsigned long long t0 = global_ns();
+  while (global_ns() - t0 < 2000000ull) __nanosleep(1000);
+}
+
 // ---- TMA ----------------------------------------------------------------
 // Orders this thread's generic-proxy shared-memory writes before later
 // async-proxy reads (TMA stores, tcgen05.mma operands).

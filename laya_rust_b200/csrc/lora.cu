@@ -17,6 +17,7 @@
 #include <cstring>
 #include <memory>
 #include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(128, 1)
     lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
                        const LoraShrinkArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, in_full;
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, in_full, stuck_bar;
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_word;
   __shared__ int row_slot[kLoraItemRows];
@@ -137,9 +138,11 @@ __global__ void __launch_bounds__(128, 1)
     }
     mbar_init(&done, 1);
     mbar_init(&in_full, 1);
+    mbar_init(&stuck_bar, 1);
     abort_word = 0;
     fence_mbar_init();
-    if (SPLITS > 1) mbar_arrive_expect_tx(&in_full, (SPLITS - 1) * own_rows * ld * 4);
+    if (SPLITS > 1)
+      mbar_arrive_expect_tx(&in_full, (SPLITS - 1) * own_rows * ld * 4 + (a.stuck == kLoraStuckExchange ? 16 : 0));
     tma_prefetch_desc(&tmX);
     tma_prefetch_desc(&tmA);
   }
@@ -167,7 +170,9 @@ __global__ void __launch_bounds__(128, 1)
       bool ok = true;
       int stage = 0;
       uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      if (a.stuck == kLoraStuckLoads)
+        ok = mbar_wait_bounded(&stuck_bar, 0, a.err, kErrLoraWait, abort_flag, a.wait_limit_ns);
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
         ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag);
         if (!ok) break;
         uint8_t* sx = smem + stage * stage_bytes;
@@ -181,11 +186,7 @@ __global__ void __launch_bounds__(128, 1)
           phase ^= 1u;
         }
       }
-      if (!ok || *abort_flag) {
-        // loads in flight land before the CTA leaves
-        const unsigned long long t0 = global_ns();
-        while (global_ns() - t0 < 2000000ull) __nanosleep(1000);
-      }
+      if (!ok || *abort_flag) wait_for_copies();
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -262,7 +263,10 @@ __global__ void __launch_bounds__(128, 1)
     if (to < SPLITS && to != rank)
       bulk_to_rank(part_in + (rank < to ? rank : rank - 1) * own_rows * ld, &in_full, part + to * own_rows * ld,
                    own_rows * ld * 4, to);
-    if (!mbar_wait_bounded(&in_full, 0, a.err, kErrLoraWait, nullptr)) ok = false;
+    if (!mbar_wait_bounded(&in_full, 0, a.err, kErrLoraWait, nullptr, a.wait_limit_ns)) {
+      ok = false;
+      wait_for_copies();
+    }
     __syncwarp();
     cluster_arrive();  // what this CTA was sent has landed
     // SPLITS threads a row, each every SPLITS-th entry
@@ -594,6 +598,8 @@ struct Plan {
   LoraLayout lay;
   std::vector<std::pair<int, int>> used;  // (slot, chunks)
   Buf dev, u;
+  int stuck_kind = -1;  // laya_lora_test_timeout_next
+  unsigned long long stuck_limit_ns = 0;
   LoraSmallPlan small;  // use: lora_small.cu, not the GEMM
   int items = 0, group = 0;
   const int4* d_item = nullptr;
@@ -627,6 +633,8 @@ struct Plan {
 // but 64 segments of 16 rows, 64 adapters of rank 64, 2624 -> 1024 (4096 pairs of 256
 // chunks): 63 and 58 us.
 bool lora_by_pairs(size_t pairs, size_t entries) { return pairs <= 1024 || pairs <= 8 * entries; }
+
+constexpr uint64_t kMaxStuckNs = 2000000000;  // laya_lora_test_timeout_next
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -823,7 +831,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
                   void* stream) {
   return op_guard([&] {
     op_require(lora && plan, "lora_run: null argument");
-    const Plan& q = plan->p;
+    Plan& q = plan->p;
     const Bank& k = *q.bank;
     op_require(lora->bank == q.bank, "lora_run: the plan belongs to another projection");
     if (q.lay.rows == 0) return;
@@ -841,6 +849,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     require_device_ptr(x, k.device, "lora_run: x");
     require_device_ptr(y, k.device, "lora_run: y");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int stuck = std::exchange(q.stuck_kind, -1);
     const uint32_t xbox = q.small.use ? q.small.xrows : kGemmABoxRows;
     CUtensorMap mx, mw, my;
     if (make_tmap_pitched(&mx, x, k.bf16, q.lay.rows, k.in, ldx, xbox))
@@ -877,6 +886,8 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       s.chunks_per_slot = k.cps;
       s.bf16 = k.bf16;
       s.err = q.d_err;
+      s.stuck = stuck == 0 ? kLoraStuckLoads : stuck == 2 ? kLoraStuckExchange : kLoraStuckNone;
+      s.wait_limit_ns = s.stuck ? q.stuck_limit_ns : 0;
       op_check(launch_lora_shrink(mxi, k.a_map, s, k.num_sms, st), "lora launch");
     }
     // x W^T and u B^T in one accumulator
@@ -909,6 +920,8 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       g.bf16 = k.bf16;
       g.early = early;
       g.err = q.d_err;
+      g.stuck = stuck == 1 ? kLoraStuckLoads : stuck == 2 ? kLoraStuckExchange : kLoraStuckNone;
+      g.wait_limit_ns = g.stuck ? q.stuck_limit_ns : 0;
       op_check(launch_lora_small(mx, mw, q.u_map, mb, k.a_map, g, q.small.fused, k.num_sms, st), "lora launch");
       return;
     }
@@ -932,6 +945,8 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     g.ldo = static_cast<int>(ldy);
     g.bias = k.bias;
     g.n_valid = k.out;
+    g.stuck = stuck == 1;
+    g.wait_limit_ns = g.stuck ? q.stuck_limit_ns : 0;
     const GemmExt ext{&q.u_map, &k.b_map[narrow], &mw_half, &k.b_map[1], q.d_off, q.d_entry_chunk, k.out_pad, early};
     op_check(launch_gemm(k.bf16 ? kEpiPlainBf16 : kEpiPlainF16, GemmMaps{&mx, &mw, &my}, g, k.num_sms, st, bn, &ext),
              "lora launch");
@@ -951,6 +966,18 @@ int laya_lora_status(laya_lora_plan* plan) {
       op_check(cudaDeviceSynchronize(), "lora_status");
       throw OpError(LAYA_E_DEVICE_TIMEOUT, "lora_run: a device-side wait expired (code " + std::to_string(err) + ")");
     }
+  });
+}
+
+int laya_lora_test_timeout_next(laya_lora_plan* plan, int kind, uint64_t limit_ns) {
+  return op_guard([&] {
+    op_require(plan, "lora_test_timeout_next: null argument");
+    Plan& q = plan->p;
+    op_require(kind >= 0 && kind <= 2 && limit_ns > 0 && limit_ns <= kMaxStuckNs,
+               "lora_test_timeout_next: kind must be 0..2 and 0 < limit_ns <= 2e9");
+    op_require(kind != 0 || q.items > 0, "lora_test_timeout_next: the plan has no launch of that kind");
+    q.stuck_kind = kind;
+    q.stuck_limit_ns = limit_ns;
   });
 }
 

@@ -89,6 +89,11 @@ inline int lora_cluster_room(int cluster, int num_sms) {
 // one 128-row item a block leaves SMs for.
 int lora_splits(int rows, int num_sms);
 
+// Timeout test: the launch's loads first wait on a barrier that nothing completes,
+// or its exchange in the cluster expects bytes that nobody sends, for
+// wait_limit_ns.
+enum LoraStuck : int { kLoraStuckNone = 0, kLoraStuckLoads = 1, kLoraStuckExchange = 2 };
+
 struct LoraShrinkArgs {
   const int4* item;
   const int* item_entry;
@@ -102,6 +107,8 @@ struct LoraShrinkArgs {
   int chunks_per_slot;
   bool bf16;
   int* err;
+  int stuck;  // see LoraStuck
+  unsigned long long wait_limit_ns;
 };
 // u entries of every row with an adapter.
 // x: box 64 x 128, A (make_tmap_pitched, [chunks * 16, in_pad]): box 64 x 16.
@@ -165,6 +172,8 @@ struct LoraSmallArgs {
   bool bf16;
   int early;              // see GemmExt; not with fused
   int* err;
+  int stuck;              // see LoraStuck
+  unsigned long long wait_limit_ns;
 };
 cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& u, const CUtensorMap& b,
                               const CUtensorMap& a_map, const LoraSmallArgs& a, bool fused, int num_sms, cudaStream_t s);

@@ -118,7 +118,7 @@ template <class T, int SPLITS, bool FUSED>
 __global__ void __launch_bounds__(kThreads)
     lora_small_kernel(const __grid_constant__ SmallMaps maps, const __grid_constant__ LoraSmallArgs a, const SmallShape sh) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, b_full, done2, in_full, in_u_full;
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done, b_full, done2, in_full, in_u_full, stuck_bar;
   __shared__ int row_slot[kMaxRows];
   __shared__ float row_scale[kMaxRows];
   __shared__ uint32_t tmem_holder;
@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(kThreads)
     mbar_init(&done2, 1);
     mbar_init(&in_full, 1);
     mbar_init(&in_u_full, 1);
+    mbar_init(&stuck_bar, 1);
     tma_prefetch_desc(&maps.w);
     tma_prefetch_desc(&maps.x);
     if (FUSED) tma_prefetch_desc(&maps.a);
@@ -193,8 +194,9 @@ __global__ void __launch_bounds__(kThreads)
     abort_word = 0;
     fence_mbar_init();
     if (SPLITS > 1) {
-      mbar_arrive_expect_tx(&in_full, (SPLITS - 1) * own_rows * kPartLd * 4);
-      if (FUSED && e0 < e1) mbar_arrive_expect_tx(&in_u_full, (SPLITS - 1) * (e1 - e0) * u_entry * 4);
+      const int extra = a.stuck == kLoraStuckExchange ? 16 : 0;
+      mbar_arrive_expect_tx(&in_full, (SPLITS - 1) * own_rows * kPartLd * 4 + extra);
+      if (FUSED && e0 < e1) mbar_arrive_expect_tx(&in_u_full, (SPLITS - 1) * (e1 - e0) * u_entry * 4 + extra);
     }
   }
   if (warp == 1) {
@@ -224,7 +226,9 @@ __global__ void __launch_bounds__(kThreads)
           phase ^= 1u;
         }
       };
-      for (int kb = kb0; kb < kb1; ++kb) {
+      if (a.stuck == kLoraStuckLoads)
+        ok = mbar_wait_bounded(&stuck_bar, 0, a.err, kErrLoraWait, abort_flag, a.wait_limit_ns);
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
         ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, a.err, kErrLoraWait, abort_flag);
         if (!ok) break;
         uint8_t* sw = ring + stage * stage_bytes;
@@ -301,11 +305,7 @@ __global__ void __launch_bounds__(kThreads)
           next();
         }
       }
-      if (!ok || *abort_flag) {
-        // loads in flight land before the CTA leaves
-        const unsigned long long t0 = global_ns();
-        while (global_ns() - t0 < 2000000ull) __nanosleep(1000);
-      }
+      if (!ok || *abort_flag) wait_for_copies();
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -433,7 +433,10 @@ __global__ void __launch_bounds__(kThreads)
           bulk_to_rank(part_u_in + (rank < to ? rank : rank - 1) * (f1 - f0) * u_entry, &in_u_full, part_u + f0 * u_entry,
                        (f1 - f0) * u_entry * 4, to);
       }
-      if (e0 < e1 && !mbar_wait_bounded(&in_u_full, 0, a.err, kErrLoraWait, nullptr)) ok = false;
+      if (e0 < e1 && !mbar_wait_bounded(&in_u_full, 0, a.err, kErrLoraWait, nullptr, a.wait_limit_ns)) {
+        ok = false;
+        wait_for_copies();
+      }
     }
     for (int e = e0; e < e1 && !by_row; ++e) {
       const int slot = chunk[e] / a.chunks_per_slot;
@@ -457,7 +460,9 @@ __global__ void __launch_bounds__(kThreads)
     }
     tc_fence_before();
     fence_proxy_async_smem();
-    __syncthreads();
+    // each thread waited for the rank-space sums by itself: where one of them gave
+    // up, all skip the adapter step (elect_one needs its whole warp)
+    ok = __syncthreads_and(ok);
     if (e0 < e1 && ok) {
       if (warp == 1 && elect_one()) {
         if (mbar_wait_bounded(&b_full, 0, a.err, kErrLoraWait, abort_flag)) {
@@ -493,7 +498,10 @@ __global__ void __launch_bounds__(kThreads)
     if (to < SPLITS && to != rank)
       bulk_to_rank(part_in + (rank < to ? rank : rank - 1) * own_rows * kPartLd, &in_full, part + to * own_rows * kPartLd,
                    own_rows * kPartLd * 4, to);
-    if (!mbar_wait_bounded(&in_full, 0, a.err, kErrLoraWait, nullptr)) ok = false;
+    if (!mbar_wait_bounded(&in_full, 0, a.err, kErrLoraWait, nullptr, a.wait_limit_ns)) {
+      ok = false;
+      wait_for_copies();
+    }
     __syncwarp();
     cluster_arrive();  // what this CTA was sent has landed
   }

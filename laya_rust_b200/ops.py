@@ -62,6 +62,7 @@ def lib():
         L.laya_lora_plan_create.argtypes = [vp, i32p, i32p, ci, ctypes.POINTER(vp)]
         L.laya_lora_run.argtypes = [vp, vp, vp, i64, vp, i64, vp]
         L.laya_lora_status.argtypes = [vp]
+        L.laya_lora_test_timeout_next.argtypes = [vp, ci, ctypes.c_uint64]
         L.laya_lora_plan_destroy.argtypes = [vp]
         L.laya_lora_plan_destroy.restype = None
         L.laya_lora_layout.argtypes = [i32p, i32p, ci, i32p, ci, i64p, i64p, i32p, i64, i32p, i64]
@@ -169,6 +170,12 @@ class LoraPlan:
     def status(self) -> None:
         """Waits for the device; raises if a bounded wait expired in a run."""
         _check(lib().laya_lora_status(self._h))
+
+    def test_timeout_next(self, kind: int, limit_ns: int = 1_000_000) -> None:
+        """Arms the next run: the loads of the rank-space product's launch (0), of
+        the projection (1) or the exchange in a cluster (2) wait in vain for
+        limit_ns; status() then raises."""
+        _check(lib().laya_lora_test_timeout_next(self._h, kind, limit_ns))
 
     def close(self) -> None:
         if getattr(self, "_h", None):
