@@ -238,11 +238,13 @@ __global__ void __launch_bounds__(128, 1)
       uint32_t v[16];
       tmem_ld_32x32b_x16(tmem + lane_base + i * 16, v);
       tmem_ld_wait();
-      if (item_slot[i] != slot) continue;
-      float f[16];
+      if (item_slot[i] == slot) {
+        float f[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[j]) * scale;
-      store_u16<T>(u_entry<T>(a.u, item_entry[i]), item.x * kLoraItemRows + r, f);
+        for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[j]) * scale;
+        store_u16<T>(u_entry<T>(a.u, item_entry[i]), item.x * kLoraItemRows + r, f);
+      }
+      __syncwarp();  // the next load takes a whole warp
     }
     tc_fence_before();
     __syncthreads();
@@ -285,6 +287,7 @@ __global__ void __launch_bounds__(128, 1)
       for (int j = 0; j < 16; ++j) f[j] *= row_scale[r];
       store_u16<T>(u_entry<T>(a.u, item_entry[i]), item.x * kLoraItemRows + r, f);
     }
+    __syncwarp();
   }
   if (warp == 1) {
     tc_fence_after();

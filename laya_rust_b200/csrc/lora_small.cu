@@ -406,6 +406,7 @@ __global__ void __launch_bounds__(kThreads)
           *reinterpret_cast<uint4*>(op + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           *reinterpret_cast<uint4*>(op + u_bytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
+        __syncwarp();  // the next load takes a whole warp
       }
     }
     // lane = row of A, from the first rank-space lane on
@@ -420,6 +421,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
           for (int j = 0; j < 16; ++j) dst[(m + j) * kPartULd] = __uint_as_float(v[j]);
         }
+        __syncwarp();
       }
     }
     fence_proxy_async_smem();
