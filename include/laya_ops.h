@@ -66,6 +66,10 @@ typedef struct laya_rope_scaling {
 /* freqs[j] = base^(-2j / rot), j < rot / 2, stretched by `s` (NULL: none);
  * *mscale the factor on cos and sin.  Host only, no device needed. */
 int laya_rope_freqs(double base, int rot, const laya_rope_scaling *s, double *freqs, float *mscale);
+/* What laya_rope computes angles with (tests and diagnostics, host only): `freq`
+ * radians per position as a 64-bit fraction of a turn, so that position * *turns
+ * (mod 2^64) is the angle with whole turns dropped. */
+int laya_rope_turns(double freq, uint64_t *turns);
 
 typedef struct {
   int32_t type;        /* LAYA_F16, LAYA_BF16 or LAYA_F32 */
@@ -73,7 +77,8 @@ typedef struct {
   int32_t inverse;
   int32_t dim, rot;    /* head size (<= LAYA_ROPE_MAX_DIM) and its rotated part (even, 2..dim) */
   float mscale;
-  const double *freqs; /* host, [rot / 2], radians per position, at most 2^20; read during the call */
+  const double *freqs; /* host, [rot / 2], radians per position, of magnitude at most 2^20, negative ones
+                        * turn the other way; read during the call */
 } laya_rope_spec;
 
 /* A [tokens, heads, dim] view and where its rotation goes; strides in elements,

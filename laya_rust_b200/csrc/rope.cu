@@ -451,6 +451,9 @@ float rope_stretch(double* f, int rot, const laya_rope_scaling* s) {
 }
 
 uint64_t rope_turns(double f) {
+  // below, f >= 0: a negative frequency turns the other way, and the fraction of a
+  // negative product would not be exact
+  if (f < 0) return 0 - rope_turns(-f);
   // f / (2 pi) as the product with 1 / (2 pi) in two doubles: the leading
   // product, its exact error, and the constant's tail
   constexpr double kInvHi = 0.15915494309189535, kInvLo = -9.839338337591243e-18;
@@ -486,6 +489,14 @@ extern "C" int laya_rope_freqs(double base, int rot, const laya_rope_scaling* s,
     for (int j = 0; j < rot / 2; ++j) f[j] = std::pow(base, -2.0 * j / rot);
     *mscale = rope_stretch(f.data(), rot, s);
     std::copy(f.begin(), f.end(), freqs);
+  });
+}
+
+extern "C" int laya_rope_turns(double freq, uint64_t* turns) {
+  return op_guard([&] {
+    op_require(turns, "rope_turns: null argument");
+    op_require(std::fabs(freq) <= kMaxFreq, "rope_turns: a frequency is not finite, or above 2^20");
+    *turns = rope_turns(freq);
   });
 }
 

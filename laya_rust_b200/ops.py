@@ -50,6 +50,7 @@ def lib():
     if not _bound:
         vp, i64, sc = ctypes.c_void_p, ctypes.c_int64, ctypes.POINTER(_CRopeScaling)
         L.laya_rope_freqs.argtypes = [ctypes.c_double, ctypes.c_int, sc, _f64p, ctypes.POINTER(ctypes.c_float)]
+        L.laya_rope_turns.argtypes = [ctypes.c_double, ctypes.POINTER(ctypes.c_uint64)]
         L.laya_rope.argtypes = [ctypes.c_int, vp, ctypes.c_char_p, ctypes.c_int,
                                 i64, vp, i64, vp]
         L.laya_set_rope_scaling.argtypes = [vp, sc, sc]
@@ -95,6 +96,14 @@ def rope_freqs(base: float, rot: int, scaling: RopeScaling | None = None) -> tup
     _check(lib().laya_rope_freqs(base, rot, ctypes.byref(scaling._c()) if scaling else None,
                                  f.ctypes.data_as(_f64p), ctypes.byref(m)))
     return f, m.value
+
+
+def rope_turns(freq: float) -> int:
+    """laya_rope_turns: the 64-bit fraction of a turn per position that `freq`
+    radians are kept as."""
+    t = ctypes.c_uint64()
+    _check(lib().laya_rope_turns(freq, ctypes.byref(t)))
+    return t.value
 
 
 class RopeSpec:
