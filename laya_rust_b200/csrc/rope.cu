@@ -458,8 +458,11 @@ uint64_t rope_turns(double f) {
   // product, its exact error, and the constant's tail
   constexpr double kInvHi = 0.15915494309189535, kInvLo = -9.839338337591243e-18;
   const double hi = f * kInvHi, lo = std::fma(f, kInvHi, -hi) + f * kInvLo;
-  const double frac = hi - std::floor(hi);  // exact
-  return static_cast<uint64_t>(frac * 18446744073709551616.0) + static_cast<uint64_t>(static_cast<int64_t>(lo * 18446744073709551616.0));
+  constexpr double kUnits = 18446744073709551616.0;
+  const double frac = (hi - std::floor(hi)) * kUnits;  // exact
+  const double whole = std::floor(frac);
+  // one rounding, of what is not whole and the low parts together
+  return static_cast<uint64_t>(whole) + static_cast<uint64_t>(std::llrint((frac - whole) + lo * kUnits));
 }
 
 cudaError_t launch_rope_table(const double* freqs, int n, float mscale, int positions, float* cosb, float* sinb,

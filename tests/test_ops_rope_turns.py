@@ -34,3 +34,11 @@ def test_bad_frequencies_are_refused(f):
 
 def test_null_argument():
     assert ops.lib().laya_rope_turns(1.0, None) == E.LAYA_E_INVALID
+
+
+def test_the_fraction_is_rounded_once():
+    """Half a 2^-64 of a turn.  Beyond that the constant's two doubles leave 2^-107 of
+    it, at most 2^20 / (2 pi) turns * 2^64 * 2^-107 = 2^-26 units, and the low
+    parts, up to 2^27 units, their own rounding of 2^-26."""
+    worst = max((off(s * f, ops.rope_turns(s * float(f))), s * f) for f in frequencies() for s in (1, -1))
+    assert worst[0] <= 0.5 + 2.0 ** -24, worst
