@@ -624,7 +624,7 @@ struct Engine {
   enum Proj { kProjQkv, kProjWo, kProjWi, kProjWo2, kProjs };
   using Bank = AdapterBank;
   std::vector<Bank> banks;      // [layer * kProjs + projection]
-  int slots = 0, slot_chunks = 0;
+  int slots = 0, slot_chunks = 0, slot_max_rank = 0;
   std::vector<int> slot_rank;   // 0: empty
   DevBuf slot_scale, u;
 
@@ -677,6 +677,7 @@ struct Engine {
     }
     slots = n;
     slot_chunks = cps;
+    slot_max_rank = max_rank;
     slot_rank.assign(n, 0);
   }
 
@@ -686,7 +687,7 @@ struct Engine {
 
   void adapter_create(int slot, int rank, float scale) {
     require_slot(slot);
-    if (rank < 1 || lora_chunks(rank) > slot_chunks) throw Error(LAYA_E_INVALID, "adapter: rank must be 1..max_rank");
+    if (rank < 1 || rank > slot_max_rank) throw Error(LAYA_E_INVALID, "adapter: rank must be 1..max_rank");
     if (!std::isfinite(scale)) throw Error(LAYA_E_INVALID, "adapter: scale is not finite");
     adapter_drop(slot);
     upload_sync(slot_scale.as<float>() + slot, &scale, sizeof scale, "adapter scale");
