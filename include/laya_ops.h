@@ -19,6 +19,13 @@
  * device (NULL: the default stream); calls enqueue work and return without
  * waiting for it, and may be captured into a graph (make the first call of a kind
  * on a device before any capture: it loads and configures the kernels).
+ *
+ * Threads: laya_rope and the calls on one laya_lora and its plans may come from
+ * several threads at once.  A run has the whole of an adapter that another thread
+ * sets, or none of it.  What is left to the caller: a plan's runs are ordered on
+ * the device (see laya_lora_run), no captured graph of runs is replayed while
+ * laya_lora_set is in progress, and no call is in progress on a handle that is
+ * destroyed.  The calls on an engine follow the rule of laya_b200.h.
  */
 #ifndef LAYA_OPS_H
 #define LAYA_OPS_H

@@ -39,6 +39,7 @@
 // No TMA load in this kernel uses multicast; every CTA loads its own operand
 // halves.  The MMA completion signal is delivered to both CTAs of the pair
 // with tcgen05.commit's cluster-multicast form.
+#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 
@@ -822,7 +823,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 template <int EPI, int BN, bool EXT>
 cudaError_t launch_one(const GemmMaps& m, const GemmArgs& args, int num_sms, cudaStream_t stream,
                        const std::conditional_t<EXT, ExtParams, NoExt>& ext) {
-  static bool configured[64] = {};
+  static std::atomic<bool> configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -932,7 +933,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
+  static std::atomic<EncodeTiledFn> fn{nullptr};
   if (!fn) {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;

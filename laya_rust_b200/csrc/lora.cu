@@ -13,9 +13,11 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <memory>
+#include <mutex>
 #include <type_traits>
 #include <utility>
 
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(256) lora_pairs_kernel(const LoraPairsArgs a) 
 
 template <class T, int SPLITS>
 cudaError_t launch_shrink(const CUtensorMap& x, const CUtensorMap& a_map, const LoraShrinkArgs& a, cudaStream_t s) {
-  static bool configured[64] = {};
+  static std::atomic<bool> configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -573,6 +575,9 @@ struct Bank {
   const void* w = nullptr;
   long long ldw = 0;
   const float* bias = nullptr;
+  // Held while an adapter is replaced and while a run is checked and enqueued: a
+  // run that another thread enqueues comes before or after the whole of it.
+  mutable std::mutex lock;
   std::vector<Slot> slot;
   Buf a, b, scale;
   CUtensorMap a_map;
@@ -719,6 +724,7 @@ int laya_lora_set(laya_lora* lora, int slot, int rank, const void* a, const void
     op_require(std::isfinite(scale), "lora_set: scale is not finite");
     const std::vector<uint16_t> ha = lora_pack_a(a, host_type, rank, k.in, k.in_pad, k.bf16);
     const std::vector<uint16_t> hb = lora_pack_b(b, host_type, rank, k.out, k.out_pad, k.bf16, {});
+    const std::lock_guard<std::mutex> held(k.lock);
     DeviceScope scope(k.device);
     // runs already queued on the caller's streams may still read the slot
     op_check(cudaDeviceSynchronize(), "lora_set");
@@ -740,6 +746,7 @@ int laya_lora_clear(laya_lora* lora, int slot) {
   return op_guard([&] {
     op_require(lora, "lora_clear: null argument");
     op_require(slot >= 0 && slot < lora->bank->slots, "lora_clear: slot out of range");
+    const std::lock_guard<std::mutex> held(lora->bank->lock);
     lora->bank->slot[slot].rank = 0;
   });
 }
@@ -754,7 +761,11 @@ int laya_lora_plan_create(laya_lora* lora, const int32_t* rows, const int32_t* s
     Plan& q = p->p;
     q.bank = lora->bank;
     const Bank& k = *q.bank;
-    const std::vector<int> chunks = k.chunks_of();
+    std::vector<int> chunks;
+    {
+      const std::lock_guard<std::mutex> held(k.lock);
+      chunks = k.chunks_of();
+    }
     q.lay = lora_layout(rows, slot, n, chunks);
     const LoraLayout& L = q.lay;
     std::vector<int> entry_chunk;
@@ -845,6 +856,7 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
     op_require(aligned16(x) && aligned16(y) && ldx % 8 == 0 && ldy % 8 == 0,
                "lora_run: x, y and their pitches must be multiples of 16 bytes");
     op_require(x != y, "lora_run: x and y must be apart");
+    const std::lock_guard<std::mutex> held(k.lock);
     for (const auto& u : q.used)
       if (lora_chunks(k.slot[u.first].rank) != u.second)
         throw OpError(LAYA_E_STATE, "lora_run: an adapter of the plan was cleared or changed its rank; make a new plan");
@@ -978,6 +990,7 @@ int laya_lora_test_timeout_next(laya_lora_plan* plan, int kind, uint64_t limit_n
     Plan& q = plan->p;
     op_require(kind >= 0 && kind <= 2 && limit_ns > 0 && limit_ns <= kMaxStuckNs,
                "lora_test_timeout_next: kind must be 0..2 and 0 < limit_ns <= 2e9");
+    const std::lock_guard<std::mutex> held(q.bank->lock);
     op_require(kind != 0 || q.items > 0, "lora_test_timeout_next: the plan has no launch of that kind");
     q.stuck_kind = kind;
     q.stuck_limit_ns = limit_ns;

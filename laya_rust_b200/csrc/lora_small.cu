@@ -30,6 +30,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -546,7 +547,7 @@ __global__ void __launch_bounds__(kThreads)
 
 template <class T, int SPLITS, bool FUSED>
 cudaError_t launch(const SmallMaps& maps, const LoraSmallArgs& a, const SmallShape& sh, size_t smem, cudaStream_t s) {
-  static bool configured[64] = {};
+  static std::atomic<bool> configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;

@@ -19,6 +19,7 @@
 // plain copy; 9872 x 32 x 64, f16: 15.0 us, 5.4 TB/s (4.2 tiles a block: ramp and
 // tail); 3001 x 15 x 80 with 20 rotated, f32: 6.9 us, 4.2 TB/s; 1 token: 1.7 us.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 #include <vector>
@@ -354,7 +355,7 @@ cudaError_t launch_kernel(const RopeArgs& a, int num_sms, cudaStream_t st) {
   // 228 KB as L1 for the loads in flight: all of it as shared memory, 9872 x 32 x
   // 64 takes 18.0 us, so 15.0.  Without a preference the split stays as the kernel
   // before left it (in turn with the adapter projection: 3.5 us more).
-  static bool configured[64] = {};
+  static std::atomic<bool> configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
