@@ -98,9 +98,18 @@ def lib():
     return _lib
 
 
+def _int32(values, what: str) -> np.ndarray:
+    """Contiguous int32 copies of whole numbers; a number that int32 cannot hold, or a
+    fraction, is refused (a cast would make another slot or length of it)."""
+    a = np.asarray(values).ravel()
+    if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
+        raise ValueError(f"{what}: whole numbers of 32 bits are needed")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
 def _adapter_array(req: "Req", adapters) -> np.ndarray:
     """One int32 slot per sequence (-1: none)."""
-    a = np.ascontiguousarray(adapters, dtype=np.int32).ravel()
+    a = _int32(adapters, "adapters")
     if a.size != req.n:
         raise ValueError(f"{a.size} adapters for {req.n} sequences")
     return a

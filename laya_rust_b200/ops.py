@@ -14,7 +14,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from .engine import Engine, _check, lib as _engine_lib
+from .engine import Engine, _check, _int32, lib as _engine_lib
 
 F16, BF16, F32 = range(3)
 TYPE = {"f16": F16, "bf16": BF16, "f32": F32}
@@ -148,8 +148,7 @@ def set_rope_scaling(engine: Engine, full: RopeScaling | None = None, sliding: R
 
 # ---- a shared projection with low-rank adapters ------------------------------------
 def _segments(rows, slots):
-    r = np.ascontiguousarray(rows, dtype=np.int32).ravel()
-    s = np.ascontiguousarray(slots, dtype=np.int32).ravel()
+    r, s = _int32(rows, "rows"), _int32(slots, "slots")
     if r.size != s.size:
         raise ValueError(f"{r.size} segments but {s.size} slots")
     return r, s
@@ -242,7 +241,7 @@ def lora_layout(rows, slots, ranks) -> tuple[np.ndarray, np.ndarray]:
     """laya_lora_layout: (off [blocks + 1], chunks [entries, 2]) of the
     segments' host plan, with no device."""
     r, s = _segments(rows, slots)
-    k = np.ascontiguousarray(ranks, dtype=np.int32).ravel()
+    k = _int32(ranks, "ranks")
     nb, ne = ctypes.c_int64(), ctypes.c_int64()
     p = lambda a: a.ctypes.data_as(_i32p)
     L = lib()
