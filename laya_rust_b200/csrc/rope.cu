@@ -426,7 +426,8 @@ bool finite_positive(double v) { return std::isfinite(v) && v > 0; }
 
 float rope_stretch(double* f, int rot, const laya_rope_scaling* s) {
   if (!s) return 1.0f;
-  op_require(std::isfinite(s->attn) && s->attn >= 0, "rope scaling: attn must not be negative");
+  op_require(s->attn >= 0 && std::isfinite(static_cast<float>(s->attn)),
+             "rope scaling: attn must not be negative, and finite in 32 bits");
   if (s->kind == LAYA_ROPE_NONE) return s->attn != 0 ? static_cast<float>(s->attn) : 1.0f;
   op_require(s->kind == LAYA_ROPE_LINEAR || s->kind == LAYA_ROPE_BASE || s->kind == LAYA_ROPE_PARTS,
              "rope scaling: unknown kind");

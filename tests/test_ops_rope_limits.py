@@ -1,0 +1,18 @@
+"""Limits of the rotary operator's numbers, checked before a device is touched."""
+import numpy as np
+import pytest
+
+from laya_rust_b200 import engine as E
+from laya_rust_b200 import ops
+
+
+@pytest.mark.parametrize("kind", [ops.ROPE_NONE, ops.ROPE_LINEAR, ops.ROPE_BASE, ops.ROPE_PARTS])
+def test_a_factor_beyond_32_bits_is_refused(kind):
+    """attn becomes a 32-bit factor on cos and sin: an infinite one would fill the
+    engine's tables with infinities and NaN."""
+    for attn in (3.5e38, 1e300):
+        with pytest.raises(E.LayaError, match="attn") as ei:
+            ops.rope_freqs(10000.0, 64, ops.RopeScaling(kind, 2.0, 512.0, 1.0, 32.0, attn))
+        assert ei.value.code == E.LAYA_E_INVALID
+    _, m = ops.rope_freqs(10000.0, 64, ops.RopeScaling(kind, 2.0, 512.0, 1.0, 32.0, 3.4e38))
+    assert m == np.float32(3.4e38)
