@@ -101,7 +101,7 @@ typedef struct {
 
 /* Rotates `count` (1..4) tensors over the same tokens, e.g. q and k, in one
  * launch, 65535 heads in all.  pos: device int32 [tokens], any values, or NULL for
- * pos0, pos0 + 1, ...  (pos0 + tokens - 1 < 2^31).  tokens == 0 does nothing. */
+ * pos0, pos0 + 1, ...  (all of them 32-bit numbers).  tokens == 0 does nothing. */
 int laya_rope(int device, const laya_rope_spec *spec, const laya_rope_tensor *tensors, int count, int64_t tokens,
               const int32_t *pos, int64_t pos0, void *stream);
 

@@ -517,7 +517,7 @@ extern "C" int laya_rope(int device, const laya_rope_spec* spec, const laya_rope
     op_require(count >= 1 && count <= kMaxTensors, "rope: 1 to 4 tensors");
     constexpr int64_t kMaxPos = 2147483647;
     op_require(tokens >= 0 && tokens <= kMaxPos, "rope: tokens out of range");
-    op_require(pos || (pos0 >= -kMaxPos && pos0 + tokens <= kMaxPos + 1 && pos0 <= kMaxPos),
+    op_require(pos || (pos0 >= -kMaxPos - 1 && pos0 <= kMaxPos && pos0 + tokens <= kMaxPos + 1),
                "rope: positions must fit 32 bits");
     op_require(reinterpret_cast<uintptr_t>(pos) % 4 == 0, "rope: pos is not aligned");
     RopeArgs a{};
