@@ -1016,9 +1016,14 @@ struct Engine {
   void set_rope_scaling(const laya_rope_scaling* full, const laya_rope_scaling* sliding) {
     if (!finalized) throw Error(LAYA_E_STATE, "engine has no weights (call laya_finalize)");
     const laya_rope_scaling* in[2] = {full, sliding};
-    for (const laya_rope_scaling* s : in) {
-      std::vector<double> probe(HD / 2, 1.0);
-      rope_stretch(probe.data(), HD, s);  // refuses bad parameters before anything changes
+    for (int i = 0; i < 2; ++i) {
+      // refuses bad parameters, and frequencies the tables cannot be made from,
+      // before anything changes
+      const auto& f = W(i == 0 ? "rope.freq_full" : "rope.freq_sliding").host;
+      std::vector<double> probe(f.begin(), f.end());
+      rope_stretch(probe.data(), HD, in[i]);
+      if (in[i] && !std::all_of(probe.begin(), probe.end(), rope_freq_fits))
+        throw Error(LAYA_E_INVALID, "rope scaling: a frequency of the model is not finite, or above 2^20");
     }
     set_device();
     ck(cudaStreamSynchronize(stream), "sync");

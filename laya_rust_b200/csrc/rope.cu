@@ -452,6 +452,8 @@ float rope_stretch(double* f, int rot, const laya_rope_scaling* s) {
   return static_cast<float>(s->attn != 0 ? s->attn : m);
 }
 
+bool rope_freq_fits(double f) { return std::fabs(f) <= kMaxFreq; }
+
 uint64_t rope_turns(double f) {
   // below, f >= 0: a negative frequency turns the other way, and the fraction of a
   // negative product would not be exact
@@ -469,7 +471,7 @@ uint64_t rope_turns(double f) {
 
 cudaError_t launch_rope_table(const double* freqs, int n, float mscale, int positions, float* cosb, float* sinb,
                               cudaStream_t s) {
-  if (n < 1 || n > 32 || positions < 0) return cudaErrorInvalidValue;
+  if (n < 1 || n > 32 || positions < 0 || !std::all_of(freqs, freqs + n, rope_freq_fits)) return cudaErrorInvalidValue;
   if (positions == 0) return cudaSuccess;
   TableArgs a{};
   for (int j = 0; j < n; ++j) a.turns[j] = rope_turns(freqs[j]);
@@ -500,7 +502,7 @@ extern "C" int laya_rope_freqs(double base, int rot, const laya_rope_scaling* s,
 extern "C" int laya_rope_turns(double freq, uint64_t* turns) {
   return op_guard([&] {
     op_require(turns, "rope_turns: null argument");
-    op_require(std::fabs(freq) <= kMaxFreq, "rope_turns: a frequency is not finite, or above 2^20");
+    op_require(rope_freq_fits(freq), "rope_turns: a frequency is not finite, or above 2^20");
     *turns = rope_turns(freq);
   });
 }
@@ -557,7 +559,7 @@ extern "C" int laya_rope(int device, const laya_rope_spec* spec, const laya_rope
       r.heads = static_cast<int>(t.heads);
     }
     for (int j = 0; j < spec->rot / 2; ++j) {
-      op_require(std::fabs(spec->freqs[j]) <= kMaxFreq, "rope: a frequency is not finite, or above 2^20");
+      op_require(rope_freq_fits(spec->freqs[j]), "rope: a frequency is not finite, or above 2^20");
       a.turns[j] = rope_turns(spec->freqs[j]);
     }
     if (a.count == 0) return;

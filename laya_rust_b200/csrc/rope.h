@@ -14,6 +14,8 @@ float rope_stretch(double* freqs, int rot, const laya_rope_scaling* s);
 // f radians per position as a 64-bit fixed-point fraction of a turn per
 // position: position * result (mod 2^64) is the angle, whole turns dropped.
 uint64_t rope_turns(double f);
+// What it takes: finite, of magnitude at most 2^20.
+bool rope_freq_fits(double f);
 
 // cosb/sinb[p][j] = mscale cos/sin(p * freqs[j]) for p < positions, j < n
 // (n <= 32), the tables the Wqkv epilogue reads.
