@@ -117,7 +117,7 @@ struct GemmExt {
   const int* chunk;
   int b_rows;
   // The launch before this one computes u and nothing else this GEMM reads:
-  // only the adapter steps wait for it, and the K loop runs beside it.  Needs
+  // only the adapter steps wait for it; the K loop starts on SMs it leaves.  Needs
   // that launch to pass grid_dep_wait() before its grid_dep_trigger() (or to
   // be an ordinary launch), so that everything before it has completed.
   bool early;

@@ -4,11 +4,13 @@
 //   y[m] = x[m] W^T + bias + s_a (x[m] A_a^T) B_a^T
 //
 // Two launches.  The first computes u = s_a (x A_a^T) in rank space, in f32, and
-// rounds it to the 16-bit operand of the second product (lora.h says how).
-// The second computes x W^T + u B^T in one f32 accumulator and rounds once: the tcgen05 GEMM of gemm.cu, whose K loop goes on
-// over the adapters of its row block (GemmExt).  It is launched with programmatic
-// serialization and waits for u only before its adapter steps, so its K loop
-// runs beside the first launch.
+// rounds it to the 16-bit operands of the second product (lora.h says how).
+// The second computes x W^T + u B^T in one f32 accumulator and rounds once: the
+// tcgen05 GEMM of gemm.cu, whose K loop goes on over the adapters of its row block
+// (GemmExt).  It is launched with programmatic serialization and waits for u only
+// before its adapter steps.  A CTA of either fills an SM's shared memory, so its
+// K loop starts beside the first launch only on the SMs that one leaves idle, and
+// on the others as its CTAs end.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(128, 1)
 // u = scale (x A^T) for one (row, chunk) pair a block: a warp takes two of the
 // chunk's 16 rows of A over all of K, so no sum leaves its warp.  A is read once
 // a pair, 32 bytes an input and pair from HBM or L2 (48 rows with an adapter each,
-// 1024 inputs, with the projection behind it: 10.5 us, by items 14).
+// 1024 inputs, with the projection behind it: 10.5 us, by items 13.4).
 template <class T>
 __global__ void __launch_bounds__(256) lora_pairs_kernel(const LoraPairsArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -396,7 +398,7 @@ cudaError_t launch_lora_pairs(const LoraPairsArgs& a, cudaStream_t s) {
 }
 
 // As many parts as keep every item on an SM (3034 rows, 1024 -> 3072, 16 adapters:
-// 4 parts 24 us, 8 parts 34; 9872 rows: 1 part 59 us, 2 parts 71).
+// 4 parts 24.5 us, 8 parts 34; 10387 rows: 1 part 63 us, 2 parts 75).
 int lora_splits(int rows, int num_sms) {
   const int halves = (rows + kLoraItemRows - 1) / kLoraItemRows;
   int splits = 1;
@@ -420,9 +422,9 @@ LoraItems lora_items(const LoraLayout& L, int num_sms) {
       for (int e = e0; e < static_cast<int>(L.chunk.size()) && (e == e0 || L.chunk[e].y > 0); ++e) v.push_back(e);
     }
   }
-  // the smallest group whose items still run at once (9872 rows of 16 adapters,
-  // 1024 -> 3072, in all: groups of 1 entry 63 us, of 2 as chosen here 59; 3034
-  // rows: 1 or 2 28 us, 4 as chosen 24, 8 27)
+  // the smallest group whose items still run at once (10387 rows of 16 adapters,
+  // 1024 -> 3072, in all: groups of 1 entry 67 us, of 2 as chosen here 63; 3034
+  // rows: 1 or 2 28.6 us, 4 as chosen 24.6, 8 27.7)
   const size_t most = num_sms / lora_splits(L.rows, num_sms);
   for (it.group = 1;; it.group *= 2) {
     size_t items = 0;
@@ -636,10 +638,10 @@ struct Plan {
 
 // The rank-space product by (row, chunk) pairs, a block each that reads 16 rows of
 // A, or by items of 128 rows?  Pairs while they are few, or few of them share
-// an adapter's chunk: 256 rows with an adapter each, 1024 -> 3072: 23 us, by items
-// 39; 2048 of them 85 and 147 us; 128 segments of 8 rows, 16 adapters, 16 and 24 us;
-// but 64 segments of 16 rows, 64 adapters of rank 64, 2624 -> 1024 (4096 pairs of 256
-// chunks): 63 and 58 us.
+// an adapter's chunk: 256 rows with an adapter each, 1024 -> 3072: 22.5 us, by items
+// 38; 2048 rows in turn with 256 adapters 100 and 159 us; 128 segments of 8 rows, 16
+// adapters, 18 and 26 us; but 64 segments of 16 rows, 64 adapters of rank 64, 2624
+// -> 1024 (4096 pairs of 256 chunks): 53 and 41 us.
 bool lora_by_pairs(size_t pairs, size_t entries) { return pairs <= 1024 || pairs <= 8 * entries; }
 
 constexpr uint64_t kMaxStuckNs = 2000000000;  // laya_lora_test_timeout_next
@@ -941,8 +943,8 @@ int laya_lora_run(laya_lora* lora, laya_lora_plan* plan, const void* x, int64_t 
       return;
     }
     // 256 x 128 tiles where 256 x 256 ones would fill at most half the
-    // clusters, as in the engine (600 rows, 1024 -> 1024, 2 adapters: 9.9 us and,
-    // wide, 12.4; 1300 rows -> 3072: 16.3 and, wide, 15.4)
+    // clusters, as in the engine (600 rows, 1024 -> 1024, 2 adapters: 10.2 us and,
+    // wide, 11.8; 1300 rows -> 3072: 16.6 and, wide, 15.9)
     const int tiles = (q.lay.rows + kGemmBM - 1) / kGemmBM * (k.out_pad / kGemmBN);
     const bool narrow = tiles * 2 <= k.num_sms / 2;
     const int bn = narrow ? kGemmBNNarrow : kGemmBN;

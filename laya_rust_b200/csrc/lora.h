@@ -24,8 +24,8 @@ constexpr int kLoraBlock = 256;
 // swizzle of a K-major operand, which swaps a row's halves in every second
 // group of four rows.  Kept in memory, so that a tile is one contiguous copy:
 // the copy unit works by rows, and rows of 128 bytes are a fourth as many as rows
-// of 32 through a swizzling tensor map (16384 rows, 1024 -> 5248, ranks to 128:
-// 165.5 us, this way 161.7).
+// of 32 through a swizzling tensor map (16384 rows, 1024 -> 5248, ranks to 128, with
+// u as one operand an entry: 165.5 us, this way 161.7).
 #ifdef __CUDACC__
 __host__ __device__
 #endif

@@ -24,9 +24,9 @@
 //
 // With more entries u comes from the launch before, and a row tile goes through
 // the list of the entries some row of it has (256 rows with an adapter each, 1024
-// -> 3072: 19.5 us; through all of the block's 256 entries 46.9, by the GEMM
-// 36.5).  Measured otherwise: one row, 1024 -> 3072, rank 16: 5.6 us; 179 rows,
-// 2624 -> 1024, rank 32: 9.3 us; 48 rows with an adapter each: 10.5 us.
+// -> 3072: 22.5 us, by the GEMM 46; through all of the block's 256 entries it took
+// 2.4 times as long).  Measured otherwise: one row, 1024 -> 3072, rank 16: 5.8 us;
+// 179 rows, 2624 -> 1024, rank 32: 9.4 us; 48 rows with an adapter each: 10.5 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -592,7 +592,7 @@ LoraSmallPlan lora_small_plan(const LoraLayout& L, int out, int chunks_per_slot,
     const int tiles = (rows + xrows - 1) / xrows;
     if (tiles > kLoraSmallTiles || (xrows > even && rows <= even)) continue;
     // without adapters the GEMM has no launch before it, and beats tiles of 128
-    // (1357 rows, 1000 -> 1536: 9.3 and 10.3 us; with one adapter 14.2 and 12.6)
+    // (1357 rows, 1000 -> 1536: 9.3 and 10.3 us; with one adapter 14.2 and 11.5)
     if (!any && !one_block && xrows > even) continue;
     LoraSmallPlan p;
     p.use = true;
@@ -633,15 +633,15 @@ LoraSmallPlan lora_small_plan(const LoraLayout& L, int out, int chunks_per_slot,
       p.off.push_back(static_cast<int>(p.list.size()));
     }
     // joint pays where the K loop carries many rows (256 rows, 1024 -> 3072, one
-    // entry: 9.9 us, apart 12.0 us); with few, more tiles cost more than a second
-    // operand (1 row: joint 5.7 us, apart 5.4 us)
+    // entry: 8.8 us, apart 10.2 us); with few, more tiles cost what a second
+    // operand does (1 row: 5.1 us either way)
     for (int width : {kCols - most * kLoraChunk, kCols}) {
       if (width < kCols && !(p.fused && most <= 4 && rows > 32)) continue;
       p.width = width;
       // every CTA on an SM of its own; failing that, within one block of rows,
       // the smaller tiles in rounds (beyond it the GEMM is faster: 1000 rows of 100
-      // adapters, 1024 -> 3072, 27 us and, in two rounds, 51; in one round: 768 rows
-      // with an adapter each, 2624 -> 1024, 56 us by the GEMM, 34 here)
+      // adapters, 1024 -> 3072, 21 us and, in two rounds, 26; in one round: 768 rows
+      // with an adapter each, 2624 -> 1024, 66 us by the GEMM, 36 here)
       if ((out + width - 1) / width * tiles <= num_sms) return p;
       if (one_block && !best.use) best = p;
     }
@@ -660,9 +660,9 @@ cudaError_t launch_lora_small(const CUtensorMap& x, const CUtensorMap& w, const 
   SmallShape sh{};
   const bool apart = fused && a.width == kCols;
   const int tiles = (a.out + a.width - 1) / a.width * row_tiles;
-  // K parts: as many as still run at once (measured at 64 rows, 1024 -> 3072: 4
-  // parts, 96 CTAs, 5.7 us; 8 parts, in two rounds, 10.3 us); tiles of 16 rows
-  // leave room for two CTAs an SM (1 row: 4 parts 4.2 us, 8 parts 3.7 us)
+  // K parts: as many as still run at once (64 rows with one adapter, 1024 -> 3072: 4
+  // parts, 7.1 us; 8 parts, in two rounds, 14 us); tiles of 16 rows leave room
+  // for two CTAs an SM (1 row: 4 parts 5.4 us, 8 parts 5.2 us)
   int splits = 1;
   while (splits < 8 && 2 * splits <= a.num_kb &&
          2 * splits * tiles <= (a.xrows <= 16 ? 2 : 1) * lora_cluster_room(2 * splits, num_sms))
